@@ -52,8 +52,12 @@ LIBRARIES: Dict[str, str] = {
     "latent_attention": "latent_attention.cu",
     "latent_prefill": "latent_prefill.cu",
     "stream_ops": "stream_ops.cu",
+    "cache_e4m3": "cache_e4m3.cu",
+    "gemm_q4": "gemm_q4.cu",
 }
 HEADERS = ["common.cuh", "tc_common.cuh", "sampling_static.h"]
+# headers that only some libraries read
+OWN_HEADERS: Dict[str, List[str]] = {"cache_e4m3": ["e4m3.cuh"], "gemm_q4": ["q4.cuh"]}
 
 # host-only libraries (no CUDA): compiled with the host C++ compiler, so that the books of the
 # cache manager also load on a machine without nvcc or a GPU
@@ -86,7 +90,7 @@ def _cxx() -> Optional[str]:
 def _digest(name: str) -> str:
     h = hashlib.sha256()
     host = name in HOST_LIBRARIES
-    for rel in [LIBRARIES[name]] + ([] if host else HEADERS):
+    for rel in [LIBRARIES[name]] + ([] if host else HEADERS + OWN_HEADERS.get(name, [])):
         with open(os.path.join(HERE, rel), "rb") as f:
             h.update(rel.encode())
             h.update(f.read())

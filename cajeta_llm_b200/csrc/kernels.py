@@ -1692,3 +1692,281 @@ def wait_errors() -> Dict[str, int]:
             if code != 0:
                 found[name] = code
     return found
+
+
+# ---- the 8-bit cache ------------------------------------------------------------------------------------------------------
+
+def _need_e4m3_cache(k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor, page_tokens: int, n_kv: int,
+                     head_dim: int, what: str) -> None:
+    shape = (k_plane.shape[0], n_kv, page_tokens, head_dim)
+    for n, t in (("k_plane", k_plane), ("v_plane", v_plane)):
+        _need(t, n, torch.float8_e4m3fn)
+        if tuple(t.shape) != shape:
+            raise KernelError(f"{what}: {n} {tuple(t.shape)} is not [pages, {n_kv}, {page_tokens}, {head_dim}]")
+    for n, t in (("k_exp", k_exp), ("v_exp", v_exp)):
+        _need(t, n, torch.uint8)
+        if tuple(t.shape) != shape[:3]:
+            raise KernelError(f"{what}: {n} {tuple(t.shape)} is not [pages, {n_kv}, {page_tokens}]")
+
+
+def _need_same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels launch on the current device's current stream: every tensor lies there."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{here}")
+
+
+def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_out: torch.Tensor, k_plane: Optional[torch.Tensor],
+                       v_plane: Optional[torch.Tensor], k_exp: Optional[torch.Tensor], v_exp: Optional[torch.Tensor], positions: torch.Tensor,
+                       row_req: Optional[torch.Tensor], table: Optional[torch.Tensor], page_tokens: int, n_heads: int, n_kv: int, head_dim: int,
+                       rotary_dim: int, inv_freq: Optional[torch.Tensor], write_kv: bool) -> None:
+    """``rope_kv_write`` into the 8-bit cache: every (token, kv head) of keys and of values becomes ``head_dim`` e4m3 codes and one
+    exponent e (``k_exp`` and ``v_exp``, uint8 [pages, n_kv, page_tokens], hold e + 127), the smallest with max|x| <= 448 2^e;
+    an entry is its code times 2^e.  Zeros, and what lies below 448 2^-100, take e = -100; what lies beyond 448 2^119 is cut to it.
+    A row whose request (below 0) or page (-1) is not there is rotated and not written.  q_out: bfloat16 [T, heads, head_dim];
+    head_dim 64 or 128."""
+    _need(q_out, "q_out", torch.bfloat16), _need(positions, "positions", torch.int32)
+    if not qkv.is_cuda or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise KernelError("rope_kv_write_e4m3: qkv must be a float32 CUDA matrix whose rows are contiguous")
+    T = qkv.shape[0]
+    if tuple(q_out.shape) != (T, n_heads, head_dim) or positions.numel() != T:
+        raise KernelError(f"rope_kv_write_e4m3: q_out {tuple(q_out.shape)} and positions {tuple(positions.shape)} do not fit {T} rows")
+    ends = [q_off + n_heads * head_dim] + ([k_off + n_kv * head_dim, v_off + n_kv * head_dim] if write_kv else [])
+    if max(ends) > qkv.shape[1] or min(q_off, *(o for o in (k_off, v_off) if write_kv), 1 << 30) < 0:
+        raise KernelError(f"rope_kv_write_e4m3: the heads' columns do not lie within the {qkv.shape[1]} of qkv")
+    if rotary_dim > 0:
+        if inv_freq is None:
+            raise KernelError("rope_kv_write_e4m3: a rotation needs inv_freq")
+        _need(inv_freq, "inv_freq", torch.float32)
+        if inv_freq.numel() < rotary_dim // 2:
+            raise KernelError(f"rope_kv_write_e4m3: inv_freq holds {inv_freq.numel()} entries, the rotation needs {rotary_dim // 2}")
+    if write_kv:
+        _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, "rope_kv_write_e4m3")
+        _need(row_req, "row_req", torch.int32), _need(table, "table", torch.int32)
+        if row_req.numel() != T or table.dim() != 2:
+            raise KernelError("rope_kv_write_e4m3: row_req must name each row's request, table must be [requests, pages]")
+    _need_same_device("rope_kv_write_e4m3", qkv, q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
+    st = library("cache_e4m3").cj_append_e4m3(
+        _ptr(qkv), _i(qkv.stride(0)), _i(q_off), _i(k_off if write_kv else 0), _i(v_off if write_kv else 0), _ptr(q_out), _ptr(k_plane), _ptr(v_plane),
+        _ptr(k_exp), _ptr(v_exp), _ptr(positions), _ptr(row_req), _ptr(table), _i(table.stride(0) if table is not None else 0), _i(page_tokens), _i(T),
+        _i(n_heads), _i(n_kv), _i(head_dim), _i(rotary_dim), _ptr(inv_freq), _i(1 if write_kv else 0), _stream())
+    _check(st, "rope_kv_write_e4m3")
+
+
+def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, what) -> None:
+    _need(q, "q", torch.bfloat16), _need(out, "out", torch.bfloat16), _need(table, "table", torch.int32)
+    if head_dim not in (64, 128):
+        raise KernelError(f"{what} takes heads of 64 or 128, not {head_dim}")
+    if n_kv <= 0 or n_heads % n_kv != 0:
+        raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv} kv heads")
+    if tuple(q.shape[-2:]) != (n_heads, head_dim) or q.dim() != 3 or out.shape != q.shape:
+        raise KernelError(f"{what}: q {tuple(q.shape)} and out {tuple(out.shape)} are not [rows, {n_heads}, {head_dim}]")
+    if table.dim() != 2:
+        raise KernelError(f"{what}: table must be [requests, pages]")
+    _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, what)
+    _need_same_device(what, q, out, k_plane, v_plane, k_exp, v_exp, table)
+
+
+@functools.lru_cache(maxsize=4096)
+def e4m3_splits(rows: int, n_heads: int, n_kv: int, span: int, sms: int) -> int:
+    """Blocks that share a row's keys in ``decode_attention_e4m3``: as many as it takes to put three blocks on every SM, of at
+    least 128 keys (a step of each of a block's warps)."""
+    group = n_heads // n_kv
+    blocks = rows * n_kv * -(-group // (16 if group > 8 else 8))
+    return max(1, min(-(-3 * sms // blocks), -(-span // 128), 64))
+
+
+def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor,
+                          v_exp: torch.Tensor, positions: torch.Tensor, row_req: torch.Tensor, table: torch.Tensor, page_tokens: int,
+                          n_heads: int, n_kv: int, head_dim: int, window: int, scale: float, max_context: int, splits: int = 0) -> None:
+    """Attention of bfloat16 query rows [T, heads, head_dim], each over its request's keys in the 8-bit cache that
+    ``rope_kv_write_e4m3`` writes: row t sees the positions from ``positions[t] + 1 - window`` (0 without a window) to
+    ``positions[t]``.  A row whose request is below 0 sees none: zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
+    that share a row's keys (0: by the size of the launch; the results' last bits depend on it).  head_dim 64 or 128."""
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, "decode_attention_e4m3")
+    _need(positions, "positions", torch.int32), _need(row_req, "row_req", torch.int32)
+    T = q.shape[0]
+    if positions.numel() != T or row_req.numel() != T:
+        raise KernelError(f"decode_attention_e4m3: positions and row_req must hold one entry for each of {T} rows")
+    if T == 0:
+        return
+    splits = splits or e4m3_splits(T, n_heads, n_kv, min(window, max_context) if window > 0 else max(1, max_context), _sm_count())
+    acc = ml = None
+    if splits > 1:
+        acc = torch.empty((T, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
+        ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
+    st = library("cache_e4m3").cj_decode_e4m3(
+        _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(positions), _ptr(row_req),
+        _ptr(None), _ptr(None), _i(0), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(T), _i(n_heads), _i(n_kv), _i(head_dim), _i(window),
+        _f(scale), _i(splits), _ptr(acc), _ptr(ml), _stream())
+    _check(st, "decode_attention_e4m3")
+    if splits > 1:
+        global launches
+        launches += 1                      # the merge kernel
+
+
+def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor,
+                           v_exp: torch.Tensor, req_start: torch.Tensor, req_prior: torch.Tensor, table: torch.Tensor, page_tokens: int,
+                           n_heads: int, n_kv: int, head_dim: int, window: int, scale: float) -> None:
+    """Attention of portions of prompts over the 8-bit cache (which holds the portions' own keys and values already): rows
+    ``req_start[r]`` to ``req_start[r + 1]`` of q [T, heads, head_dim] (bfloat16) are request r's tokens from position
+    ``req_prior[r]`` on, each sees its request's keys up to its own position, under a window the last ``window`` of them.  Rows of no
+    request are left as they were.  head_dim 64 or 128."""
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, "prefill_attention_e4m3")
+    _need(req_start, "req_start", torch.int32), _need(req_prior, "req_prior", torch.int32)
+    R = req_prior.numel()
+    if req_start.numel() != R + 1 or table.shape[0] < R:
+        raise KernelError(f"prefill_attention_e4m3: req_start {tuple(req_start.shape)} and table {tuple(table.shape)} do not fit {R} requests")
+    T = q.shape[0]
+    if T == 0 or R == 0:
+        return
+    st = library("cache_e4m3").cj_decode_e4m3(
+        _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(None), _ptr(None),
+        _ptr(req_start), _ptr(req_prior), _i(R), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(T), _i(n_heads), _i(n_kv), _i(head_dim),
+        _i(window), _f(scale), _i(1), _ptr(None), _ptr(None), _stream())
+    _check(st, "prefill_attention_e4m3")
+
+
+# ---- 4-bit weights --------------------------------------------------------------------------------------------------------
+
+class Q4Weight:
+    """A weight [features, K], or [groups, features, K] of a mixture, in 4 bits: codes -8 .. 7 and a scale for each ``group`` of 32 or
+    64 neighbouring entries along K, laid out once for the products (:func:`gemm_q4`).  A scale has five significant bits, so that
+    code times scale is a bfloat16 number: products of few and of many rows see exactly the same weights.
+
+    ``quantise`` makes one from a float32 or bfloat16 weight, ``from_codes`` from codes and scales; both wait until it lies there."""
+
+    def __init__(self, data: torch.Tensor, shape, group: int, features: int = 0, groups: int = 0):
+        self.data = data                       # uint8, the layout
+        self.shape = tuple(shape)
+        self.group = group                     # 32 or 64
+        self.k = int(shape[-1])
+        self.features = int(shape[-2])
+        self.groups = int(shape[0]) if len(shape) == 3 else 1
+        self.dtype = torch.uint8
+        self.device = data.device
+
+    @staticmethod
+    def _fits(shape, group: int) -> None:
+        if len(shape) not in (2, 3) or min(shape) < 1:
+            raise KernelError(f"Q4Weight: a weight is [features, K] or [groups, features, K], found {tuple(shape)}")
+        if shape[-1] % 8 != 0:
+            raise KernelError(f"Q4Weight: K must be a multiple of 8, found {shape[-1]}")
+        if group != 32 and (group <= 0 or group % 64 != 0):
+            raise KernelError(f"Q4Weight: group must be 32 or a multiple of 64, found {group}")
+
+    @staticmethod
+    def _steady(what: str) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError(f"{what}: weights are laid out before a step is captured")
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, group: int = 64) -> "Q4Weight":
+        """``codes``: int8 [.., features, K] from -8 to 7; ``scales``: [.., features, ceil(K / group)], finite numbers of at most five
+        significant bits (float32 or bfloat16); group: 32 or a multiple of 64."""
+        cls._fits(codes.shape, group)
+        _need(codes, "codes", torch.int8)
+        cls._steady("Q4Weight.from_codes")
+        want = tuple(codes.shape[:-1]) + (-(-codes.shape[-1] // group),)
+        if tuple(scales.shape) != want or scales.dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"Q4Weight: scales must be float32 or bfloat16 {want}, found {scales.dtype} {tuple(scales.shape)}")
+        scales = scales.to(torch.float32).contiguous()
+        if int(codes.amin()) < -8 or int(codes.amax()) > 7:
+            raise KernelError("Q4Weight: codes lie between -8 and 7")
+        if not bool(((scales.view(torch.int32) & 0x7ffff) == 0).all()) or not bool(torch.isfinite(scales).all()):
+            raise KernelError("Q4Weight: scales must be finite and have at most five significant bits")
+        return cls._lay_out(codes, scales, group)
+
+    @classmethod
+    def quantise(cls, w: torch.Tensor, group: int = 64) -> "Q4Weight":
+        """The scale of a group is the smallest number of five significant bits that is at least max|w| / 7, a code w / scale rounded
+        to the nearest integer (of two, the even one)."""
+        return cls._lay_out(*cls.codes_of(w, group), group)
+
+    @classmethod
+    def codes_of(cls, w: torch.Tensor, group: int = 64):
+        """(codes, scales) that ``quantise`` lays out."""
+        cls._fits(w.shape, group)
+        _need(w, "w")
+        cls._steady("Q4Weight.quantise")
+        _need_same_device("Q4Weight.quantise", w)
+        K = w.shape[-1]
+        codes = torch.empty(w.shape, dtype=torch.int8, device=w.device)
+        scales = torch.empty(tuple(w.shape[:-1]) + (-(-K // group),), dtype=torch.float32, device=w.device)
+        st = library("gemm_q4").cj_q4_quantise(_ptr(w), _i(_code(w)), _ptr(codes), _ptr(scales), _ll(w.numel() // K), _i(K), _i(group), _stream())
+        _check(st, "Q4Weight.quantise")
+        return codes, scales
+
+    @classmethod
+    def _lay_out(cls, codes: torch.Tensor, scales: torch.Tensor, group: int) -> "Q4Weight":
+        _need_same_device("Q4Weight", codes, scales)
+        groups, (features, K) = (codes.shape[0] if codes.dim() == 3 else 1), codes.shape[-2:]
+        held = 32 if group == 32 else 64
+        size = library("gemm_q4").cj_q4_bytes
+        size.restype = ctypes.c_longlong
+        data = torch.empty((int(size(_i(groups), _i(features), _i(K), _i(1 if held == 32 else 0))),), dtype=torch.uint8, device=codes.device)
+        st = library("gemm_q4").cj_q4_layout(_ptr(codes), _ptr(scales), _ptr(data), _i(groups), _i(features), _i(K), _i(group), _stream())
+        _check(st, "Q4Weight")
+        # the products ask for their first codes before they wait for the kernels before them, and may run on any stream
+        torch.cuda.current_stream().synchronize()
+        return cls(data, codes.shape, held)
+
+    def first(self, n: int) -> "Q4Weight":
+        """The first ``n`` groups of a mixture's weights, or the first ``n`` features of a dense one, in the same memory."""
+        if not 1 <= n <= self.shape[0]:
+            raise KernelError(f"Q4Weight.first: {n} of {self.shape[0]}")
+        return self if n == self.shape[0] else Q4Weight(self.data, (n,) + self.shape[1:], self.group)
+
+    def numel(self) -> int:
+        return math.prod(self.shape)
+
+
+def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torch.Tensor] = None, accumulate: bool = False,
+            w_up: Optional[Q4Weight] = None, group_offsets: Optional[torch.Tensor] = None, a_row_index: Optional[torch.Tensor] = None) -> None:
+    """out[M, N] (+)= a[M, K] . w[N, K]^T (+ bias) for bfloat16 rows and 4-bit weights; products and sums in float32 of the weights'
+    exact values.  out: float32, or bfloat16 (rounded once; no ``accumulate``).  ``w_up``: out = silu(a w^T) (a w_up^T), no bias.
+    ``group_offsets`` (int32 [G + 1]) with a mixture's weights: output row s belongs to the group whose range holds s, and reads row
+    ``a_row_index[s]`` of ``a`` (zeros where that row is not there), or row s.  Rows of ``out`` outside all ranges are left alone.
+    K a multiple of 8; a's rows contiguous, their stride a multiple of four entries."""
+    if not isinstance(w, Q4Weight) or (w_up is not None and not isinstance(w_up, Q4Weight)):
+        raise KernelError("gemm_q4: w and w_up must be Q4Weight")
+    if not a.is_cuda or a.dtype != torch.bfloat16 or a.dim() != 2 or a.stride(1) != 1:
+        raise KernelError("gemm_q4: a must be a bfloat16 CUDA matrix whose rows are contiguous")
+    if not out.is_cuda or out.dim() != 2 or out.stride(1) != 1 or out.dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError("gemm_q4: out must be a float32 or bfloat16 CUDA matrix whose rows are contiguous")
+    M = out.shape[0]
+    if a.shape[1] != w.k or out.shape[1] != w.features:
+        raise KernelError(f"gemm_q4: shapes a {tuple(a.shape)} w {w.shape} out {tuple(out.shape)} do not agree")
+    if a_row_index is None and a.shape[0] != M:
+        raise KernelError(f"gemm_q4: {a.shape[0]} rows of a for {M} of out")
+    if accumulate and (out.dtype != torch.float32 or w_up is not None):
+        raise KernelError("gemm_q4: accumulate goes with a float32 result of one weight")
+    if w_up is not None and (w_up.shape != w.shape or w_up.group != w.group):
+        raise KernelError("gemm_q4: w_up must match w")
+    if bias is not None:
+        _need(bias, "bias", torch.float32)
+        if bias.numel() != w.features or w_up is not None:
+            raise KernelError(f"gemm_q4: bias must hold {w.features} entries and goes with one weight")
+    if (group_offsets is not None) != (len(w.shape) == 3):
+        raise KernelError("gemm_q4: group_offsets go with a mixture's weights [groups, features, K]")
+    if group_offsets is not None:
+        _need(group_offsets, "group_offsets", torch.int32)
+        if group_offsets.numel() != w.groups + 1:
+            raise KernelError("gemm_q4: group_offsets must hold one more entry than w has groups")
+    if a_row_index is not None:
+        _need(a_row_index, "a_row_index", torch.int32)
+        if a_row_index.numel() != M:
+            raise KernelError(f"gemm_q4: a_row_index must hold an entry for each of {M} rows")
+    _need_same_device("gemm_q4", a, w.data, out, bias, group_offsets, a_row_index)
+    if M == 0:
+        return
+    if a.shape[0] == 0:
+        raise KernelError("gemm_q4: a has no rows")
+    n_tok = 8 if M <= 8 or group_offsets is not None and M <= 4 * w.groups else 16 if M <= 16 else 32
+    pieces = 1 if n_tok == 8 else 2
+    st = library("gemm_q4").cj_gemm_q4(
+        _ptr(a), _ll(a.stride(0)), _i(a.shape[0]), _ptr(w.data), _ptr(w_up.data if w_up is not None else None), _ptr(bias), _ptr(out),
+        _i(_code(out)), _ll(out.stride(0)), _i(M), _i(w.features), _i(w.k), _i(w.groups), _i(1 if w.group == 32 else 0), _ptr(group_offsets),
+        _ptr(a_row_index), _i(1 if accumulate else 0), _i(n_tok), _i(pieces), _stream())
+    _check(st, "gemm_q4")
