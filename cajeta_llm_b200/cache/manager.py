@@ -81,6 +81,10 @@ class CacheManager:
         self.books = CacheBooks(specs, counts, page_tokens, max_seqs, max_tokens_per_seq)
         self.k: List[torch.Tensor] = []
         self.v: List[Optional[torch.Tensor]] = []      # None for a group that keeps no values
+        # an 8-bit cache's exponents + 127, one for each (token, kv head); empty for the other types
+        self.e4m3 = cache_dtype == torch.float8_e4m3fn
+        self.k_exp: List[torch.Tensor] = []
+        self.v_exp: List[Optional[torch.Tensor]] = []
         self.state: Dict[object, torch.Tensor] = {}      # by schedule entry (int) or by name (str)
         if self.device is not None:
             for spec, planes, pages in zip(specs, plane_count, counts):
@@ -88,6 +92,9 @@ class CacheManager:
                 self.k.append(torch.zeros(shape, dtype=cache_dtype, device=self.device))
                 v_shape = shape[:-1] + (spec.value_dim or spec.head_dim,)
                 self.v.append(torch.zeros(v_shape, dtype=cache_dtype, device=self.device) if spec.values else None)
+                if self.e4m3:
+                    self.k_exp.append(torch.zeros(shape[:-1], dtype=torch.uint8, device=self.device))
+                    self.v_exp.append(torch.zeros(shape[:-1], dtype=torch.uint8, device=self.device) if spec.values else None)
             for i, need in enumerate(state_needs):
                 if need is not None:
                     self.state[i] = torch.zeros((max_seqs,) + tuple(need.shape), dtype=need.dtype, device=self.device)
@@ -145,6 +152,14 @@ class CacheManager:
         p = self.entry_plane[entry]
         return self.k[g][p], (self.v[g][p] if self.v[g] is not None else None), g
 
+    def exponents(self, entry: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """The planes of exponents beside an entry's planes of codes (None where the cache has none)."""
+        g = self.entry_group[entry]
+        if g is None or not self.e4m3:
+            return None, None
+        p = self.entry_plane[entry]
+        return self.k_exp[g][p], (self.v_exp[g][p] if self.v_exp[g] is not None else None)
+
     def bytes_per_token(self) -> int:
         """Cache bytes one token occupies over all planes."""
         size = torch.empty((), dtype=self.cache_dtype).element_size()
@@ -153,6 +168,8 @@ class CacheManager:
             planes = sum(1 for e, gg in enumerate(self.entry_group) if gg == g and self.entry_plane[e] is not None
                          and self._owns(e))
             total += planes * spec.kv_heads * (spec.head_dim + ((spec.value_dim or spec.head_dim) if spec.values else 0)) * size
+            if self.e4m3:
+                total += planes * spec.kv_heads * (2 if spec.values else 1)
         return total
 
     def _owns(self, entry: int) -> bool:

@@ -14,7 +14,7 @@ spaces or commas, and the generated ids are printed, followed by
 ``[N tokens, budget | eos | stop | cancel]`` as the reference prints it
 (cli/Main.cajeta:83-122).  ``--prompt`` may be given several times; the prompts are then
 served together.  ``chat`` needs a chat template and a tokenizer and is not offered.
-Added flags: ``--dtype bfloat16|float32``, ``--max-batch-tokens N``, ``--num-blocks N``,
+Added flags: ``--dtype bfloat16|float32``, ``--cache-dtype float8_e4m3``, ``--weight-dtype int4``, ``--max-batch-tokens N``, ``--num-blocks N``,
 ``--no-warmup`` (skip the throw-away steps at load).
 
 A second verb writes a random-weights model folder from a configuration and a seed:
@@ -85,6 +85,10 @@ def parse_run(args: Sequence[str]):
             i = _need_val(args, i, a); o.chunk = int(args[i])
         elif a == "--dtype":
             i = _need_val(args, i, a); o.dtype = args[i]
+        elif a == "--cache-dtype":
+            i = _need_val(args, i, a); o.cache_dtype = args[i]
+        elif a == "--weight-dtype":
+            i = _need_val(args, i, a); o.weight_dtype = args[i]
         elif a == "--max-batch-tokens":
             i = _need_val(args, i, a); o.max_batch_tokens = int(args[i])
         elif a == "--num-blocks":

@@ -28,8 +28,8 @@ template <int HD>
 __global__ void __launch_bounds__(256) append_e4m3_kernel(
     const float* __restrict__ qkv, int ld, int q_off, int k_off, int v_off, __nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ kplane,
     uint8_t* __restrict__ vplane, uint8_t* __restrict__ kexp, uint8_t* __restrict__ vexp, const int* __restrict__ positions,
-    const int* __restrict__ row_req, const int* __restrict__ table, int table_stride, int page_tokens, int n_heads, int n_kv, int rot,
-    const float* __restrict__ inv_freq, int write_kv) {
+    const int* __restrict__ row_req, const int* __restrict__ table, int table_rows, int table_stride, int page_tokens, int n_pages,
+    int n_heads, int n_kv, int rot, const float* __restrict__ inv_freq, int write_kv) {
     constexpr int VEC = HD / 32;
     __shared__ float cs[HD / 2], sn[HD / 2];
     cj::after_predecessor();
@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
     long long base = -1;                    // row of (page, kv head 0, token) in the planes; -1: no page, nothing is written
     if (write_kv) {
         const int req = row_req[t], at = pos >= 0 ? pos / page_tokens : -1;
-        const int page = req >= 0 && at >= 0 && at < table_stride ? table[(size_t)req * table_stride + at] : -1;
-        if (page >= 0) base = (long long)page * n_kv * page_tokens + pos % page_tokens;
+        const int page = req >= 0 && req < table_rows && at >= 0 && at < table_stride ? table[(size_t)req * table_stride + at] : -1;
+        if (page >= 0 && page < n_pages) base = (long long)page * n_kv * page_tokens + pos % page_tokens;
     }
     __syncthreads();
     const int slots = n_heads + (base >= 0 ? 2 * n_kv : 0);
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : 3) decode_e4m3_ke
     const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const uint8_t* __restrict__ kplane, const uint8_t* __restrict__ vplane,
     const uint8_t* __restrict__ kexp, const uint8_t* __restrict__ vexp, const int* __restrict__ positions, const int* __restrict__ row_req,
     const int* __restrict__ req_start, const int* __restrict__ req_prior, int n_requests, const int* __restrict__ table, int table_stride,
-    int page_tokens, int n_heads, int n_kv, int head_batches, int window, float scale_log2, int splits, float* __restrict__ part_acc, float* __restrict__ part_ml) {
+    int page_tokens, int n_pages, int n_heads, int n_kv, int head_batches, int window, float scale_log2, int splits, float* __restrict__ part_acc, float* __restrict__ part_ml) {
     constexpr int NR = ROWS / 8;           // rows of a fragment a lane holds: g, and g + 8
     constexpr int QS = HD / 16;            // steps of 16 of the head's entries
     constexpr int KW = HD / 16;            // words of a key a lane holds
@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : 3) decode_e4m3_ke
     if (positions) {
         req = row_req[t];
         p = positions[t];
+        if (req >= n_requests) req = -1;
     } else {
         // portions: the request whose rows hold this one (none: the row is left alone)
         req = 0;
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : 3) decode_e4m3_ke
         int row = -1;
         if (key < last) {
             const int page = tab[key / page_tokens];
-            if (page >= 0) row = (page * n_kv + kvh) * page_tokens + key % page_tokens;
+            if (page >= 0 && page < n_pages) row = (page * n_kv + kvh) * page_tokens + key % page_tokens;
         }
         uint32_t kw[4][KW];
 #pragma unroll
@@ -408,10 +409,10 @@ __global__ void __launch_bounds__(128) decode_e4m3_merge_kernel(__nv_bfloat16* _
 
 // qkv: float32 [T, ld], columns from q_off, k_off, v_off (even, as ld); q_out: bf16 [T, n_heads, hd]; planes: e4m3 codes
 // [pages, n_kv, page_tokens, hd], exponents + 127 [pages, n_kv, page_tokens].  hd: 64 or 128; rotary_dim even, at most hd.
-// A row without a request or a page is rotated and not written.
+// A row without a request (of table_rows) or a page (of n_pages) is rotated and not written.
 CJ_EXPORT int cj_append_e4m3(const float* qkv, int ld, int q_off, int k_off, int v_off, void* q_out, void* kplane, void* vplane,
-                             void* kexp, void* vexp, const int* positions, const int* row_req, const int* table, int table_stride,
-                             int page_tokens, int T, int n_heads, int n_kv, int hd, int rotary_dim, const float* inv_freq, int write_kv,
+                             void* kexp, void* vexp, const int* positions, const int* row_req, const int* table, int table_rows, int table_stride,
+                             int page_tokens, int n_pages, int T, int n_heads, int n_kv, int hd, int rotary_dim, const float* inv_freq, int write_kv,
                              cudaStream_t stream) {
     if (T <= 0) return 0;
     if (!qkv || !q_out || !positions || n_heads <= 0) return CJ_ERR_ARG;
@@ -427,7 +428,7 @@ CJ_EXPORT int cj_append_e4m3(const float* qkv, int ld, int q_off, int k_off, int
     const dim3 grid(T, parts);
     auto kern = hd == 128 ? append_e4m3_kernel<128> : append_e4m3_kernel<64>;
     cj::launch(kern, dim3(grid), dim3(256), 0, stream, qkv, ld, q_off, k_off, v_off, (__nv_bfloat16*)q_out, (uint8_t*)kplane,
-               (uint8_t*)vplane, (uint8_t*)kexp, (uint8_t*)vexp, positions, row_req, table, table_stride, page_tokens, n_heads, n_kv,
+               (uint8_t*)vplane, (uint8_t*)kexp, (uint8_t*)vexp, positions, row_req, table, table_rows, table_stride, page_tokens, n_pages, n_heads, n_kv,
                rotary_dim, inv_freq, write_kv);
     return launch_status();
 }
@@ -435,15 +436,16 @@ CJ_EXPORT int cj_append_e4m3(const float* qkv, int ld, int q_off, int k_off, int
 // q, out: bf16 [T, n_heads, hd]; the cache as cj_append_e4m3 writes it.  splits > 1: every row's keys are dealt to that many
 // blocks; part_acc float32 [T, n_heads, splits, hd] and part_ml [T, n_heads, splits, 2] are scratch.  hd: 64 or 128.
 // positions null: the rows are portions of requests, req_start int32 [n_requests + 1], req_prior [n_requests] (one split).
+// table: int32 [n_requests, table_stride]; a row of no request sees no key, and a page of no number below n_pages holds none.
 CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const void* vplane, const void* kexp, const void* vexp,
                              int n_pages, const int* positions, const int* row_req, const int* req_start, const int* req_prior,
                              int n_requests, const int* table, int table_stride, int page_tokens, int T, int n_heads, int n_kv, int hd, int window, float scale, int splits, float* part_acc, float* part_ml,
                              cudaStream_t stream) {
     if (T <= 0) return 0;
     if (!q || !out || !kplane || !vplane || !kexp || !vexp || !table) return CJ_ERR_ARG;
-    if (positions ? !row_req : (!req_start || !req_prior || n_requests <= 0 || splits != 1)) return CJ_ERR_ARG;
+    if (positions ? !row_req : (!req_start || !req_prior || splits != 1)) return CJ_ERR_ARG;
     if (splits < 1 || (splits > 1 && (!part_acc || !part_ml))) return CJ_ERR_ARG;
-    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || window < 0) return CJ_ERR_SIZE;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || window < 0 || n_requests <= 0 || n_pages <= 0) return CJ_ERR_SIZE;
     if (hd != 64 && hd != 128) return CJ_ERR_SIZE;
     if (((uintptr_t)q | (uintptr_t)kplane | (uintptr_t)vplane) & 15) return CJ_ERR_ALIGN;
     if ((uintptr_t)out & 3) return CJ_ERR_ALIGN;
@@ -455,7 +457,7 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
                           : (rows == 8 ? decode_e4m3_kernel<64, 8> : decode_e4m3_kernel<64, 16>);
     cj::launch(kern, dim3(grid), dim3(WARPS * 32), 0, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane,
                (const uint8_t*)vplane, (const uint8_t*)kexp, (const uint8_t*)vexp, positions, row_req, req_start, req_prior, n_requests, table,
-               table_stride, page_tokens, n_heads, n_kv, head_batches, window, scale * 1.4426950408889634f, splits, part_acc, part_ml);
+               table_stride, page_tokens, n_pages, n_heads, n_kv, head_batches, window, scale * 1.4426950408889634f, splits, part_acc, part_ml);
     if (splits > 1) {
         const int status = launch_status();
         if (status != 0) return status;

@@ -1709,6 +1709,10 @@ def _need_e4m3_cache(k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.
             raise KernelError(f"{what}: {n} {tuple(t.shape)} is not [pages, {n_kv}, {page_tokens}]")
 
 
+def _on_device(t: torch.Tensor) -> bool:
+    return t.is_cuda
+
+
 def _need_same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The kernels launch on the current device's current stream: every tensor lies there."""
     here = torch.cuda.current_device()
@@ -1724,10 +1728,10 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     """``rope_kv_write`` into the 8-bit cache: every (token, kv head) of keys and of values becomes ``head_dim`` e4m3 codes and one
     exponent e (``k_exp`` and ``v_exp``, uint8 [pages, n_kv, page_tokens], hold e + 127), the smallest with max|x| <= 448 2^e;
     an entry is its code times 2^e.  Zeros, and what lies below 448 2^-100, take e = -100; what lies beyond 448 2^119 is cut to it.
-    A row whose request (below 0) or page (-1) is not there is rotated and not written.  q_out: bfloat16 [T, heads, head_dim];
+    A row whose request (none of ``table``'s) or page (-1) is not there is rotated and not written.  q_out: bfloat16 [T, heads, head_dim];
     head_dim 64 or 128."""
     _need(q_out, "q_out", torch.bfloat16), _need(positions, "positions", torch.int32)
-    if not qkv.is_cuda or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
+    if not _on_device(qkv) or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError("rope_kv_write_e4m3: qkv must be a float32 CUDA matrix whose rows are contiguous")
     T = qkv.shape[0]
     if tuple(q_out.shape) != (T, n_heads, head_dim) or positions.numel() != T:
@@ -1749,12 +1753,12 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     _need_same_device("rope_kv_write_e4m3", qkv, q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
     st = library("cache_e4m3").cj_append_e4m3(
         _ptr(qkv), _i(qkv.stride(0)), _i(q_off), _i(k_off if write_kv else 0), _i(v_off if write_kv else 0), _ptr(q_out), _ptr(k_plane), _ptr(v_plane),
-        _ptr(k_exp), _ptr(v_exp), _ptr(positions), _ptr(row_req), _ptr(table), _i(table.stride(0) if table is not None else 0), _i(page_tokens), _i(T),
-        _i(n_heads), _i(n_kv), _i(head_dim), _i(rotary_dim), _ptr(inv_freq), _i(1 if write_kv else 0), _stream())
+        _ptr(k_exp), _ptr(v_exp), _ptr(positions), _ptr(row_req), _ptr(table), _i(table.shape[0] if write_kv else 0), _i(table.stride(0) if write_kv else 0),
+        _i(page_tokens), _i(k_plane.shape[0] if write_kv else 0), _i(T), _i(n_heads), _i(n_kv), _i(head_dim), _i(rotary_dim), _ptr(inv_freq), _i(1 if write_kv else 0), _stream())
     _check(st, "rope_kv_write_e4m3")
 
 
-def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, what) -> None:
+def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, what) -> None:
     _need(q, "q", torch.bfloat16), _need(out, "out", torch.bfloat16), _need(table, "table", torch.int32)
     if head_dim not in (64, 128):
         raise KernelError(f"{what} takes heads of 64 or 128, not {head_dim}")
@@ -1764,6 +1768,8 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tok
         raise KernelError(f"{what}: q {tuple(q.shape)} and out {tuple(out.shape)} are not [rows, {n_heads}, {head_dim}]")
     if table.dim() != 2:
         raise KernelError(f"{what}: table must be [requests, pages]")
+    if window < 0:
+        raise KernelError(f"{what}: window must be positive (or 0 for none), found {window}")
     _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, what)
     _need_same_device(what, q, out, k_plane, v_plane, k_exp, v_exp, table)
 
@@ -1782,13 +1788,15 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
                           n_heads: int, n_kv: int, head_dim: int, window: int, scale: float, max_context: int, splits: int = 0) -> None:
     """Attention of bfloat16 query rows [T, heads, head_dim], each over its request's keys in the 8-bit cache that
     ``rope_kv_write_e4m3`` writes: row t sees the positions from ``positions[t] + 1 - window`` (0 without a window) to
-    ``positions[t]``.  A row whose request is below 0 sees none: zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
+    ``positions[t]``.  A row of none of ``table``'s requests (-1) sees none: zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
     that share a row's keys (0: by the size of the launch; the results' last bits depend on it).  head_dim 64 or 128."""
-    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, "decode_attention_e4m3")
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, "decode_attention_e4m3")
     _need(positions, "positions", torch.int32), _need(row_req, "row_req", torch.int32)
     T = q.shape[0]
     if positions.numel() != T or row_req.numel() != T:
         raise KernelError(f"decode_attention_e4m3: positions and row_req must hold one entry for each of {T} rows")
+    if not 0 <= splits <= 65535:
+        raise KernelError(f"decode_attention_e4m3: splits must lie between 0 and 65535, found {splits}")
     if T == 0:
         return
     splits = splits or e4m3_splits(T, n_heads, n_kv, min(window, max_context) if window > 0 else max(1, max_context), _sm_count())
@@ -1798,7 +1806,7 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
         ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
     st = library("cache_e4m3").cj_decode_e4m3(
         _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(positions), _ptr(row_req),
-        _ptr(None), _ptr(None), _i(0), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(T), _i(n_heads), _i(n_kv), _i(head_dim), _i(window),
+        _ptr(None), _ptr(None), _i(table.shape[0]), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(T), _i(n_heads), _i(n_kv), _i(head_dim), _i(window),
         _f(scale), _i(splits), _ptr(acc), _ptr(ml), _stream())
     _check(st, "decode_attention_e4m3")
     if splits > 1:
@@ -1813,7 +1821,7 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     ``req_start[r]`` to ``req_start[r + 1]`` of q [T, heads, head_dim] (bfloat16) are request r's tokens from position
     ``req_prior[r]`` on, each sees its request's keys up to its own position, under a window the last ``window`` of them.  Rows of no
     request are left as they were.  head_dim 64 or 128."""
-    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, "prefill_attention_e4m3")
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, "prefill_attention_e4m3")
     _need(req_start, "req_start", torch.int32), _need(req_prior, "req_prior", torch.int32)
     R = req_prior.numel()
     if req_start.numel() != R + 1 or table.shape[0] < R:
@@ -1931,9 +1939,9 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
     K a multiple of 8; a's rows contiguous, their stride a multiple of four entries."""
     if not isinstance(w, Q4Weight) or (w_up is not None and not isinstance(w_up, Q4Weight)):
         raise KernelError("gemm_q4: w and w_up must be Q4Weight")
-    if not a.is_cuda or a.dtype != torch.bfloat16 or a.dim() != 2 or a.stride(1) != 1:
+    if not _on_device(a) or a.dtype != torch.bfloat16 or a.dim() != 2 or a.stride(1) != 1:
         raise KernelError("gemm_q4: a must be a bfloat16 CUDA matrix whose rows are contiguous")
-    if not out.is_cuda or out.dim() != 2 or out.stride(1) != 1 or out.dtype not in (torch.float32, torch.bfloat16):
+    if not _on_device(out) or out.dim() != 2 or out.stride(1) != 1 or out.dtype not in (torch.float32, torch.bfloat16):
         raise KernelError("gemm_q4: out must be a float32 or bfloat16 CUDA matrix whose rows are contiguous")
     M = out.shape[0]
     if a.shape[1] != w.k or out.shape[1] != w.features:

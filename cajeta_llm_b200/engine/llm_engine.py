@@ -87,7 +87,8 @@ class LlmEngine:
         options.validate()
         if not torch.cuda.is_available():
             raise RuntimeError("no CUDA device: this engine runs on a B200 and has no CPU path")
-        runtime = Runtime(dtype=options.dtype, device=options.device)
+        runtime = Runtime(dtype=options.dtype, device=options.device, cache_dtype=options.cache_dtype,
+                          weight_dtype=options.weight_dtype)
         eog: List[int] = []
         if options.random_weights or not options.model:
             config = options.config

@@ -37,6 +37,21 @@ class Model:
         self.head_part = make_part("head", plan.head, "", runtime, vocab_size=self.vocab, hidden_size=self.hidden,
                                    weight_name=plan.lm_head_name, embedding=self.embedding_part)
 
+        self._check_held(runtime)
+
+    def _check_held(self, runtime: Runtime) -> None:
+        for block in self.blocks if runtime.e4m3_cache or runtime.q4_weights else ():
+            for name in ("mixer", "feed_forward"):
+                part = getattr(block, name, None)
+                if part is None:
+                    continue
+                kind = getattr(getattr(part, "spec", None), "kind", type(part).__name__)
+                what = f"the {name.replace('_', '-')} '{kind}' of '{block.prefix}' with its parameters"
+                if runtime.e4m3_cache and name == "mixer" and part.cache_need() is not None and not part.takes_e4m3_cache:
+                    raise ValueError(f"an 8-bit cache is not built into {what}")
+                if runtime.q4_weights and not part.takes_q4_weights:
+                    raise ValueError(f"4-bit weights are not built into {what}")
+
     def parts(self):
         return ([self.embedding_part] + list(self.blocks) + [b for b in self.before if b is not None]
                 + [self.final_norm, self.head_part])
@@ -120,6 +135,8 @@ class Model:
             for v in vars(p).values():
                 if isinstance(v, torch.Tensor):
                     yield v
+                elif isinstance(getattr(v, "data", None), torch.Tensor):      # a 4-bit weight
+                    yield v.data
                 elif hasattr(v, "params") and hasattr(v, "runtime") and v is not getattr(p, "embedding", None):
                     stack.append(v)
 

@@ -5,7 +5,8 @@ EngineOptions.cajeta:98-122: ``ctx`` 4096 (most tokens one request may hold),
 ``--block-size``), ``chunk`` 0 (0 = portions are cut by the token budget alone, N pins
 the largest portion), ``device``.  This engine adds ``dtype`` (``bfloat16`` serving
 path or the true ``float32`` path), ``max_batch_tokens`` (token budget of one mixed
-step), ``num_blocks`` (cache pages per layer group; 0 = enough for ``max_seqs``
+step), ``cache_dtype`` and ``weight_dtype`` (keys and values cached in 8 bits, matrices held
+in 4), ``num_blocks`` (cache pages per layer group; 0 = enough for ``max_seqs``
 requests of ``ctx`` tokens), the random-weights mode (``random_weights``, ``seed``) and
 ``warmup`` (the reference always warms at load with one throw-away prefill and decode step,
 LlmEngine.cajeta:294-324; here it can be switched off).
@@ -26,6 +27,8 @@ class EngineOptions:
     chunk: int = 0
     device: str = "cuda:0"
     dtype: str = "bfloat16"
+    cache_dtype: str = ""              # "" = dtype; "float8_e4m3": 8-bit keys and values, a power of two for each (token, kv head)
+    weight_dtype: str = ""             # "" = dtype; "int4": the layers' matrices in 4 bits, a scale for each 64 entries along K
     max_batch_tokens: int = 2048
     num_blocks: int = 0
     random_weights: bool = False       # draw the weights from ``seed`` instead of reading them
@@ -47,5 +50,10 @@ class EngineOptions:
             raise ValueError(f"chunk must be >= 0, found {self.chunk}")
         if self.dtype not in ("bfloat16", "float32"):
             raise ValueError(f"dtype must be bfloat16 or float32, found '{self.dtype}'")
+        if self.cache_dtype not in ("", "float8_e4m3") or self.weight_dtype not in ("", "int4"):
+            raise ValueError(f"cache_dtype must be float8_e4m3 (or '' for dtype) and weight_dtype int4 (or ''), found '{self.cache_dtype}' "
+                             f"and '{self.weight_dtype}'")
+        if (self.cache_dtype or self.weight_dtype) and self.dtype != "bfloat16":
+            raise ValueError("an 8-bit cache and 4-bit weights go with dtype bfloat16")
         if not self.model and self.config is None:
             raise ValueError("either a model folder or a configuration is required")

@@ -75,6 +75,8 @@ class EntryContext:
     block_table: Optional[torch.Tensor]      # int32 [requests, width] of the entry's group
     page_tokens: int
     state: Optional[torch.Tensor]            # [max_seqs, ...] per-request state of this entry
+    k_exp: Optional[torch.Tensor] = None     # an 8-bit cache's exponents beside its planes
+    v_exp: Optional[torch.Tensor] = None
     state_offset: int = 0                    # where, in a request's flat state vector, the part being run finds its share
 
 
@@ -313,7 +315,8 @@ class ModelRunner:
             if self.model.before[i] is not None:
                 self.model.before[i].forward(hs, ctx)
             k_plane, v_plane, group = self.cache.plane(i)
-            ectx = EntryContext(index=i, writes_cache=e.cache_from is None, k_plane=k_plane, v_plane=v_plane,
+            k_exp, v_exp = self.cache.exponents(i)
+            ectx = EntryContext(index=i, k_exp=k_exp, v_exp=v_exp, writes_cache=e.cache_from is None, k_plane=k_plane, v_plane=v_plane,
                                 block_table=ctx.tables[group] if group is not None else None,
                                 page_tokens=self.page_tokens, state=self.cache.state.get(i))
             self.model.blocks[e.layer].forward(hs, ctx, ectx)

@@ -63,7 +63,7 @@ import torch
 
 from ..csrc import kernels as K
 from .base import KvNeed, Part, make_part, register_part
-from .linear import project, project_split, splits_few_rows
+from .linear import first_rows, project, project_split, splits_few_rows
 from .plan import ParamSpec
 
 
@@ -117,6 +117,9 @@ class PagedAttention(Part):
         self.norm_whole = bool(self.qk_norm and self.qk_norm.get("whole"))
         self.mixed = bool(self.proj_conv or self.head_temp or self.talk or self.sink or self.norm_whole)
         self.general = self.general or self.mixed
+        # an 8-bit cache and 4-bit weights are built for the plain path (no optional parameter)
+        self.takes_q4_weights = not self.general and self.hidden % 8 == 0 and self.q_dim % 8 == 0
+        self.takes_e4m3_cache = not self.general and self.head_dim in (64, 128)
         if self.general and (self.qkv_bias or self.out_bias):
             raise ValueError("the general attention path is built without biases")
         if self.mixed and (self.softcap > 0.0 or self.head_gate or self.values_from_keys):
@@ -199,6 +202,10 @@ class PagedAttention(Part):
             libs |= {"attention_decode", "attention_prefill_tc" if self.head_dim == 128 else "attention_prefill"}
         else:
             libs.add("attention_paged")
+        if self.runtime.e4m3_cache:
+            libs.add("cache_e4m3")
+        if self.runtime.q4_weights:
+            libs.add("gemm_q4")
         if "attention_paged" in libs and self.runtime.act_dtype == torch.float32:
             libs.add("attention_f32")
         if self.runtime.fast_kernels and self.hidden >= 128:
@@ -210,7 +217,7 @@ class PagedAttention(Part):
         rows = [self.fetch(source, self.n_proj[n]) for n in (("q", "k") if self.values_from_keys else ("q", "k", "v"))]
         if self.head_gate:
             rows.append(self.fetch(source, self.name(self.head_gate)))      # the gate's rows ride along: one product
-        self.w_qkv = torch.cat(rows, dim=0).contiguous()
+        self.w_qkv = self.runtime.held(torch.cat(rows, dim=0).contiguous())
         if self.qk_norm and not self.unit_qk:
             self.q_norm_w = self.fetch(source, self.name(self.qk_norm["q"]))
             self.k_norm_w = self.fetch(source, self.name(self.qk_norm["k"]))
@@ -221,7 +228,7 @@ class PagedAttention(Part):
                 setattr(self, attr, self.fetch(source, self.name(n)))
         if self.qkv_bias:
             self.b_qkv = torch.cat([self.fetch(source, self.name(f"{n}_proj.bias")) for n in ("q", "k", "v")], dim=0).contiguous()
-        self.w_o = self.fetch(source, self.n_proj["o"])
+        self.w_o = self.runtime.held(self.fetch(source, self.n_proj["o"]))
         if self.out_bias:
             self.b_o = self.fetch(source, self.name("o_proj.bias"))
 
@@ -241,9 +248,11 @@ class PagedAttention(Part):
         n_out = self.q_dim + (2 * self.kv_dim if write else 0)
         qkv = torch.empty((T, n_out), dtype=torch.float32, device=x.device)
         K.tag = "qkv"
-        project(rt, x, self.w_qkv[:n_out], qkv, bias=None if self.b_qkv is None else self.b_qkv[:n_out])
+        project(rt, x, first_rows(self.w_qkv, n_out), qkv, bias=None if self.b_qkv is None else self.b_qkv[:n_out])
         q = torch.empty((T, self.heads, self.head_dim), dtype=rt.act_dtype, device=x.device)
         K.tag = "rope + cache write"
+        if rt.e4m3_cache:
+            return self._project_out(self._attend_e4m3(qkv, q, write, ctx, entry), residual)
         K.rope_kv_write(qkv, 0, self.q_dim, self.q_dim + self.kv_dim, q, entry.k_plane, entry.v_plane,
                         ctx.positions, ctx.row_req, entry.block_table, entry.page_tokens, self.heads, self.kv_heads,
                         self.head_dim, pos.rotary_dim, pos.inv_freq, write)
@@ -267,12 +276,35 @@ class PagedAttention(Part):
             K.paged_attention(q, out, entry.k_plane, entry.v_plane, ctx.positions, ctx.row_req, entry.block_table,
                               entry.page_tokens, self.heads, self.kv_heads, self.head_dim, self.window, self.scale,
                               req_start=getattr(ctx, "req_start", None), h_req_start=getattr(ctx, "h_req_start", None))
+        return self._project_out(out, residual)
+
+    def _project_out(self, out: torch.Tensor, residual: torch.Tensor) -> Optional[torch.Tensor]:
+        """The output projection, added to the residual stream; or its partial sums, owed to it (the next norm adds them)."""
+        rt = self.runtime
+        out = out.view(out.shape[0], self.q_dim)
         K.tag = "o"
-        parts = project_split(rt, out.view(T, self.q_dim), self.w_o, bias=self.b_o, out_scale=self.out_scale) if self.allow_pending else None
+        parts = project_split(rt, out, self.w_o, bias=self.b_o, out_scale=self.out_scale) if self.allow_pending else None
         if parts is None:
-            project(rt, out.view(T, self.q_dim), self.w_o, residual, bias=self.b_o, accumulate=True, out_scale=self.out_scale)
+            project(rt, out, self.w_o, residual, bias=self.b_o, accumulate=True, out_scale=self.out_scale)
         K.tag = None
-        return parts                         # partial sums owed to the residual stream (the next norm adds them), or None
+        return parts
+
+    def _attend_e4m3(self, qkv: torch.Tensor, q: torch.Tensor, write: bool, ctx, entry) -> torch.Tensor:
+        """Rotation, cache write and attention over the 8-bit cache."""
+        pos = self.position
+        K.rope_kv_write_e4m3(qkv, 0, self.q_dim, self.q_dim + self.kv_dim, q, entry.k_plane, entry.v_plane, entry.k_exp, entry.v_exp,
+                             ctx.positions, ctx.row_req, entry.block_table, entry.page_tokens, self.heads, self.kv_heads, self.head_dim,
+                             pos.rotary_dim, pos.inv_freq, write)
+        out = torch.empty_like(q)
+        K.tag = "attention"
+        if getattr(ctx, "all_single", False):
+            K.decode_attention_e4m3(q, out, entry.k_plane, entry.v_plane, entry.k_exp, entry.v_exp, ctx.positions, ctx.row_req,
+                                    entry.block_table, entry.page_tokens, self.heads, self.kv_heads, self.head_dim, self.window, self.scale,
+                                    ctx.max_context)
+        else:
+            K.prefill_attention_e4m3(q, out, entry.k_plane, entry.v_plane, entry.k_exp, entry.v_exp, ctx.req_start, ctx.req_prior,
+                                     entry.block_table, entry.page_tokens, self.heads, self.kv_heads, self.head_dim, self.window, self.scale)
+        return out
 
     def _forward_general(self, x: torch.Tensor, residual: torch.Tensor, ctx, entry) -> Optional[torch.Tensor]:
         """The path of a mixer with any of the optional parameters: one product for q | k | (v) | (gate), heads made

@@ -45,15 +45,26 @@ class Runtime:
     float32's accuracy (on the FMA pipe, or on the tensor cores with each operand as the sum
     of three bfloat16 parts and the parts' products down to 2^-24 of the operands'; no
     reduced-precision matrix mode).
+
+    On the bfloat16 path ``cache_dtype`` ``"float8_e4m3"`` keeps keys and values in 8 bits (``e4m3_cache``) and
+    ``weight_dtype`` ``"int4"`` the matrices of mixers and feed-forwards in 4 (``q4_weights``), for the parts that say they
+    take them (``takes_e4m3_cache``, ``takes_q4_weights``); a model with another part refuses them.
     """
 
-    def __init__(self, dtype: str = "bfloat16", device: str = "cuda:0", fast_kernels: bool = True):
+    def __init__(self, dtype: str = "bfloat16", device: str = "cuda:0", fast_kernels: bool = True, cache_dtype: str = "",
+                 weight_dtype: str = ""):
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}, found '{dtype}'")
         self.dtype_name = dtype
         self.act_dtype = DTYPES[dtype]
         self.matrix_dtype = DTYPES[dtype]
-        self.cache_dtype = DTYPES[dtype]
+        if cache_dtype not in ("", "float8_e4m3") or weight_dtype not in ("", "int4"):
+            raise ValueError(f"cache_dtype must be float8_e4m3 and weight_dtype int4 (or '' for dtype), found '{cache_dtype}' and '{weight_dtype}'")
+        if (cache_dtype or weight_dtype) and (dtype != "bfloat16" or not fast_kernels):
+            raise ValueError("an 8-bit cache and 4-bit weights are built for the bfloat16 path")
+        self.e4m3_cache = cache_dtype == "float8_e4m3"
+        self.q4_weights = weight_dtype == "int4"
+        self.cache_dtype = torch.float8_e4m3fn if self.e4m3_cache else DTYPES[dtype]
         self.device = torch.device(device)
         self.fast_kernels = fast_kernels and dtype == "bfloat16"
         self._decode_scratch = None
@@ -79,6 +90,13 @@ class Runtime:
 
     def matrix(self, t: torch.Tensor) -> torch.Tensor:
         return t.to(device=self.device, dtype=self.matrix_dtype).contiguous()
+
+    def held(self, t: torch.Tensor):
+        """A matrix of a mixer or a feed-forward as the products read it: itself, or in 4 bits."""
+        if not self.q4_weights:
+            return t
+        from ..csrc.kernels import Q4Weight
+        return Q4Weight.quantise(t)
 
     def vector(self, t: torch.Tensor) -> torch.Tensor:
         return t.to(device=self.device, dtype=torch.float32).contiguous()
@@ -123,6 +141,8 @@ class StateNeed:
 
 class Part:
     category = ""
+    takes_e4m3_cache = False           # a mixer: writes and reads an 8-bit cache when the runtime asks for one
+    takes_q4_weights = False           # a mixer or a feed-forward: holds its matrices in 4 bits when the runtime asks for them
 
     def __init__(self, spec: PartSpec, prefix: str, runtime: Runtime):
         self.spec = spec

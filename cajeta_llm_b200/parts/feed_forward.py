@@ -61,7 +61,7 @@ import torch
 
 from ..csrc import kernels as K
 from .base import Part, register_part
-from .linear import project, project_split, splits_few_rows
+from .linear import first_rows, project, project_split, splits_few_rows
 from .plan import ParamSpec
 
 
@@ -86,6 +86,7 @@ class DenseSwiGLU(Part):
         if activation not in GATES:
             raise ValueError(f"activation must be one of {', '.join(sorted(GATES))}, found '{activation}'")
         self.gate_alpha, self.gate_cubic = GATES[activation]
+        self.takes_q4_weights = activation == "silu" and not self.bias and self.hidden % 8 == 0 and self.inter % 8 == 0
         self.w_gate = self.w_up = self.w_down = None
         self.b_gate = self.b_up = self.b_down = None
 
@@ -102,15 +103,13 @@ class DenseSwiGLU(Part):
         return p
 
     def libraries(self) -> set:
-        libs = {"gemm_simt"}
+        libs = {"gemm_simt"} | ({"gemm_q4"} if self.runtime.q4_weights else set())
         if self.runtime.fast_kernels and self.hidden >= 128:
             libs |= {"gemm_tc", "gemm_tc2"}
         return libs
 
     def load(self, source) -> None:
-        self.w_gate = self.fetch(source, self.n_gate)
-        self.w_up = self.fetch(source, self.n_up)
-        self.w_down = self.fetch(source, self.n_down)
+        self.w_gate, self.w_up, self.w_down = (self.runtime.held(self.fetch(source, n)) for n in (self.n_gate, self.n_up, self.n_down))
         if self.bias:
             self.b_gate, self.b_up, self.b_down = (self.fetch(source, n + ".b") for n in (self.n_gate, self.n_up, self.n_down))
 
@@ -232,6 +231,9 @@ class SparseMoE(Part):
             raise ValueError(f"top_k must be between 1 and num_experts ({self.num_experts}), found {self.top_k}")
         if self.num_experts > 1024:
             raise ValueError(f"num_experts {self.num_experts} is more than the router kernel takes (1024)")
+        self.takes_q4_weights = (self.gated and self.act_limit == 0.0 and self.act_alpha == 1.0 and self.shared_act_limit == 0.0
+                                 and self.shared_act_alpha == 1.0 and self.weight_on == "output" and self.hidden % 8 == 0
+                                 and self.inter % 8 == 0 and self.shared_inter % 8 == 0)
         self.router = None
         self.w_gate = self.w_up = self.w_down = None
         self.ws_gate = self.ws_up = self.ws_down = None
@@ -265,7 +267,7 @@ class SparseMoE(Part):
         return self.name(self.n_expert[proj].format(e=e))
 
     def libraries(self) -> set:
-        libs = {"rowwise", "moe_route", "gemm_simt"} | ({"recurrent"} if self.weight_on == "input" else set())
+        libs = {"rowwise", "moe_route", "gemm_simt"} | ({"gemm_q4"} if self.runtime.q4_weights else set()) | ({"recurrent"} if self.weight_on == "input" else set())
         if self.runtime.fast_kernels and self.hidden >= 128:
             libs |= {"gemm_tc", "gemm_tc2"}
         return libs
@@ -297,7 +299,7 @@ class SparseMoE(Part):
                     self.w_gate[E:].copy_(ws_gate.view(C, I, self.hidden))
                 self.w_up[E:].copy_(ws_up.view(C, I, self.hidden))
                 self.w_down[E:].copy_(ws_down.view(self.hidden, C, I).permute(1, 0, 2))
-                if rt.fast_kernels:
+                if rt.fast_kernels and not rt.q4_weights:
                     # steps with many rows run the shared expert as dense products of its own (see
                     # forward): gate and up are then the chunks' rows seen as one matrix, the down
                     # projection is held a second time, whole
@@ -307,6 +309,10 @@ class SparseMoE(Part):
             if self.shared_gate:
                 self.shared_gate_w = self.fetch(source, self.n_shared_sg).reshape(-1).contiguous()
 
+        # (in 4 bits the shared expert's chunks stay groups of the products whatever the step's rows: one copy, one set of scales)
+        for n in ("w_gate", "w_up", "w_down", "ws_gate", "ws_up", "ws_down") if rt.q4_weights else ():
+            if getattr(self, n) is not None:
+                setattr(self, n, rt.held(getattr(self, n)))
         self._prepare_split_router()
 
     # Router logits on the tensor cores, float32-grade.  The normed row arrives as three
@@ -422,11 +428,11 @@ class SparseMoE(Part):
             project(rt, x, self.w_up[:G], act, group_offsets=offsets, a_row_index=slot_token, max_group_rows=T, act=self.activation)
         else:
             K.tag = "experts gate/up"
-            project(rt, x, self.w_gate[:G], act, w_up=self.w_up[:G], group_offsets=offsets, a_row_index=slot_token,
+            project(rt, x, first_rows(self.w_gate, G), act, w_up=first_rows(self.w_up, G), group_offsets=offsets, a_row_index=slot_token,
                     max_group_rows=T, act_limit=self.act_limit, act_alpha=self.act_alpha)
         y = torch.empty((n_slots, self.hidden), dtype=torch.float32, device=dev)
         K.tag = "experts down"
-        project(rt, act, self.w_down[:G], y, group_offsets=offsets, max_group_rows=T, offsets_settled=True)
+        project(rt, act, first_rows(self.w_down, G), y, group_offsets=offsets, max_group_rows=T, offsets_settled=True)
 
         shared = None
         if C > 0:

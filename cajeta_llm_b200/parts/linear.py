@@ -6,7 +6,7 @@ mixture of experts.  On the bfloat16 path it runs on the tensor cores (tcgen05 /
 when the shapes allow TMA (K a multiple of 8, 16-byte aligned rows) and are large
 enough to fill a tile; otherwise, and always on the float32 path, it runs through
 ``K.gemm`` (the FMA pipe, or three bfloat16 parts an operand on the tensor cores), whose
-results do not depend on the batch at all.  Few rows (decode) put the
+results do not depend on the batch at all.  A weight held in 4 bits (``K.Q4Weight``) goes to ``K.gemm_q4``.  Few rows (decode) put the
 weights on the rows of the tensor-core product, many rows (prompt portions) the tokens.
 """
 from __future__ import annotations
@@ -77,6 +77,11 @@ def _pair_tile(runtime, rows: int, w: torch.Tensor, swiglu: bool, grouped: bool)
     return 256 if feature_tiles * -(-rows // 256) >= runtime.sm_count // 2 else 128
 
 
+def first_rows(w, n: int):
+    """The first ``n`` features of a dense weight, or groups of a mixture's, whichever way it is held."""
+    return w.first(n) if isinstance(w, K.Q4Weight) else w[:n]
+
+
 def project(runtime, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
             accumulate: bool = False, w_up: Optional[torch.Tensor] = None, group_offsets: Optional[torch.Tensor] = None,
             a_row_index: Optional[torch.Tensor] = None, max_group_rows: Optional[int] = None,
@@ -100,6 +105,12 @@ def project(runtime, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, *, bia
         raise ValueError("project: out_scale goes with a float32 result of one weight")
     if act and (w_up is not None or out.dtype != runtime.act_dtype):
         raise ValueError("project: act goes with one weight and a result in the activation dtype")
+    if isinstance(w, K.Q4Weight):
+        gate_other = w_up is not None and (act_alpha != 1.0 or act_cubic != 0.0 or bias is not None or bias_up is not None)
+        if act or act_limit != 0.0 or out_scale != 1.0 or gate_other:
+            raise ValueError("project: 4-bit weights go with a plain product (and a bias) or with silu(gate) * up")
+        K.gemm_q4(x, w, out, bias=bias, accumulate=accumulate, w_up=w_up, group_offsets=group_offsets, a_row_index=a_row_index)
+        return
     if not _tc_ok(runtime, x, w):
         K.gemm(x, w, out, bias=bias, accumulate=accumulate, w_up=w_up, group_offsets=group_offsets, a_row_index=a_row_index,
                act_limit=act_limit, act_alpha=act_alpha, out_scale=out_scale, act_cubic=act_cubic, bias_up=bias_up, act=act,
