@@ -1,0 +1,384 @@
+// Products with 4-bit weights for many rows, on the 5th-generation tensor cores (tcgen05):
+//
+//     out[t, f] (+)= sum_k (s q)[f, k] x[t, k]   (+ bias[f]; or silu of it times a second product)
+//
+// with the weights and their layout of gemm_q4.cu.  A code times its scale is a bfloat16 number, so the weights are turned into
+// bfloat16 on their way and the product is that of the unpacked weights to the bit.  They are the product's 128 rows and are read from
+// tensor memory: eight warps take a tile of 128 features x 64 of K out of shared memory, each a piece of 16 features (a 16-byte load a
+// lane), and put it there with one 16x256b store, whose lanes hold what the layout gave them; nothing is written back to shared
+// memory, whose bandwidth the other operand needs.  The rows of x are the product's columns, up to 256 of them, so that the codes'
+// conversion (140 issue slots a scheduler and tile of 128 x 64) hides behind the product (256 clocks for 128 rows, 512 for 256).
+//
+// Persistent blocks, one an SM: two warps load (x by TMA, the codes of a tile by one bulk copy), one thread issues the products, four
+// warps drain an accumulator while the next fills where tensor memory has room for two.  The gated form puts 16 features of the gate and 16
+// of the other weight on each warp's 32 lanes, so that their sums meet by a shuffle.  Bound by the tensor core for many rows; for a
+// mixture whose groups have a few dozen rows by the weights' bytes and by the groups' last, part-filled tiles.
+#define CJ_LIB "gemm_q4_tc"
+#include "common.cuh"
+#include "q4.cuh"
+#include "tc_common.cuh"
+
+using namespace tc;
+
+namespace {
+
+constexpr int LOAD0 = 0, PRODUCT = 1, EPI0 = 2, CONV0 = 6, LOAD1 = 14;      // warps
+constexpr int THREADS = 15 * 32;
+constexpr int MAX_STAGES = 8, MAX_SLOTS = 8, MAX_GROUPS = 1024;
+constexpr int SLOT_COLS = 32;                 // 128 rows x 64 bfloat16
+constexpr int SMEM_LIMIT = 222 * 1024;        // (with the groups' table, 4 KB, what a block can have)
+constexpr int BAR_BYTES = 512;
+
+struct Args {
+    const uint8_t* w;
+    const uint8_t* w_up;
+    const float* bias;
+    void* out;
+    const int* offsets;
+    long long ldo;
+    int rows, features, K, groups, half_out, accumulate;
+    int tok;                   // rows of x a tile takes
+    int stages, slots, accs;   // ring of shared memory, ring of tensor memory, accumulators
+    int x_bytes, stage_bytes;
+};
+
+struct Tile {
+    int group, f, tok0, tok_end;
+};
+
+// dense: features run fastest (neighbouring blocks share the rows of x); grouped: rows run fastest (they share weights)
+__device__ __forceinline__ Tile tile_of(const Args& p, int tile, int feat_tiles, const int* before) {
+    Tile t;
+    if (!p.offsets) {
+        t.group = 0;
+        t.f = tile % feat_tiles;
+        t.tok0 = tile / feat_tiles * p.tok;
+        t.tok_end = min(p.rows, t.tok0 + p.tok);
+        return t;
+    }
+    int lo = 0, hi = p.groups;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] * feat_tiles <= tile) lo = mid; else hi = mid;
+    }
+    const int n = before[lo + 1] - before[lo], local = tile - before[lo] * feat_tiles;
+    t.group = lo;
+    t.f = local / n;
+    t.tok0 = max(0, p.offsets[lo]) + local % n * p.tok;
+    t.tok_end = min(min(p.rows, p.offsets[lo + 1]), t.tok0 + p.tok);
+    return t;
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// 16 lanes x 32 columns: lane (g, t) gives, for the eight columns of step j, columns 2 t, 2 t + 1 of row g and then of row g + 8
+__device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+          "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t s) {
+    const __nv_bfloat162 r = __hmul2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&s);
+    return *(const uint32_t*)&r;
+}
+
+template <bool GATED, bool HALF>
+__global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const Args p) {
+    constexpr int FEAT = GATED ? 64 : 128;                         // features a tile takes
+    constexpr int PIECE = q4::piece_bytes(HALF), TILE = q4::tile_bytes(HALF);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
+    uint64_t* full = bars;                        // [stages] x and codes have landed
+    uint64_t* empty = full + MAX_STAGES;          // [stages] the products have read x (and the codes were converted before)
+    uint64_t* a_full = empty + MAX_STAGES;        // [slots] the weights lie in tensor memory
+    uint64_t* a_empty = a_full + MAX_SLOTS;       // [slots] the products have read them
+    uint64_t* acc_full = a_empty + MAX_SLOTS;     // [accs]
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+    __shared__ int before[MAX_GROUPS + 1];        // tiles of rows of the groups before
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < p.slots; ++s) mbar_init(&a_full[s], 8), mbar_init(&a_empty[s], 1);
+        for (int s = 0; s < p.accs; ++s) mbar_init(&acc_full[s], 1), mbar_init(&acc_empty[s], 4);
+        fence_barrier_init();
+    }
+    if (warp == PRODUCT) tmem_alloc(tmem_slot, 512);
+    if (p.offsets) {
+        cj::after_predecessor();
+        if (warp == EPI0) {
+            int carry = 0;
+            for (int g0 = 0; g0 < p.groups; g0 += 32) {
+                const int g = g0 + lane;
+                int n = 0;
+                if (g < p.groups) n = max(0, (min(p.rows, p.offsets[g + 1]) - max(0, p.offsets[g]) + p.tok - 1) / p.tok);
+                int inc = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += v;
+                }
+                if (g < p.groups) before[g] = carry + inc - n;
+                carry += __shfl_sync(0xffffffffu, inc, 31);
+            }
+            if (lane == 0) before[p.groups] = carry;
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    // (tensor memory is held: a following kernel's blocks may be set up beside this one)
+    cj::release_successor();
+    const uint32_t tmem = *tmem_slot;
+    const int feat_tiles = (p.features + FEAT - 1) / FEAT, tiles_f = (p.features + 127) / 128, n_kb = (p.K + 63) / 64;
+    const int total = (p.offsets ? before[p.groups] : (p.rows + p.tok - 1) / p.tok) * feat_tiles;
+    const uint32_t acc0 = p.slots * SLOT_COLS;
+
+    if (warp == LOAD0 || warp == LOAD1) {
+        // ---- loads: one warp the even blocks of K, one the odd (what one thread has under way in bulk loads is bounded)
+        if (elect_one()) {
+            const uint32_t mine = warp == LOAD0 ? 0 : 1;
+            if (!mine) tma_prefetch_descriptor(&map_x);
+            auto codes = [&](const Tile& t, int kb, uint8_t* st, uint64_t* bar) {
+                if (GATED) {
+                    // the gate's four pieces and the other weight's
+                    const size_t at = (((size_t)t.group * tiles_f + (t.f >> 1)) * n_kb + kb) * TILE + (t.f & 1) * 4 * PIECE;
+                    bulk_load(st + p.x_bytes, p.w + at, 4 * PIECE, bar);
+                    bulk_load(st + p.x_bytes + 4 * PIECE, p.w_up + at, 4 * PIECE, bar);
+                } else
+                    bulk_load(st + p.x_bytes, p.w + (((size_t)t.group * tiles_f + t.f) * n_kb + kb) * TILE, TILE, bar);
+            };
+            // weights are written by no kernel of a step: the first ring of codes leaves before the wait for the kernel that makes x
+            uint32_t early = 0;
+            if (!p.offsets) {
+                if ((int)blockIdx.x < total) {
+                    const Tile t = tile_of(p, blockIdx.x, feat_tiles, before);
+                    for (; (int)early < min(n_kb, p.stages); ++early) {
+                        if ((early & 1) != mine) continue;
+                        mbar_expect_tx(&full[early], p.x_bytes + TILE);
+                        codes(t, early, smem + (size_t)early * p.stage_bytes, &full[early]);
+                    }
+                }
+                cj::after_predecessor();
+            }
+            uint32_t it = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                const Tile t = tile_of(p, tile, feat_tiles, before);
+                for (int kb = 0; kb < n_kb; ++kb, ++it) {
+                    if ((it & 1) != mine) continue;
+                    const int s = it % p.stages;
+                    uint8_t* st = smem + (size_t)s * p.stage_bytes;
+                    if (it >= early) {
+                        ok = mbar_wait(&empty[s], ((it / p.stages) & 1) ^ 1, 1);
+                        if (!ok) break;
+                        mbar_expect_tx(&full[s], p.x_bytes + TILE);
+                        codes(t, kb, st, &full[s]);
+                    }
+                    tma_load_2d(st, &map_x, &full[s], kb * 64, t.tok0);
+                }
+            }
+        }
+    } else if (warp == PRODUCT) {
+        // ---- products
+        if (elect_one()) {
+            uint32_t it = 0, at = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++at) {
+                const Tile t = tile_of(p, tile, feat_tiles, before);
+                const int as = at % p.accs;
+                ok = mbar_wait(&acc_empty[as], ((at / p.accs) & 1) ^ 1, 2);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint32_t acc = tmem + acc0 + as * p.tok;
+                const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
+                for (int kb = 0; kb < n_kb; ++kb, ++it) {
+                    const int s = it % p.stages, slot = it % p.slots;
+                    // (the slot's weights came out of the stage: x lies there too)
+                    ok = mbar_wait(&a_full[slot], (it / p.slots) & 1, 3) && mbar_wait(&full[s], (it / p.stages) & 1, 4);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint64_t dx = umma_desc_sw128(smem + (size_t)s * p.stage_bytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_bf16_a_tmem(acc, tmem + slot * SLOT_COLS + 8 * k, dx + 2 * k, idesc, (kb | k) ? 1u : 0u);
+                    umma_commit(&empty[s]);
+                    umma_commit(&a_empty[slot]);
+                }
+                if (ok) umma_commit(&acc_full[as]);
+            }
+        }
+    } else if (warp >= CONV0) {
+        // ---- codes to bfloat16: a piece of 16 features a warp, into the 16 lanes of tensor memory that are the piece's rows
+        const int q = warp & 3, upper = (warp - CONV0) >> 2;       // the quarter of the lanes this warp may touch, and which half of it
+        const int piece = GATED ? upper * 4 + q : q * 2 + upper;
+        const uint32_t lanes = (uint32_t)(q * 32 + upper * 16) << 16;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+            for (int kb = 0; kb < n_kb; ++kb, ++it) {
+                const int s = it % p.stages, slot = it % p.slots;
+                ok = mbar_wait_warp(&full[s], (it / p.stages) & 1, 5);
+                if (!ok) break;
+                const uint8_t* src = smem + (size_t)s * p.stage_bytes + p.x_bytes + piece * PIECE;
+                const uint4 c = *(const uint4*)(src + lane * 16);
+                uint32_t sc[HALF ? 2 : 1];
+#pragma unroll
+                for (int h = 0; h < (HALF ? 2 : 1); ++h) sc[h] = *(const uint32_t*)(src + 512 + (h * 8 + (lane >> 2)) * 4);
+                uint32_t v[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a = (j < 2 ? c.x : c.y) >> (8 * (j & 1)), b = (j < 2 ? c.z : c.w) >> (8 * (j & 1));
+                    const uint32_t s2 = sc[HALF ? j >> 1 : 0], lo = __byte_perm(s2, 0, 0x1010), hi = __byte_perm(s2, 0, 0x3232);
+                    v[4 * j] = times(q4::pair(a), lo);
+                    v[4 * j + 1] = times(q4::pair(a >> 4), lo);
+                    v[4 * j + 2] = times(q4::pair(b), hi);
+                    v[4 * j + 3] = times(q4::pair(b >> 4), hi);
+                }
+                ok = mbar_wait_warp(&a_empty[slot], ((it / p.slots) & 1) ^ 1, 6);
+                if (!ok) break;
+                tcgen05_fence_after();
+                tmem_st_16x256b_x4(tmem + slot * SLOT_COLS + lanes, v);
+                tmem_st_wait();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[slot]);
+            }
+        }
+    } else {
+        // ---- epilogue: warps 2 .. 5, a quarter of the lanes each; a lane is a feature, columns are rows of x
+        if (!p.offsets) cj::after_predecessor();
+        const int q = warp & 3;
+        uint32_t at = 0;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++at) {
+            const Tile t = tile_of(p, tile, feat_tiles, before);
+            const int as = at % p.accs;
+            if (!mbar_wait_warp(&acc_full[as], (at / p.accs) & 1, 7)) break;
+            tcgen05_fence_after();
+            const uint32_t src = tmem + acc0 + as * p.tok + ((uint32_t)(q * 32) << 16);
+            const int n = t.tok_end - t.tok0;
+            const int feature = GATED ? t.f * 64 + q * 16 + (lane & 15) : t.f * 128 + q * 32 + lane;
+            const bool in = feature < p.features;
+            const float bias = !GATED && p.bias && in ? p.bias[feature] : 0.0f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < n; c0 += 16) {
+                uint32_t v[16];
+                tmem_ld16(src + c0, v);
+                tmem_ld_wait();
+                if (GATED) {
+                    // lanes 0 .. 15 hold the gate's sums, 16 .. 31 the other weight's: the lower take the first eight rows, the upper the others
+                    const bool low = lane < 16;
+                    const int first = c0 + (low ? 0 : 8);
+                    __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)(t.tok0 + first) * p.ldo + feature;
+                    float* dst32 = (float*)p.out + (size_t)(t.tok0 + first) * p.ldo + feature;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float mine = __uint_as_float(low ? v[j] : v[8 + j]);
+                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(low ? v[8 + j] : v[j]), 16);
+                        const float y = cj::gated_act_fast(low ? mine : other, low ? other : mine, 0.0f, 1.0f, 0.0f);
+                        if (in && first + j < n) {
+                            if (p.half_out) dst[(size_t)j * p.ldo] = __float2bfloat16_rn(y);
+                            else dst32[(size_t)j * p.ldo] = y;
+                        }
+                    }
+                } else if (in) {
+                    const size_t o = (size_t)(t.tok0 + c0) * p.ldo + feature;
+                    if (p.half_out) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c0 + j < n) ((__nv_bfloat16*)p.out)[o + (size_t)j * p.ldo] = __float2bfloat16_rn(__uint_as_float(v[j]) + bias);
+                    } else if (p.accumulate) {
+                        float old[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) old[j] = c0 + j < n ? ((const float*)p.out)[o + (size_t)j * p.ldo] : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c0 + j < n) ((float*)p.out)[o + (size_t)j * p.ldo] = old[j] + (__uint_as_float(v[j]) + bias);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (c0 + j < n) ((float*)p.out)[o + (size_t)j * p.ldo] = __uint_as_float(v[j]) + bias;
+                    }
+                }
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[as]);
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == PRODUCT) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// The rows that a mixture's groups read, side by side: out[s] = x[index[s]], zeros where there is no such row.  A warp a row.
+__global__ void __launch_bounds__(256) q4_gather_kernel(uint4* __restrict__ out, const __nv_bfloat16* __restrict__ x, long long ldx, int x_rows,
+                                                        const int* __restrict__ index, int rows, int n16) {
+    cj::after_predecessor();
+    cj::release_successor();
+    const int s = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (s >= rows) return;
+    const int r = index[s];
+    const uint4* src = r >= 0 && r < x_rows ? (const uint4*)(x + (size_t)r * ldx) : nullptr;
+    for (int i = threadIdx.x & 31; i < n16; i += 32) out[(size_t)s * n16 + i] = src ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+}
+
+}  // namespace
+
+// x bf16 [x_rows, ldx] -> out bf16 [rows, K]; x, ldx, K and out of 16 bytes
+CJ_EXPORT int cj_q4_gather(const void* x, long long ldx, int x_rows, const int* index, void* out, int rows, int K, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (!x || !index || !out || K <= 0 || x_rows <= 0) return CJ_ERR_ARG;
+    if ((K & 7) || (ldx & 7) || (((uintptr_t)x | (uintptr_t)out) & 15)) return CJ_ERR_ALIGN;
+    cj::launch(q4_gather_kernel, dim3((rows + 7) / 8), dim3(256), 0, stream, (uint4*)out, (const __nv_bfloat16*)x, ldx, x_rows, index, rows, K / 8);
+    return cj::launch_status();
+}
+
+// As cj_gemm_q4, without gathered rows: row s of out comes from row s of x (x_rows of them; rows past the last are zeros).  x and ldx
+// of 16 bytes; tok: rows of x a tile takes, a multiple of 16 from 16 to 256.
+CJ_EXPORT int cj_gemm_q4_tc(const void* x, long long ldx, int x_rows, const void* w, const void* w_up, const float* bias, void* out, int out_dtype,
+                            long long ldo, int rows, int features, int K, int groups, int half, const int* offsets, int accumulate, int tok,
+                            int sms, cudaStream_t stream) {
+    if (rows <= 0) return 0;
+    if (!x || !w || !out || features <= 0 || K <= 0 || groups <= 0 || x_rows <= 0 || sms <= 0) return CJ_ERR_ARG;
+    if (out_dtype != CJ_F32 && out_dtype != CJ_BF16) return CJ_ERR_DTYPE;
+    if (accumulate && (out_dtype != CJ_F32 || w_up)) return CJ_ERR_DTYPE;
+    if ((w_up && bias) || (!offsets && groups != 1)) return CJ_ERR_ARG;
+    if ((ldx & 7) || ldx < K || ((uintptr_t)x & 15) || (((uintptr_t)w | (uintptr_t)w_up) & 15)) return CJ_ERR_ALIGN;
+    if (groups > MAX_GROUPS || tok < 16 || tok > 256 || tok % 16 != 0) return CJ_ERR_SIZE;
+    const int feat_tiles = (features + (w_up ? 63 : 127)) / (w_up ? 64 : 128);
+    if ((long long)feat_tiles * ((rows + 15) / 16 + groups) > 0x7fffffffLL) return CJ_ERR_SIZE;
+    CUtensorMap map;
+    if (!make_map_bf16(&map, x, x_rows, K, ldx, tok)) return CJ_ERR_ARG;
+    Args a{(const uint8_t*)w, (const uint8_t*)w_up, bias, out, offsets, ldo, rows, features, K, groups, out_dtype == CJ_BF16 ? 1 : 0, accumulate,
+           tok, 0, 0, 0, tok * 128, 0};
+    a.stage_bytes = a.x_bytes + (q4::tile_bytes(half != 0) + 1023) / 1024 * 1024;
+    a.stages = min(MAX_STAGES, (SMEM_LIMIT - 1024 - BAR_BYTES) / a.stage_bytes);
+    // two accumulators where at least three slots of weights fit beside them
+    a.accs = 2 * tok + 3 * SLOT_COLS <= 512 ? 2 : 1;
+    a.slots = min(MAX_SLOTS, (512 - a.accs * tok) / SLOT_COLS);
+    const int smem = a.stages * a.stage_bytes + BAR_BYTES + 1024;
+    const long long most = offsets ? sms : (long long)feat_tiles * ((rows + tok - 1) / tok);
+    auto kern = w_up ? (half ? gemm_q4_tc_kernel<true, true> : gemm_q4_tc_kernel<true, false>)
+                     : (half ? gemm_q4_tc_kernel<false, true> : gemm_q4_tc_kernel<false, false>);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    cj::launch(kern, dim3((unsigned)(most < sms ? most : sms)), dim3(THREADS), smem, stream, map, a);
+    return cj::launch_status();
+}
+
+CJ_EXPORT int cj_gemm_q4_tc_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, tc::g_error_flag, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}

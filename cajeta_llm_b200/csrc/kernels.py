@@ -1685,7 +1685,8 @@ def wait_errors() -> Dict[str, int]:
     when all is well.  Only libraries that are already loaded are asked."""
     found = {}
     for name, symbol in (("gemm_tc", "cj_gemm_tc_error"), ("gemm_tc2", "cj_gemm_tc2_error"), ("gemm_f32_tc", "cj_gemm_f32_tc_error"),
-                         ("attention_prefill_tc", "cj_prefill_attention_tc_error"), ("attention_flash_tc", "cj_attention_flash_tc_error")):
+                         ("attention_prefill_tc", "cj_prefill_attention_tc_error"), ("attention_flash_tc", "cj_attention_flash_tc_error"),
+                         ("gemm_q4_tc", "cj_gemm_q4_tc_error")):
         lib = _libs.get(name)
         if lib is not None:
             code = int(getattr(lib, symbol)())
@@ -1930,6 +1931,21 @@ class Q4Weight:
         return math.prod(self.shape)
 
 
+Q4_TC_ROWS = 32      # rows (of a group, on average) from which on a product with 4-bit weights runs on tcgen05
+
+
+@functools.lru_cache(maxsize=4096)
+def q4_tile_rows(rows: int, features: int, groups: int, gated: bool, sms: int) -> int:
+    """Rows of x that a tile of the tensor-core product with 4-bit weights takes."""
+    if groups:
+        # tiles that most groups of an even split fill once (mean and two standard deviations)
+        mean = rows / groups
+        return min(256, -(-int(mean + 2.0 * mean ** 0.5) // 16) * 16)
+    feature_tiles = -(-features // (64 if gated else 128))
+    # rounds of the machine times what a tile of that many rows takes (its columns, and some for its start)
+    return min(range(256, 15, -16), key=lambda n: -(-feature_tiles * -(-rows // n) // sms) * (n + 16))
+
+
 def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torch.Tensor] = None, accumulate: bool = False,
             w_up: Optional[Q4Weight] = None, group_offsets: Optional[torch.Tensor] = None, a_row_index: Optional[torch.Tensor] = None) -> None:
     """out[M, N] (+)= a[M, K] . w[N, K]^T (+ bias) for bfloat16 rows and 4-bit weights; products and sums in float32 of the weights'
@@ -1971,10 +1987,27 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
         return
     if a.shape[0] == 0:
         raise KernelError("gemm_q4: a has no rows")
+    half = 1 if w.group == 32 else 0
+    per_group = M / w.groups
+    if per_group > Q4_TC_ROWS and a.stride(0) % 8 == 0 and a.data_ptr() % 16 == 0:
+        global launches
+        x, x_rows = a, a.shape[0]
+        if a_row_index is not None:
+            x = torch.empty((M, w.k), dtype=torch.bfloat16, device=a.device)
+            st = library("gemm_q4_tc").cj_q4_gather(_ptr(a), _ll(a.stride(0)), _i(x_rows), _ptr(a_row_index), _ptr(x), _i(M), _i(w.k), _stream())
+            _check(st, "gemm_q4")
+            x_rows = M
+        tok = q4_tile_rows(M, w.features, w.groups if group_offsets is not None else 0, w_up is not None, _sm_count())
+        st = library("gemm_q4_tc").cj_gemm_q4_tc(
+            _ptr(x), _ll(x.stride(0)), _i(x_rows), _ptr(w.data), _ptr(w_up.data if w_up is not None else None), _ptr(bias), _ptr(out), _i(_code(out)),
+            _ll(out.stride(0)), _i(M), _i(w.features), _i(w.k), _i(w.groups), _i(half), _ptr(group_offsets), _i(1 if accumulate else 0), _i(tok),
+            _i(_sm_count()), _stream())
+        _check(st, "gemm_q4")
+        return
     n_tok = 8 if M <= 8 or group_offsets is not None and M <= 4 * w.groups else 16 if M <= 16 else 32
     pieces = 1 if n_tok == 8 else 2
     st = library("gemm_q4").cj_gemm_q4(
         _ptr(a), _ll(a.stride(0)), _i(a.shape[0]), _ptr(w.data), _ptr(w_up.data if w_up is not None else None), _ptr(bias), _ptr(out),
-        _i(_code(out)), _ll(out.stride(0)), _i(M), _i(w.features), _i(w.k), _i(w.groups), _i(1 if w.group == 32 else 0), _ptr(group_offsets),
+        _i(_code(out)), _ll(out.stride(0)), _i(M), _i(w.features), _i(w.k), _i(w.groups), _i(half), _ptr(group_offsets),
         _ptr(a_row_index), _i(1 if accumulate else 0), _i(n_tok), _i(pieces), _stream())
     _check(st, "gemm_q4")

@@ -205,7 +205,7 @@ class PagedAttention(Part):
         if self.runtime.e4m3_cache:
             libs.add("cache_e4m3")
         if self.runtime.q4_weights:
-            libs.add("gemm_q4")
+            libs |= {"gemm_q4", "gemm_q4_tc"}
         if "attention_paged" in libs and self.runtime.act_dtype == torch.float32:
             libs.add("attention_f32")
         if self.runtime.fast_kernels and self.hidden >= 128:

@@ -103,7 +103,7 @@ class DenseSwiGLU(Part):
         return p
 
     def libraries(self) -> set:
-        libs = {"gemm_simt"} | ({"gemm_q4"} if self.runtime.q4_weights else set())
+        libs = {"gemm_simt"} | ({"gemm_q4", "gemm_q4_tc"} if self.runtime.q4_weights else set())
         if self.runtime.fast_kernels and self.hidden >= 128:
             libs |= {"gemm_tc", "gemm_tc2"}
         return libs
@@ -267,7 +267,7 @@ class SparseMoE(Part):
         return self.name(self.n_expert[proj].format(e=e))
 
     def libraries(self) -> set:
-        libs = {"rowwise", "moe_route", "gemm_simt"} | ({"gemm_q4"} if self.runtime.q4_weights else set()) | ({"recurrent"} if self.weight_on == "input" else set())
+        libs = {"rowwise", "moe_route", "gemm_simt"} | ({"gemm_q4", "gemm_q4_tc"} if self.runtime.q4_weights else set()) | ({"recurrent"} if self.weight_on == "input" else set())
         if self.runtime.fast_kernels and self.hidden >= 128:
             libs |= {"gemm_tc", "gemm_tc2"}
         return libs
