@@ -1,0 +1,468 @@
+// Attention of portions of prompts over the 8-bit cache (cache_e4m3.cu) on the 5th-generation tensor cores (tcgen05), heads of 64 or 128.
+//
+// A block takes 256 query rows of one request and one query head, as two tiles of 128 rows that share every tile of 128 keys and values:
+//     S = q . (code_k 2^e_k)^T        scores [128 x 128] in tensor memory
+//     P = exp2(S scale - m)           four warps a query tile, a row a thread; P as bfloat16 over the columns of its scores
+//     O += P . (code_v 2^e_v)         O in tensor memory
+// A code times its power of two is a bfloat16 number exactly, whatever the exponents of the tokens beside it (f16 would keep more bits of P,
+// but only values within 22 octaves of each other: a row's values could vanish beside larger ones that it does not even see).  So three warps
+// turn codes into the bfloat16 tiles in shared memory that both products read, and the rest is attention over a bfloat16 cache: P, as there, is
+// the one rounding.  The codes come with plain 16-byte loads, pages of any size, a tile's keys in registers while its predecessor's values are
+// converted (half the bytes of a bfloat16 cache: 16 KB a tile).  The two query tiles take turns between the exponential unit and the tensor
+// core, each key tile is worked on as two halves of 64 keys, and the reference maximum moves only when it grows by more than 2^8.
+// Every wait is bounded (tc_common.cuh).
+#define CJ_LIB "attention_e4m3_tc"
+#include "common.cuh"
+#include "e4m3.cuh"
+#include "tc_common.cuh"
+
+using namespace tc;
+
+namespace {
+
+constexpr int BM = 128, QT = 2, BN = 128;         // query rows a tile, tiles a block, keys a tile
+constexpr int STAGES = 2;
+constexpr int CONV_WARPS = 3, PRODUCT = 3, SOFT0 = 4;
+constexpr int THREADS = 12 * 32;                  // three warps a scheduler: 168 registers a thread
+constexpr int HALF_BYTES = 128 * 64 * 2;          // [128 x 64] f16, swizzled: 16 KB
+constexpr float RESCALE_THRESHOLD = 8.0f;         // in log2 units
+constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
+
+template <int HD>
+struct Smem {
+    static constexpr int TILE = HALF_BYTES * (HD / 64);
+    static constexpr int Q = 0, K = QT * TILE, V = K + STAGES * TILE, TAB = V + STAGES * TILE;
+    // a converting warp's look-ups of two tiles: rows of the planes, the keys' and the values' powers of two
+    static constexpr int TAB_WARP = 2 * BN * (4 + 4 + 4), BAR = TAB + CONV_WARPS * TAB_WARP;
+    static constexpr int TOTAL = BAR + 256 + 1024;
+};
+
+struct Args {
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    const uint8_t *kplane, *vplane, *kexp, *vexp;
+    const int *req_start, *req_prior, *table;
+    int n_requests, table_stride, page_tokens, n_pages, n_heads, n_kv, window;
+    float scale_log2;
+    int total_rows, block_rows;
+};
+
+struct QueryTile {
+    int rows, p0, begin, end;      // rows of the step (0: empty), position of the first, key tiles [begin, end] of the block's
+};
+
+// four codes times a power of two, as bfloat16
+__device__ __forceinline__ uint2 scaled_codes(uint32_t w, f32x2 f) {
+    uint32_t lo, hi;
+    cj::e4m3x4_to_f16(w, lo, hi);
+    const float2 a = __half22float2(*(const __half2*)&lo), b = __half22float2(*(const __half2*)&hi);
+    const float2 x = unpack2(mul2(pack2(a.x, a.y), f)), y = unpack2(mul2(pack2(b.x, b.y), f));
+    const __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), v = __floats2bfloat162_rn(y.x, y.y);
+    return make_uint2(*(const uint32_t*)&u, *(const uint32_t*)&v);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __grid_constant__ CUtensorMap map_q, const Args p) {
+    using S = Smem<HD>;
+    constexpr int TILE = S::TILE;
+    // blocks beyond the portions' row blocks leave before anything else (a captured step's layout has room for more than it brings)
+    cj::after_predecessor();
+    {
+        int tiles = 0;
+        for (int r = threadIdx.x & 31; r < p.n_requests; r += 32)
+            tiles += (__ldcg(p.req_start + r + 1) - __ldcg(p.req_start + r) + p.block_rows - 1) / p.block_rows;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        if ((int)blockIdx.y >= tiles) return;
+    }
+    // the last row blocks of every request first: they see the most keys
+    int req = -1, row0 = 0, rows = 0;
+    {
+        int b = (int)blockIdx.y;
+        for (int level = 0; req < 0; ++level) {
+            bool any = false;
+            for (int r = 0; r < p.n_requests; ++r) {
+                const int lo = p.req_start[r], n = p.req_start[r + 1] - lo;
+                const int tiles = (n + p.block_rows - 1) / p.block_rows;
+                if (tiles <= level) continue;
+                any = true;
+                if (b-- == 0) {
+                    req = r;
+                    row0 = lo + (tiles - 1 - level) * p.block_rows;
+                    rows = min(p.block_rows, lo + n - row0);
+                    break;
+                }
+            }
+            if (!any) return;
+        }
+    }
+    rows = min(rows, p.total_rows - row0);
+    if (rows <= 0) return;
+    const int h = blockIdx.x, kvh = h / (p.n_heads / p.n_kv);
+    const int p0 = p.req_prior[req] + (row0 - p.req_start[req]);
+    const int p_last = min(p0 + rows - 1, p.table_stride * p.page_tokens - 1);
+    const int key_from = (p.window > 0 && p0 + 1 > p.window) ? p0 + 1 - p.window : 0;
+    const int kt_begin = key_from / BN;
+    QueryTile qt[QT];
+#pragma unroll
+    for (int g = 0; g < QT; ++g) {
+        qt[g].rows = max(0, min(BM, rows - g * BM));
+        qt[g].p0 = p0 + g * BM;
+        const int from = (p.window > 0 && qt[g].p0 + 1 > p.window) ? qt[g].p0 + 1 - p.window : 0;
+        qt[g].begin = from / BN - kt_begin;
+        qt[g].end = qt[g].rows > 0 ? (qt[g].p0 + qt[g].rows - 1) / BN - kt_begin : qt[g].begin - 1;
+    }
+    const int n_tiles = max(qt[0].end, qt[1].end) + 1;
+    const int* tab = p.table + (size_t)req * p.table_stride;
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = (uint64_t*)(smem + S::BAR);
+    uint64_t* q_full = bars;                      // the queries have landed
+    uint64_t* k_full = bars + 1;                  // [STAGES]
+    uint64_t* k_empty = k_full + STAGES;
+    uint64_t* v_full = k_empty + STAGES;
+    uint64_t* v_empty = v_full + STAGES;
+    uint64_t* s_full = v_empty + STAGES;          // [QT] a query tile's scores are complete (and every product before them)
+    uint64_t* p_full = s_full + QT;               // [QT][2] the weights of a tile's first / last 64 keys are written
+    uint64_t* half_done = p_full + 2 * QT;        // [QT] the output product over a tile's first 64 keys is done
+    uint64_t* o_done = half_done + QT;            // [QT] the last output product is done
+    uint32_t* tmem_slot = (uint32_t*)(o_done + QT);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&k_full[s], CONV_WARPS * 32), mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], CONV_WARPS * 32), mbar_init(&v_empty[s], 1);
+        }
+        for (int g = 0; g < QT; ++g) {
+            mbar_init(&s_full[g], 1), mbar_init(&half_done[g], 1), mbar_init(&o_done[g], 1);
+            mbar_init(&p_full[2 * g], BM), mbar_init(&p_full[2 * g + 1], BM);
+        }
+        fence_barrier_init();
+    }
+    if (warp == PRODUCT) tmem_alloc(tmem_slot, TM_COLS);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    cj::release_successor();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp < CONV_WARPS) {
+        // ---- codes -> f16 tiles ----------------------------------------------------------------------
+        constexpr int PIECES = HD / 16;                    // of 16 codes a row
+        constexpr int ROWS_WARP = 32 / PIECES, ROWS_PASS = CONV_WARPS * ROWS_WARP, PASSES = (BN + ROWS_PASS - 1) / ROWS_PASS;
+        const int piece = lane % PIECES, r0 = warp * ROWS_WARP + lane / PIECES;
+        // This warp's look-ups of tiles i and i + 1 (every warp makes them all: four keys a lane, and no barrier between the warps)
+        int* rows_w = (int*)(smem + S::TAB + warp * S::TAB_WARP);
+        float* kf_w = (float*)(rows_w + 2 * BN);
+        float* vf_w = kf_w + 2 * BN;
+        int page[4], ek[4], ev[4];
+        auto ask_pages = [&](int i) {                      // pages of tile i's keys lane, lane + 32, ...
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = (kt_begin + i) * BN + j * 32 + lane;
+                page[j] = key >= key_from && key <= p_last ? __ldg(tab + key / p.page_tokens) : -1;
+            }
+        };
+        auto ask_exponents = [&](int i) {                  // their rows in the planes (-1: none), exponents on the way
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = (kt_begin + i) * BN + j * 32 + lane;
+                const int row = page[j] >= 0 && page[j] < p.n_pages ? (page[j] * p.n_kv + kvh) * p.page_tokens + key % p.page_tokens : -1;
+                rows_w[(i & 1) * BN + j * 32 + lane] = row;
+                ek[j] = row >= 0 ? (int)p.kexp[row] : 0;
+                ev[j] = row >= 0 ? (int)p.vexp[row] : 0;
+            }
+            __syncwarp();
+        };
+        auto factors = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                kf_w[(i & 1) * BN + j * 32 + lane] = __uint_as_float((uint32_t)ek[j] << 23);
+                vf_w[(i & 1) * BN + j * 32 + lane] = __uint_as_float((uint32_t)ev[j] << 23);
+            }
+            __syncwarp();
+        };
+        uint4 kc[PASSES], vc[PASSES];
+        auto load = [&](int i, const uint8_t* plane, uint4 (&c)[PASSES]) {
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) {
+                const int row = r0 + j * ROWS_PASS < BN ? rows_w[(i & 1) * BN + r0 + j * ROWS_PASS] : -1;
+                c[j] = row >= 0 ? __ldg((const uint4*)(plane + (size_t)row * HD + piece * 16)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        auto put = [&](int i, bool values, const uint4 (&c)[PASSES]) -> bool {
+            const int s = i % STAGES;
+            if (!mbar_wait_warp(values ? &v_empty[s] : &k_empty[s], ((i / STAGES) & 1) ^ 1, 11)) return false;
+            uint8_t* half = smem + (values ? S::V : S::K) + s * TILE + (piece >> 2) * HALF_BYTES;
+            const float* factor = (values ? vf_w : kf_w) + (i & 1) * BN;
+            const int chunk = (piece & 3) * 2;
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) {
+                const int r = r0 + j * ROWS_PASS;
+                if (r >= BN) break;
+                const f32x2 f = pack2(factor[r], factor[r]);
+                const uint2 a = scaled_codes(c[j].x, f), b = scaled_codes(c[j].y, f), d = scaled_codes(c[j].z, f), e = scaled_codes(c[j].w, f);
+                *(uint4*)(half + r * 128 + ((chunk ^ (r & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+                *(uint4*)(half + r * 128 + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+            }
+            fence_async_shared();
+            mbar_arrive(values ? &v_full[s] : &k_full[s]);
+            return true;
+        };
+        // in the order the products want them: K0, V0, K1, V1, ...  While the values of a tile are converted the next tile's keys and
+        // exponents and the pages of the one after are on their way; while those keys are, their values
+        ask_pages(0);
+        ask_exponents(0);
+        load(0, p.kplane, kc);
+        load(0, p.vplane, vc);
+        if (n_tiles > 1) ask_pages(1);
+        factors(0);
+        bool ok = put(0, false, kc);
+        for (int i = 0; i < n_tiles && ok; ++i) {
+            const bool next = i + 1 < n_tiles;
+            if (next) {
+                ask_exponents(i + 1);
+                load(i + 1, p.kplane, kc);
+                if (i + 2 < n_tiles) ask_pages(i + 2);
+            }
+            ok = put(i, true, vc);
+            if (!ok || !next) break;
+            factors(i + 1);
+            load(i + 1, p.vplane, vc);
+            ok = put(i + 1, false, kc);
+        }
+    } else if (warp == PRODUCT) {
+        // ---- products, in the order S_a(0) S_b(0), then per key tile i: PV_a(i) S_a(i + 1) PV_b(i) S_b(i + 1), each PV in two halves of
+        // 64 keys.  S_g(i + 1) overwrites the columns PV_g(i) reads P from; one thread's products run in the order they were issued
+        if (elect_one()) {
+            // rows [row0, row0 + 256) of the [rows, heads x HD] view, columns of this head (rows past the step's end read as zero)
+            const int q_tiles = qt[1].rows > 0 ? 2 : 1;
+            mbar_expect_tx(q_full, q_tiles * TILE);
+            for (int g = 0; g < q_tiles; ++g)
+                for (int half = 0; half < HD / 64; ++half)
+                    tma_load_2d(smem + S::Q + g * TILE + half * HALF_BYTES, &map_q, q_full, h * HD + half * 64, row0 + g * BM);
+            bool ok = mbar_wait(q_full, 0, 12);
+            int p_seen[QT] = {0, 0};
+            auto uses = [&](int g, int i) { return i >= qt[g].begin && i <= qt[g].end; };
+            auto scores = [&](int g, int i) {
+                const int s = i % STAGES;
+                const uint32_t acc = tmem_base + TM_S + g * BN;
+#pragma unroll
+                for (int half = 0; half < HD / 64; ++half) {
+                    const uint64_t dq = umma_desc_sw128(smem + S::Q + g * TILE + half * HALF_BYTES);
+                    const uint64_t dk = umma_desc_sw128(smem + S::K + s * TILE + half * HALF_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_bf16(acc, dq + 2 * k, dk + 2 * k, umma_idesc_bf16(128, BN), (half | k) ? 1u : 0u);
+                }
+                umma_commit(&s_full[g]);
+            };
+            if (ok) ok = mbar_wait(&k_full[0], 0, 13);
+            if (ok) {
+                tcgen05_fence_after();
+#pragma unroll
+                for (int g = 0; g < QT; ++g)
+                    if (uses(g, 0)) scores(g, 0);
+                umma_commit(&k_empty[0]);
+            }
+            for (int i = 0; i < n_tiles && ok; ++i) {
+                const int s = i % STAGES;
+                const bool next = i + 1 < n_tiles;
+                ok = mbar_wait(&v_full[s], (i / STAGES) & 1, 19);
+                if (!ok) break;
+                const uint64_t dv = umma_desc_mn_sw128(smem + S::V + s * TILE, HALF_BYTES);
+                bool k_there = false;
+#pragma unroll
+                for (int g = 0; g < QT; ++g) {
+                    if (!ok) break;
+                    if (uses(g, i)) {
+                        const uint32_t acc = tmem_base + TM_O + g * HD, pa = tmem_base + TM_S + g * BN;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            ok = mbar_wait(&p_full[2 * g + half], p_seen[g] & 1, 15);
+                            if (!ok) break;
+                            tcgen05_fence_after();
+                            // 16 keys are 8 columns of P and two 8-row groups of V (2048 bytes); B is MN-major (bit 16)
+#pragma unroll
+                            for (int k = 4 * half; k < 4 * half + 4; ++k)
+                                umma_bf16_a_tmem(acc, pa + 8 * k, dv + (uint64_t)(k * 2048 >> 4), umma_idesc_bf16(128, HD) | (1u << 16),
+                                                 (i > qt[g].begin || k > 0) ? 1u : 0u);
+                            if (half == 0) umma_commit(&half_done[g]);
+                        }
+                        if (!ok) break;
+                        ++p_seen[g];
+                        if (i == qt[g].end) umma_commit(&o_done[g]);
+                    }
+                    if (g == QT - 1) umma_commit(&v_empty[s]);
+                    if (next && (uses(g, i + 1) || g == QT - 1)) {
+                        if (!k_there) {
+                            ok = mbar_wait(&k_full[(i + 1) % STAGES], ((i + 1) / STAGES) & 1, 13);
+                            if (!ok) break;
+                            tcgen05_fence_after();
+                            k_there = true;
+                        }
+                        if (uses(g, i + 1)) scores(g, i + 1);
+                        if (g == QT - 1) umma_commit(&k_empty[(i + 1) % STAGES]);
+                    }
+                }
+            }
+        }
+    } else {
+        // ---- softmax of one query tile, a row a thread ------------------------------------------------------------
+        const int g = (warp - SOFT0) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const QueryTile mine = g == 0 ? qt[0] : qt[1];
+        const int pos = mine.p0 + r, from = (p.window > 0 && pos + 1 > p.window) ? pos + 1 - p.window : 0;
+        const size_t row_at = ((size_t)(row0 + g * BM + r) * p.n_heads + h) * HD;
+        const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+        const uint32_t s_addr = tmem_base + TM_S + g * BN + lane_off, o_addr = tmem_base + TM_O + g * HD + lane_off;
+        float m_ref = -INFINITY, l = 0.0f;
+        bool ok = true;
+        const int n_mine = mine.end - mine.begin + 1;
+        for (int j = 0; j < n_mine && ok; ++j) {
+            ok = mbar_wait_warp(&s_full[g], j & 1, 16);
+            if (!ok) break;
+            tcgen05_fence_after();
+            // columns [lo, lo + span] are keys this row may see (span < 0: none)
+            const int kbase = (kt_begin + mine.begin + j) * BN, lo = max(from - kbase, 0), span = min(pos - kbase, BN - 1) - lo;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                constexpr int HC = BN / 2;
+                uint32_t v[HC];
+                tmem_ld32<0>(s_addr + half * HC, v);
+                tmem_ld32<32>(s_addr + half * HC + 32, v);
+                tmem_ld_wait();
+                if (lo != 0 || span != BN - 1) {
+#pragma unroll
+                    for (int c = 0; c < HC; ++c)
+                        if (!((unsigned)(half * HC + c - lo) <= (unsigned)span && span >= 0)) v[c] = 0xff800000u;       // -inf
+                }
+                // one pass with the reference maximum so far; again only where these keys raise it by more than the threshold
+                float m_use = m_ref, factor = 1.0f, sum;
+                bool rescale = false;
+                uint32_t packed[HC];                   // only [0, 32) is used
+#pragma unroll 1
+                for (int attempt = 0;; ++attempt) {
+                    const float neg_sub = m_use == -INFINITY ? 0.0f : -m_use;
+                    const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2), sub2 = pack2(neg_sub, neg_sub);
+                    f32x2 sum2a = pack2(0.0f, 0.0f), sum2b = sum2a;
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < HC; c += 4) {
+                        const float2 t0 = unpack2(fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, sub2));
+                        const float2 t1 = unpack2(fma2(pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, sub2));
+                        const float e0 = ex2(t0.x), e1 = ex2(t0.y), e2 = ex2(t1.x), e3 = ex2(t1.y);
+                        sum2a = add2(sum2a, pack2(e0, e1));
+                        sum2b = add2(sum2b, pack2(e2, e3));
+                        const __nv_bfloat162 b0 = __floats2bfloat162_rn(e0, e1), b1 = __floats2bfloat162_rn(e2, e3);
+                        packed[c >> 1] = *(const uint32_t*)&b0;
+                        packed[(c >> 1) + 1] = *(const uint32_t*)&b1;
+                        mx0 = max3(mx0, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+                        mx1 = max3(mx1, __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+                    }
+                    const float2 sa = unpack2(sum2a), sb = unpack2(sum2b);
+                    sum = (sa.x + sa.y) + (sb.x + sb.y);
+                    if (attempt == 1) break;
+                    const float mx = fmaxf(mx0, mx1) * p.scale_log2;
+                    float m_new = m_ref;
+                    if (mx > m_ref + RESCALE_THRESHOLD || m_ref == -INFINITY) m_new = fmaxf(m_ref, mx);
+                    if (!__any_sync(0xffffffffu, m_new != m_ref)) break;
+                    rescale = m_new != m_ref && m_ref != -INFINITY;
+                    factor = rescale ? exp2f(m_ref - m_new) : 1.0f;
+                    m_use = m_new;
+                }
+                tmem_st32<0>(s_addr + half * (HC / 2), packed);
+                l = l * factor + sum;
+                m_ref = m_use;
+                // O may be rescaled once the product before is done (that over the last tile's second half was before this tile's scores were)
+                if (half == 1) {
+                    ok = mbar_wait_warp(&half_done[g], j & 1, 17);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                }
+                if (__any_sync(0xffffffffu, rescale)) {        // rare
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_addr + c0, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * factor);
+                        tmem_st16(o_addr + c0, o);
+                    }
+                }
+                tmem_st_wait();
+                tcgen05_fence_before();
+                mbar_arrive(&p_full[2 * g + half]);
+            }
+        }
+        // ---- the rows' results ----------------------------------------------------------------------------------
+        if (ok && n_mine > 0) ok = mbar_wait_warp(&o_done[g], 0, 18);
+        if (ok && n_mine > 0) {
+            tcgen05_fence_after();
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            __nv_bfloat16* dst = p.out + row_at;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + c0, o);
+                tmem_ld_wait();
+                if (r < mine.rows) {
+                    uint4 u[2];
+                    __nv_bfloat162* b = (__nv_bfloat162*)u;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) b[q] = __floats2bfloat162_rn(__uint_as_float(o[2 * q]) * inv, __uint_as_float(o[2 * q + 1]) * inv);
+                    *(uint4*)(dst + c0) = u[0];
+                    *(uint4*)(dst + c0 + 8) = u[1];
+                }
+            }
+        }
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == PRODUCT) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem_base, TM_COLS);
+    }
+}
+
+}  // namespace
+
+// q, out: bf16 [total_rows, n_heads, hd]; the cache as cj_append_e4m3 writes it; rows req_start[r] .. req_start[r + 1] are request r's
+// from position req_prior[r] on.  hd: 64 or 128; scale > 0.  block_rows: query rows a block, 128 or 256 (0: by the size of the launch).
+CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, const void* vplane, const void* kexp, const void* vexp, int n_pages,
+                                 const int* req_start, const int* req_prior, int n_requests, int total_rows, const int* table, int table_stride,
+                                 int page_tokens, int n_heads, int n_kv, int hd, int window, float scale, int block_rows, int sms,
+                                 cudaStream_t stream) {
+    if (total_rows <= 0 || n_requests <= 0) return 0;
+    if (!q || !out || !kplane || !vplane || !kexp || !vexp || !req_start || !req_prior || !table) return CJ_ERR_ARG;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || n_pages <= 0 || window < 0 || !(scale > 0.0f)) return CJ_ERR_SIZE;
+    if (hd != 64 && hd != 128) return CJ_ERR_SIZE;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kplane | (uintptr_t)vplane) & 15) return CJ_ERR_ALIGN;
+    if ((long long)n_pages * n_kv * page_tokens > 0x7fffffffLL || (long long)table_stride * page_tokens > 0x7fffffffLL - 256) return CJ_ERR_SIZE;
+    if (block_rows != 128 && block_rows != 256) {
+        // 256 rows a block unless that leaves more than half of the SMs without one
+        const long long blocks = ((long long)(total_rows + 255) / 256 + n_requests - 1) * n_heads;
+        block_rows = 2 * blocks <= sms ? 128 : 256;
+    }
+    const long long row_blocks = ((long long)total_rows + block_rows - 1) / block_rows + n_requests;
+    if (row_blocks > 65535) return CJ_ERR_SIZE;
+    CUtensorMap map_q;
+    if (!make_map_bf16(&map_q, q, total_rows, (long long)n_heads * hd, (long long)n_heads * hd, BM)) return CJ_ERR_ARG;
+    const Args a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane, (const uint8_t*)vplane, (const uint8_t*)kexp,
+                 (const uint8_t*)vexp, req_start, req_prior, table, n_requests, table_stride, page_tokens, n_pages, n_heads, n_kv, window,
+                 scale * 1.4426950408889634f, total_rows, block_rows};
+    auto kern = hd == 128 ? prefill_e4m3_tc_kernel<128> : prefill_e4m3_tc_kernel<64>;
+    const int smem = hd == 128 ? Smem<128>::TOTAL : Smem<64>::TOTAL;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    cj::launch(kern, dim3(n_heads, (unsigned)row_blocks), dim3(THREADS), smem, stream, map_q, a);
+    return cj::launch_status();
+}
+
+CJ_EXPORT int cj_prefill_e4m3_tc_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, tc::g_error_flag, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}

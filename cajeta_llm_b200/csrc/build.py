@@ -53,12 +53,13 @@ LIBRARIES: Dict[str, str] = {
     "latent_prefill": "latent_prefill.cu",
     "stream_ops": "stream_ops.cu",
     "cache_e4m3": "cache_e4m3.cu",
+    "attention_e4m3_tc": "attention_e4m3_tc.cu",
     "gemm_q4": "gemm_q4.cu",
     "gemm_q4_tc": "gemm_q4_tc.cu",
 }
 HEADERS = ["common.cuh", "tc_common.cuh", "sampling_static.h"]
 # headers that only some libraries read
-OWN_HEADERS: Dict[str, List[str]] = {"cache_e4m3": ["e4m3.cuh"], "gemm_q4": ["q4.cuh"], "gemm_q4_tc": ["q4.cuh"]}
+OWN_HEADERS: Dict[str, List[str]] = {"cache_e4m3": ["e4m3.cuh"], "attention_e4m3_tc": ["e4m3.cuh"], "gemm_q4": ["q4.cuh"], "gemm_q4_tc": ["q4.cuh"]}
 
 # host-only libraries (no CUDA): compiled with the host C++ compiler, so that the books of the
 # cache manager also load on a machine without nvcc or a GPU

@@ -1686,7 +1686,7 @@ def wait_errors() -> Dict[str, int]:
     found = {}
     for name, symbol in (("gemm_tc", "cj_gemm_tc_error"), ("gemm_tc2", "cj_gemm_tc2_error"), ("gemm_f32_tc", "cj_gemm_f32_tc_error"),
                          ("attention_prefill_tc", "cj_prefill_attention_tc_error"), ("attention_flash_tc", "cj_attention_flash_tc_error"),
-                         ("gemm_q4_tc", "cj_gemm_q4_tc_error")):
+                         ("gemm_q4_tc", "cj_gemm_q4_tc_error"), ("attention_e4m3_tc", "cj_prefill_e4m3_tc_error")):
         lib = _libs.get(name)
         if lib is not None:
             code = int(getattr(lib, symbol)())
@@ -1759,7 +1759,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     _check(st, "rope_kv_write_e4m3")
 
 
-def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, what) -> None:
+def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, what) -> None:
     _need(q, "q", torch.bfloat16), _need(out, "out", torch.bfloat16), _need(table, "table", torch.int32)
     if head_dim not in (64, 128):
         raise KernelError(f"{what} takes heads of 64 or 128, not {head_dim}")
@@ -1769,8 +1769,8 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tok
         raise KernelError(f"{what}: q {tuple(q.shape)} and out {tuple(out.shape)} are not [rows, {n_heads}, {head_dim}]")
     if table.dim() != 2:
         raise KernelError(f"{what}: table must be [requests, pages]")
-    if window < 0:
-        raise KernelError(f"{what}: window must be positive (or 0 for none), found {window}")
+    if window < 0 or not scale > 0.0:
+        raise KernelError(f"{what}: window must be positive (or 0 for none) and scale positive, found {window} and {scale}")
     _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, what)
     _need_same_device(what, q, out, k_plane, v_plane, k_exp, v_exp, table)
 
@@ -1791,7 +1791,7 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
     ``rope_kv_write_e4m3`` writes: row t sees the positions from ``positions[t] + 1 - window`` (0 without a window) to
     ``positions[t]``.  A row of none of ``table``'s requests (-1) sees none: zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
     that share a row's keys (0: by the size of the launch; the results' last bits depend on it).  head_dim 64 or 128."""
-    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, "decode_attention_e4m3")
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, "decode_attention_e4m3")
     _need(positions, "positions", torch.int32), _need(row_req, "row_req", torch.int32)
     T = q.shape[0]
     if positions.numel() != T or row_req.numel() != T:
@@ -1815,6 +1815,9 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
         launches += 1                      # the merge kernel
 
 
+E4M3_ROW_BY_ROW = 32     # rows of a step of portions up to which they are taken one by one
+
+
 def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor,
                            v_exp: torch.Tensor, req_start: torch.Tensor, req_prior: torch.Tensor, table: torch.Tensor, page_tokens: int,
                            n_heads: int, n_kv: int, head_dim: int, window: int, scale: float) -> None:
@@ -1822,13 +1825,20 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     ``req_start[r]`` to ``req_start[r + 1]`` of q [T, heads, head_dim] (bfloat16) are request r's tokens from position
     ``req_prior[r]`` on, each sees its request's keys up to its own position, under a window the last ``window`` of them.  Rows of no
     request are left as they were.  head_dim 64 or 128."""
-    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, "prefill_attention_e4m3")
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, "prefill_attention_e4m3")
     _need(req_start, "req_start", torch.int32), _need(req_prior, "req_prior", torch.int32)
     R = req_prior.numel()
     if req_start.numel() != R + 1 or table.shape[0] < R:
         raise KernelError(f"prefill_attention_e4m3: req_start {tuple(req_start.shape)} and table {tuple(table.shape)} do not fit {R} requests")
     T = q.shape[0]
     if T == 0 or R == 0:
+        return
+    if T > E4M3_ROW_BY_ROW:
+        st = library("attention_e4m3_tc").cj_prefill_e4m3_tc(
+            _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(req_start), _ptr(req_prior),
+            _i(R), _i(T), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(n_heads), _i(n_kv), _i(head_dim), _i(window), _f(scale), _i(0),
+            _i(_sm_count()), _stream())
+        _check(st, "prefill_attention_e4m3")
         return
     st = library("cache_e4m3").cj_decode_e4m3(
         _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(None), _ptr(None),

@@ -203,7 +203,7 @@ class PagedAttention(Part):
         else:
             libs.add("attention_paged")
         if self.runtime.e4m3_cache:
-            libs.add("cache_e4m3")
+            libs |= {"cache_e4m3", "attention_e4m3_tc"}
         if self.runtime.q4_weights:
             libs |= {"gemm_q4", "gemm_q4_tc"}
         if "attention_paged" in libs and self.runtime.act_dtype == torch.float32:

@@ -86,7 +86,7 @@ EXPERTS = K.Q4Weight(torch.zeros(1, dtype=torch.uint8), (4, 70, 128), 64)
     (decode, dict(q=torch.zeros(3, 4, 64))), (decode, dict(out=torch.zeros(2, 4, 64, dtype=torch.bfloat16))), (decode, dict(head_dim=96)),
     (decode, dict(n_heads=3)), (decode, dict(n_kv=3)), (decode, dict(positions=i32(2))), (decode, dict(row_req=i32(2))), (decode, dict(table=i32(8))),
     (decode, dict(page_tokens=8)), (decode, dict(v_exp=torch.zeros(3, 2, 16, dtype=torch.int8))), (decode, dict(splits=-1)), (decode, dict(window=-1)),
-    (prefill, dict(req_start=i32(2))), (prefill, dict(table=i32(1, 4))), (prefill, dict(req_prior=torch.zeros(2))), (prefill, dict(window=-5)),
+    (prefill, dict(req_start=i32(2))), (prefill, dict(table=i32(1, 4))), (prefill, dict(req_prior=torch.zeros(2))), (prefill, dict(window=-5)), (prefill, dict(scale=0.0)),
     (product, dict(w=torch.zeros(70, 128))), (product, dict(a=torch.zeros(3, 128))), (product, dict(a=torch.zeros(128, 3, dtype=torch.bfloat16).T)),
     (product, dict(a=torch.zeros(3, 64, dtype=torch.bfloat16))), (product, dict(a=torch.zeros(4, 128, dtype=torch.bfloat16))),
     (product, dict(out=torch.zeros(3, 71))), (product, dict(out=torch.zeros(3, 70, dtype=torch.float16))),
