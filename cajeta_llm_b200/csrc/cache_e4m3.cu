@@ -11,8 +11,12 @@
 
 #include "common.cuh"
 #include "e4m3.cuh"
+#include "tc_common.cuh"
 
 using namespace cj;
+using tc::mbar_expect_tx;
+using tc::mbar_init;
+using tc::mbar_wait_warp;
 
 namespace {
 
@@ -115,43 +119,70 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Attention of single rows.  A block of four warps takes one row, the query heads of one kv head (up to ROWS at a time) and a
-// stretch of the row's keys; each warp walks over its 32-key pieces with a running softmax of its own, codes straight from
-// global memory into the registers that the products read (mma.sync m16n8k16, f16 in, float32 out: an e4m3 code is an f16 number
-// exactly).  The order of a product's K is free as long as both operands keep it: a lane's share of a key is 32 neighbouring
-// bytes, and its share of a value row 16, so every load is 16 bytes and no shared memory lies between.
+// stretch of the row's keys; each warp walks over its 32-key pieces with a running softmax of its own and a ring of shared memory of its
+// own, filled by bulk copies of a page's run of rows a step ahead (registers that loads are on their way to would make every shuffle and
+// exponential wait for them).  The codes go into the products as they are: both are of e4m3 numbers (mma.sync m16n8k32, float32 out), the other operand cut into two of them.  A bfloat16 query is exactly a number of four significant bits plus one of
+// four; a weight p is one plus one and a rest of at most 2^-8 p (measured on random rows: 7e-4 of the result, half of what one rounding to
+// bfloat16 leaves).  Up to eight heads take rows 0 .. 7 of a product with their first parts and rows 8 .. 15 with their second.
 //     S = q . code_k          rows: heads, columns: keys          s = S scale 2^e_k
-//     O = (p 2^(e_v - R)) . code_v   with R the largest exponent of the values so far: the weights stay at most 1 in f16
-// Queries come as bfloat16 and are brought to [2^10, 2^11) at their largest entry by a power of two, so that f16 holds all eight
-// bits of every entry down to 2^-24 of the largest.  Bound by DRAM: 2 (HD + 1) bytes a key.
+//     O = (p 2^(e_v - R)) . code_v   with R the largest exponent of the values so far
+// The order of a product's K is free as long as both operands keep it: a lane's share of a key is HD / 4 neighbouring bytes and of
+// four value rows HD / 8 each (turned by byte permutes: four keys of an entry side by side).
+// Queries are brought to [2^7, 2^8) at their largest entry by a power of two: an entry's parts keep its bits down to 2^-21 of that.
+// Weights lie under 2^8: their parts keep what is above 2^-22 of the largest so far (times the values' powers of two).
+// Bound by DRAM: 2 (HD + 1) bytes a key.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
 constexpr int STEP = 32;                   // keys of a warp's step
+constexpr int STAGES = 2, BLOCKS = 3;      // steps of a warp's ring, blocks an SM
 
-template <int ROWS>
-__device__ __forceinline__ void mma_f16(float (&c)[ROWS == 16 ? 4 : 2], float (&idle)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                        uint32_t b0, uint32_t b1) {
-    float& c2 = ROWS == 16 ? c[ROWS == 16 ? 2 : 0] : idle[0];
-    float& c3 = ROWS == 16 ? c[ROWS == 16 ? 3 : 1] : idle[1];
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c2), "+f"(c3)
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the codes nearest to lo and hi (in that order), and what they leave
+__device__ __forceinline__ uint32_t first_part(float& lo, float& hi) {
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
+    const float2 f = __half22float2(*(const __half2*)&h);
+    lo -= f.x;
+    hi -= f.y;
+    return c;
+}
+__device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
+    return c;
 }
 
 template <int HD, int ROWS>
-__global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : 3) decode_e4m3_kernel(
+__global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4m3_kernel(
     const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const uint8_t* __restrict__ kplane, const uint8_t* __restrict__ vplane,
     const uint8_t* __restrict__ kexp, const uint8_t* __restrict__ vexp, const int* __restrict__ positions, const int* __restrict__ row_req,
     const int* __restrict__ req_start, const int* __restrict__ req_prior, int n_requests, const int* __restrict__ table, int table_stride,
-    int page_tokens, int n_pages, int n_heads, int n_kv, int head_batches, int window, float scale_log2, int splits, float* __restrict__ part_acc, float* __restrict__ part_ml) {
-    constexpr int NR = ROWS / 8;           // rows of a fragment a lane holds: g, and g + 8
-    constexpr int QS = HD / 16;            // steps of 16 of the head's entries
-    constexpr int KW = HD / 16;            // words of a key a lane holds
+    int page_tokens, int page_shift, int n_pages, int n_heads, int n_kv, int head_batches, int window, float scale_log2, int splits,
+    float* __restrict__ part_acc, float* __restrict__ part_ml) {
+    constexpr int NR = ROWS / 8;           // heads a lane's fragments hold: g (and g + 8)
+    constexpr int QS = HD / 32;            // steps of 32 of the head's entries
+    constexpr int KW = HD / 16;            // words of a key that are a lane's
+    constexpr int VW = HD / 32;            // words of a value row a lane holds
     constexpr int NT = HD / 8;             // column tiles of the output
     cj::after_predecessor();
     cj::release_successor();
-    __shared__ float red[WARPS][ROWS][HD + 4];
+    extern __shared__ __align__(128) uint8_t ring[];                   // [WARPS][STAGES][keys, values][STEP][HD], then the warps' results
+    float (*red)[ROWS][HD + 4] = (float (*)[ROWS][HD + 4])ring;
     __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS];
     __shared__ int sr[WARPS];
+    __shared__ uint64_t bars[WARPS][STAGES];
     const int t = blockIdx.x, split = blockIdx.z;
     const int kvh = blockIdx.y / head_batches, hb = blockIdx.y % head_batches;
     const int group = n_heads / n_kv, h0 = kvh * group + hb * ROWS, n_h = min(ROWS, group - hb * ROWS);
@@ -176,159 +207,255 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : 3) decode_e4m3_ke
     const int first = from + split * per, last = min(p + 1, first + per);
     const int* tab = table + (size_t)max(req, 0) * table_stride;
 
-    uint32_t qa[QS][2 * NR];
+    // Lane j looks up key j of a step: its page two steps before the products, from it the key's row in the planes (-1: none) and its exponents one
+    // step before; the first lane of every run of keys that lie side by side in a page copies the run's codes.
+    uint64_t* bar = bars[warp];
+    if (lane < STAGES) mbar_init(&bar[lane], 1);
+    tc::fence_barrier_init();
+    __syncwarp();
+    const uint32_t mine = tc::smem_u32(ring) + warp * STAGES * 2 * STEP * HD;
+    int page = -1, at_page = 0, k_next = 0, v_next = 0;      // (exponents + 127; v_next below 0: no key)
+    auto ask_page = [&](int k0) {
+        const int key = k0 + lane, n = page_shift >= 0 ? key >> page_shift : key / page_tokens;
+        at_page = key - n * page_tokens;
+        page = key < last ? __ldg(tab + n) : -1;
+    };
+    auto ask = [&](int k0, int stage) {
+        const bool there = page >= 0 && page < n_pages;
+        const long long row = there ? ((long long)page * n_kv + kvh) * page_tokens + at_page : 0;
+        const uint32_t have = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) mbar_expect_tx(&bar[stage], __popc(have) * 2 * HD);
+        __syncwarp();
+        if (there && (lane == 0 || at_page == 0)) {
+            const uint32_t n = min(min(page_tokens - at_page, STEP - lane), last - (k0 + lane)) * HD;
+            const uint32_t dst = mine + (stage * 2 * STEP + lane) * HD;
+            bulk_load(dst, kplane + row * HD, n, &bar[stage]);
+            bulk_load(dst + STEP * HD, vplane + row * HD, n, &bar[stage]);
+        }
+        k_next = there ? (int)kexp[row] : 0;
+        v_next = there ? (int)vexp[row] : -1;
+    };
+    int k0 = first + warp * STEP;
+    constexpr int STRIDE = WARPS * STEP;
+    ask_page(k0);
+    if (k0 < last) ask(k0, 0);
+    ask_page(k0 + STRIDE);
+
+    // the queries' two parts; qa[i]: heads g and g + 8 (or g's second parts), entries t4 HD / 4 + 8 i + {0 .. 3} and {4 .. 7}
+    uint32_t qa[NR][QS][4];
     float back[NR];                        // what undoes the queries' power of two, with the scale in units of log 2
+    {
+        uint32_t hi[NR][QS][2], lo[NR][QS][2];
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        uint32_t w[2 * QS];
-        const int head = g + 8 * r;
+        for (int r = 0; r < NR; ++r) {
+            uint32_t w[4 * QS];
+            const int head = g + 8 * r;
 #pragma unroll
-        for (int i = 0; i < QS / 2; ++i) {
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (head < n_h) u = *(const uint4*)(q + ((size_t)t * n_heads + h0 + head) * HD + t4 * (HD / 4) + i * 8);
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            for (int i = 0; i < QS; ++i) {
+                uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                if (head < n_h) u = *(const uint4*)(q + ((size_t)t * n_heads + h0 + head) * HD + t4 * (HD / 4) + i * 8);
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            }
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4 * QS; ++i) most = fmaxf(most, fmaxf(fabsf(bf16_low(w[i])), fabsf(bf16_high(w[i]))));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int e = query_exponent(most);
+            const float up = power_of_two(e);
+            back[r] = most < INFINITY ? scale_log2 * power_of_two(-e) : NAN;      // (a code would cut it to 448)
+#pragma unroll
+            for (int i = 0; i < QS; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x0 = bf16_low(w[4 * i + 2 * j]) * up, x1 = bf16_high(w[4 * i + 2 * j]) * up;
+                    float x2 = bf16_low(w[4 * i + 2 * j + 1]) * up, x3 = bf16_high(w[4 * i + 2 * j + 1]) * up;
+                    hi[r][i][j] = first_part(x0, x1) | first_part(x2, x3) << 16;
+                    lo[r][i][j] = codes_of(x0 * 16.0f, x1 * 16.0f) | codes_of(x2 * 16.0f, x3 * 16.0f) << 16;
+                }
         }
-        float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2 * QS; ++i) most = fmaxf(most, fmaxf(fabsf(bf16_low(w[i])), fabsf(bf16_high(w[i]))));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = query_exponent(most);
-        const float up = power_of_two(e);
-        back[r] = scale_log2 * power_of_two(-e);
+        for (int i = 0; i < QS; ++i)
 #pragma unroll
-        for (int i = 0; i < QS; ++i) {
-            qa[i][r] = pack_f16(bf16_low(w[2 * i]) * up, bf16_high(w[2 * i]) * up);
-            qa[i][NR + r] = pack_f16(bf16_low(w[2 * i + 1]) * up, bf16_high(w[2 * i + 1]) * up);
-        }
+            for (int j = 0; j < 2; ++j) {
+                qa[0][i][2 * j] = hi[0][i][j];
+                qa[0][i][2 * j + 1] = NR == 2 ? hi[NR - 1][i][j] : lo[0][i][j];
+                if (NR == 2) qa[NR - 1][i][2 * j] = lo[0][i][j], qa[NR - 1][i][2 * j + 1] = lo[NR - 1][i][j];
+            }
     }
 
-    float o[NT][ROWS == 16 ? 4 : 2], idle[2] = {0.0f, 0.0f};
+    float o[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int e = 0; e < 2 * NR; ++e) o[i][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
     float m[NR], l[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
-    int R = -1000;
+    int R = 0;                             // + 127
 
-    for (int k0 = first + warp * STEP; k0 < last; k0 += WARPS * STEP) {
-        // lane j looks up key j: its row in the planes (-1: none) and its two exponents
-        const int key = k0 + lane;
-        int row = -1;
-        if (key < last) {
-            const int page = tab[key / page_tokens];
-            if (page >= 0 && page < n_pages) row = (page * n_kv + kvh) * page_tokens + key % page_tokens;
+    uint32_t phase = 0;
+    for (int stage = 0; k0 < last; k0 += STRIDE) {
+        const int k_exp = k_next, v_exp = v_next;
+        const bool more = k0 + STRIDE < last;
+        if (more) {
+            ask(k0 + STRIDE, stage ^ 1);
+            ask_page(k0 + 2 * STRIDE);
         }
-        uint32_t kw[4][KW];
+        if (!mbar_wait_warp(&bar[stage], phase, 21)) {
+            if (more) mbar_wait_warp(&bar[stage ^ 1], phase ^ stage, 22);        // (the copies end before the block does)
+            break;
+        }
+        const uint8_t* keys = ring + (warp * STAGES + stage) * 2 * STEP * HD;
+        const uint8_t* values = keys + STEP * HD;
+        const uint32_t there = __ballot_sync(0xffffffffu, v_exp >= 0);
+        // ---- scores: s[b][2 r + e] of head g + 8 r and key 8 b + 2 t4 + e
+        float s[4][2 * NR];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            const int at = __shfl_sync(0xffffffffu, row, b * 8 + g);
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < KW / 4; ++i) {
-                uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (at >= 0) u = ldg_stream(kplane + (size_t)at * HD + t4 * (HD / 4) + i * 16);
-                kw[b][4 * i] = u.x, kw[b][4 * i + 1] = u.y, kw[b][4 * i + 2] = u.z, kw[b][4 * i + 3] = u.w;
-            }
-        }
-        const int ek = row >= 0 ? (int)kexp[row] - 127 : 0, ev = row >= 0 ? (int)vexp[row] - 127 : -1000;
-        // the values of this lane's keys: 16 u + {2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4}, entries [g HD / 8, (g + 1) HD / 8)
-        uint32_t vw[2][4][HD / 32];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = __shfl_sync(0xffffffffu, row, u * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1));
-                const uint8_t* src = vplane + (size_t)max(at, 0) * HD + g * (HD / 8);
-                if (HD == 128) {
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (at >= 0) x = ldg_stream(src);
-                    vw[u][i][0] = x.x, vw[u][i][1] = x.y, vw[u][i][HD / 32 - 2] = x.z, vw[u][i][HD / 32 - 1] = x.w;
-                } else {
-                    uint2 x = make_uint2(0u, 0u);
-                    if (at >= 0) x = __ldg((const uint2*)src);
-                    vw[u][i][0] = x.x, vw[u][i][1] = x.y;
+                const uint4 k = *(const uint4*)(keys + (b * 8 + g) * HD + t4 * (HD / 4) + i * 16);
+                mma_e4m3(c, qa[0][2 * i], k.x, k.y);
+                mma_e4m3(c, qa[0][2 * i + 1], k.z, k.w);
+                if (NR == 2) {
+                    mma_e4m3(d, qa[NR - 1][2 * i], k.x, k.y);
+                    mma_e4m3(d, qa[NR - 1][2 * i + 1], k.z, k.w);
                 }
             }
-
-        // ---- scores: s[b][0, 1] of head g and keys 8 b + 2 t4 + {0, 1}, s[b][2, 3] of head g + 8
-        float s[4][ROWS == 16 ? 4 : 2];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-#pragma unroll
-            for (int e = 0; e < 2 * NR; ++e) s[b][e] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < QS; ++i) {
-                uint32_t b0, b1;
-                e4m3x4_to_f16(kw[b][i], b0, b1);
-                mma_f16<ROWS>(s[b], idle, qa[i][0], NR == 2 ? qa[i][NR - 1] : 0u, qa[i][NR], NR == 2 ? qa[i][2 * NR - 1] : 0u, b0, b1);
+            for (int e = 0; e < 2; ++e) {
+                s[b][e] = fmaf(NR == 2 ? d[e] : c[2 + e], 0.0625f, c[e]);
+                if (NR == 2) s[b][2 * NR - 2 + e] = fmaf(d[2 + e], 0.0625f, c[2 + e]);
             }
         }
+        // in units of the scores' own scale until the exponential: m is the largest so far times that scale
+        const float kf = __int_as_float(k_exp << 23);
         float mx[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) mx[r] = m[r];
-        const float kf = power_of_two(ek);
+        for (int r = 0; r < NR; ++r) mx[r] = -INFINITY;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float f = __shfl_sync(0xffffffffu, kf, b * 8 + 2 * t4 + e);
-                const bool in = __shfl_sync(0xffffffffu, row, b * 8 + 2 * t4 + e) >= 0;
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    const float v = in ? s[b][2 * r + e] * back[r] * f : -INFINITY;
-                    s[b][2 * r + e] = v;
-                    mx[r] = fmaxf(mx[r], v);
-                }
+                for (int r = 0; r < NR; ++r) s[b][2 * r + e] *= f;
             }
-        const int most = max(R, __reduce_max_sync(0xffffffffu, ev));
-        float old[NR], use[NR];
+        if (there != 0xffffffffu) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (!(there >> (b * 8 + 2 * t4 + e) & 1))
+#pragma unroll
+                        for (int r = 0; r < NR; ++r) s[b][2 * r + e] = -INFINITY;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) mx[r] = fmaxf(mx[r], s[b][2 * r + e]);
+        const int most = max(R, __reduce_max_sync(0xffffffffu, v_exp));
+        bool moved = most != R;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-            use[r] = mx[r] == -INFINITY ? 0.0f : mx[r];
-            old[r] = exp2f(m[r] - use[r]);
-            l[r] *= old[r];
-            m[r] = mx[r];
-            old[r] *= power_of_two(max(R - most, -126));
+            mx[r] = fmaxf(m[r], mx[r] * back[r]);
+            moved = moved || mx[r] != m[r];
         }
-        R = most;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int e = 0; e < 2 * NR; ++e) o[i][e] *= old[e >> 1];
-        const float vf = power_of_two(max(ev - R, -126));
-        uint32_t pa[4][NR];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const float f0 = __shfl_sync(0xffffffffu, vf, b * 8 + 2 * t4), f1 = __shfl_sync(0xffffffffu, vf, b * 8 + 2 * t4 + 1);
+        if (__any_sync(0xffffffffu, moved)) {
+            const float down = power_of_two(max(R - most, -126));
+            float old[NR];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                const float p0 = exp2f(s[b][2 * r] - use[r]), p1 = exp2f(s[b][2 * r + 1] - use[r]);
-                l[r] += p0 + p1;
-                pa[b][r] = pack_f16(p0 * f0, p1 * f1);
+                old[r] = mx[r] == -INFINITY ? 1.0f : ex2(m[r] - mx[r]);
+                l[r] *= old[r];
+                old[r] *= down;
+                m[r] = mx[r];
+            }
+            R = most;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] *= old[NR == 2 ? e >> 1 : 0];
+        }
+        // ---- weights: their parts as the first operand of one product (up to eight heads: both) or two.  (At most 2^8: a code goes to 448)
+        const float vf = power_of_two(max(v_exp - R + 8, -126));
+        uint32_t hi[NR][2], lo[NR][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = __shfl_sync(0xffffffffu, vf, (2 * u + (j >> 1)) * 8 + 2 * t4 + (j & 1));
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const float sub = m[r] == -INFINITY ? 0.0f : -m[r];
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float w = ex2(fmaf(s[2 * u + (j >> 1)][2 * r + (j & 1)], back[r], sub));
+                    l[r] += w;
+                    x[j] = w * f[j];
+                }
+                hi[r][u] = first_part(x[0], x[1]) | first_part(x[2], x[3]) << 16;
+                if (NR == 2) lo[r][u] = codes_of(x[0], x[1]) | codes_of(x[2], x[3]) << 16;
+                else lo[r][u] = codes_of(x[0] * 16.0f, x[1] * 16.0f) | codes_of(x[2] * 16.0f, x[3] * 16.0f) << 16;
             }
         }
-        // ---- values: column tile i holds entries g HD / 8 + i of the eight g
+        const uint32_t pa[4] = {hi[0][0], NR == 2 ? hi[NR - 1][0] : lo[0][0], hi[0][1], NR == 2 ? hi[NR - 1][1] : lo[0][1]};
+        const uint32_t pb[4] = {lo[0][0], lo[NR - 1][0], lo[0][1], lo[NR - 1][1]};
+        // ---- values: column tile i holds entries g HD / 8 + i of the eight g; four keys of an entry to a word
+        uint32_t vw[2][4][VW];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {
-                uint32_t lo01 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x5140), lo23 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x7362);
-                uint32_t hi01 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x5140), hi23 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x7362);
-                uint32_t b0[4], b1[4];
-                e4m3x4_to_f16(lo01, b0[0], b0[1]);
-                e4m3x4_to_f16(lo23, b0[2], b0[3]);
-                e4m3x4_to_f16(hi01, b1[0], b1[1]);
-                e4m3x4_to_f16(hi23, b1[2], b1[3]);
+            for (int i = 0; i < 4; ++i) {
+                const int row = u * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1);
+                if (HD == 128) {
+                    const uint4 x = *(const uint4*)(values + row * HD + g * 16);
+                    vw[u][i][0] = x.x, vw[u][i][1] = x.y, vw[u][i][VW - 2] = x.z, vw[u][i][VW - 1] = x.w;
+                } else {
+                    const uint2 x = *(const uint2*)(values + row * HD + g * 8);
+                    vw[u][i][0] = x.x, vw[u][i][1] = x.y;
+                }
+            }
+        if (there != 0xffffffffu) {
+            // rows of no key hold what was there before
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    mma_f16<ROWS>(o[4 * w + i], idle, pa[2 * u][0], NR == 2 ? pa[2 * u][NR - 1] : 0u, pa[2 * u + 1][0],
-                                  NR == 2 ? pa[2 * u + 1][NR - 1] : 0u, b0[i], b1[i]);
+                    if (!(there >> (u * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) & 1))
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vw[u][i][w] = 0;
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+            uint32_t b[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t x01 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x5140), x23 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x5140);
+                const uint32_t y01 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x7362), y23 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x7362);
+                b[u][0] = __byte_perm(x01, x23, 0x5410);
+                b[u][1] = __byte_perm(x01, x23, 0x7632);
+                b[u][2] = __byte_perm(y01, y23, 0x5410);
+                b[u][3] = __byte_perm(y01, y23, 0x7632);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                mma_e4m3(o[4 * w + i], pa, b[0][i], b[1][i]);
+                if (NR == 2) mma_e4m3(o[4 * w + i], pb, b[0][i], b[1][i]);
+            }
+        }
+        __syncwarp();                      // (every lane has read this step's stage)
+        phase ^= stage;
+        stage ^= 1;
     }
+    __syncthreads();                       // the ring becomes the results' place
 
     // ---- the four warps' results, added in their order
 #pragma unroll
@@ -338,11 +465,11 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : 3) decode_e4m3_ke
         if (t4 == 0) sm[warp][g + 8 * r] = m[r], sl[warp][g + 8 * r] = l[r];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            red[warp][g + 8 * r][2 * t4 * NT + i] = o[i][2 * r];
-            red[warp][g + 8 * r][(2 * t4 + 1) * NT + i] = o[i][2 * r + 1];
+            red[warp][g + 8 * r][2 * t4 * NT + i] = NR == 2 ? o[i][2 * r] : fmaf(o[i][2], 0.0625f, o[i][0]);
+            red[warp][g + 8 * r][(2 * t4 + 1) * NT + i] = NR == 2 ? o[i][2 * r + 1] : fmaf(o[i][3], 0.0625f, o[i][1]);
         }
     }
-    if (lane == 0) sr[warp] = R;
+    if (lane == 0) sr[warp] = R - 127 - 8;
     __syncthreads();
     for (int i = tid; i < n_h * (HD / 2); i += WARPS * 32) {
         const int row = i / (HD / 2), d = 2 * (i % (HD / 2));
@@ -445,7 +572,7 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
     if (!q || !out || !kplane || !vplane || !kexp || !vexp || !table) return CJ_ERR_ARG;
     if (positions ? !row_req : (!req_start || !req_prior || splits != 1)) return CJ_ERR_ARG;
     if (splits < 1 || (splits > 1 && (!part_acc || !part_ml))) return CJ_ERR_ARG;
-    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || window < 0 || n_requests <= 0 || n_pages <= 0) return CJ_ERR_SIZE;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || window < 0 || n_requests <= 0 || n_pages <= 0 || !(scale > 0.0f)) return CJ_ERR_SIZE;
     if (hd != 64 && hd != 128) return CJ_ERR_SIZE;
     if (((uintptr_t)q | (uintptr_t)kplane | (uintptr_t)vplane) & 15) return CJ_ERR_ALIGN;
     if ((uintptr_t)out & 3) return CJ_ERR_ALIGN;
@@ -455,9 +582,12 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
     const dim3 grid(T, n_kv * head_batches, splits);
     auto kern = hd == 128 ? (rows == 8 ? decode_e4m3_kernel<128, 8> : decode_e4m3_kernel<128, 16>)
                           : (rows == 8 ? decode_e4m3_kernel<64, 8> : decode_e4m3_kernel<64, 16>);
-    cj::launch(kern, dim3(grid), dim3(WARPS * 32), 0, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane,
+    const int smem = max(WARPS * STAGES * 2 * STEP * hd, WARPS * rows * (hd + 4) * 4);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    cj::launch(kern, dim3(grid), dim3(WARPS * 32), smem, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane,
                (const uint8_t*)vplane, (const uint8_t*)kexp, (const uint8_t*)vexp, positions, row_req, req_start, req_prior, n_requests, table,
-               table_stride, page_tokens, n_pages, n_heads, n_kv, head_batches, window, scale * 1.4426950408889634f, splits, part_acc, part_ml);
+               table_stride, page_tokens, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, n_pages, n_heads, n_kv, head_batches, window, scale * 1.4426950408889634f, splits, part_acc, part_ml);
     if (splits > 1) {
         const int status = launch_status();
         if (status != 0) return status;
@@ -466,4 +596,10 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
         cj::launch(merge, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, stream, (__nv_bfloat16*)out, (const float*)part_acc, (const float*)part_ml, n, splits);
     }
     return launch_status();
+}
+
+CJ_EXPORT int cj_cache_e4m3_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, tc::g_error_flag, sizeof(int)) != cudaSuccess) return -1;
+    return v;
 }

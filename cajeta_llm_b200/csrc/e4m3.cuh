@@ -19,19 +19,21 @@ __device__ __forceinline__ int block_exponent(float most) {
     return min(max(e, -100), 119);
 }
 
-// The power of two that brings the largest entry of a query head to [2^10, 2^11) (0 entries, and what is beyond float32's reach
+// The power of two that brings the largest entry of a query head to [2^7, 2^8) (0 entries, and what is beyond float32's reach
 // after it, keep a finite one)
 __device__ __forceinline__ int query_exponent(float most) {
-    const int e = 10 - ((int)(__float_as_uint(most) >> 23) - 127);
+    const int e = 7 - ((int)(__float_as_uint(most) >> 23) - 127);
     return min(max(e, -100), 100);
 }
 
 __device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *(const uint32_t*)&v;
+// 2^x, 0 for -inf (relative error 2^-22)
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // four codes as two pairs of f16 (every e4m3 number is an f16 number)

@@ -1686,7 +1686,8 @@ def wait_errors() -> Dict[str, int]:
     found = {}
     for name, symbol in (("gemm_tc", "cj_gemm_tc_error"), ("gemm_tc2", "cj_gemm_tc2_error"), ("gemm_f32_tc", "cj_gemm_f32_tc_error"),
                          ("attention_prefill_tc", "cj_prefill_attention_tc_error"), ("attention_flash_tc", "cj_attention_flash_tc_error"),
-                         ("gemm_q4_tc", "cj_gemm_q4_tc_error"), ("attention_e4m3_tc", "cj_prefill_e4m3_tc_error")):
+                         ("gemm_q4_tc", "cj_gemm_q4_tc_error"), ("attention_e4m3_tc", "cj_prefill_e4m3_tc_error"),
+                         ("cache_e4m3", "cj_cache_e4m3_error")):
         lib = _libs.get(name)
         if lib is not None:
             code = int(getattr(lib, symbol)())

@@ -62,10 +62,10 @@ def attention(q, rows, k, v, table, page_tokens, kv, window, scale):
     return out, size
 
 
-def close(got, want, size, weights=2.0 ** -11):
-    # the result's rounding, the weights' rounding (single rows: to f16, 2^-11 of each; portions: to bfloat16, 2^-8), and 2^-12 for
-    # exponentials of float32 scores
-    worst = ((got.to(F64) - want).abs() - HALF * want.abs() - (weights + 2.0 ** -12) * size).max()
+def close(got, want, size):
+    # the result's rounding, the weights' (portions: to bfloat16, 2^-8 of each; single rows: a rest of 2^-4 is rounded to 2^-4 of itself),
+    # and 2^-12 for exponentials of float32 scores
+    worst = ((got.to(F64) - want).abs() - HALF * want.abs() - (2.0 ** -8 + 2.0 ** -12) * size).max()
     assert float(worst) <= 1e-30, float(worst)
 
 
@@ -206,7 +206,7 @@ def test_values_of_far_apart_exponents_and_unseen_nan():
         qs = torch.randn((n, heads, hd), device=DEV).to(torch.bfloat16)
         K.prefill_attention_e4m3(qs, many, k, v, ke, ve, ints([0, n]), ints([0]), table, P, heads, kv, hd, 0, 0.05)
         want, size = attention(qs, [(0, p) for p in range(n)], ks, vs, table, P, kv, 0, 0.05)
-        close(many, want, size, HALF)
+        close(many, want, size)
 
 
 # ---- portions of prompts ------------------------------------------------------------------------------------------------
@@ -241,7 +241,7 @@ def test_portions_of_prompts(heads, kv, hd, page_tokens, window, portions):
                              hd, window, scale)
     assert (out[len(rows):] == 7.0).all()                                       # rows of no request are left as they were
     want, size = attention(q[:len(rows)], rows, stands_for(k, ke), stands_for(v, ve), table, page_tokens, kv, window, scale)
-    close(out[:len(rows)], want, size, HALF)
+    close(out[:len(rows)], want, size)
     assert not K.wait_errors()
 
 
@@ -290,4 +290,4 @@ def test_another_stream_than_the_default_one():
         K.prefill_attention_e4m3(q, out, k, v, ke, ve, ints([0, 40]), ints([60]), table, P, heads, kv, hd, 0, 0.1)
     side.synchronize()
     want, size = attention(q, [(0, 60 + i) for i in range(40)], stands_for(k, ke), stands_for(v, ve), table, P, kv, 0, 0.1)
-    close(out, want, size, HALF)
+    close(out, want, size)
