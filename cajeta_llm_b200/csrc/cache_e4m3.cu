@@ -121,15 +121,15 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 // Attention of single rows.  A block of four warps takes one row, the query heads of one kv head (up to ROWS at a time) and a
 // stretch of the row's keys; each warp walks over its 32-key pieces with a running softmax of its own and a ring of shared memory of its
 // own, filled by bulk copies of a page's run of rows a step ahead (registers that loads are on their way to would make every shuffle and
-// exponential wait for them).  The codes go into the products as they are: both are of e4m3 numbers (mma.sync m16n8k32, float32 out), the other operand cut into two of them.  A bfloat16 query is exactly a number of four significant bits plus one of
-// four; a weight p is one plus one and a rest of at most 2^-8 p (measured on random rows: 7e-4 of the result, half of what one rounding to
-// bfloat16 leaves).  Up to eight heads take rows 0 .. 7 of a product with their first parts and rows 8 .. 15 with their second.
-//     S = q . code_k          rows: heads, columns: keys          s = S scale 2^e_k
-//     O = (p 2^(e_v - R)) . code_v   with R the largest exponent of the values so far
-// The order of a product's K is free as long as both operands keep it: a lane's share of a key is HD / 4 neighbouring bytes and of
-// four value rows HD / 8 each (turned by byte permutes: four keys of an entry side by side).
-// Queries are brought to [2^7, 2^8) at their largest entry by a power of two: an entry's parts keep its bits down to 2^-21 of that.
-// Weights lie under 2^8: their parts keep what is above 2^-22 of the largest so far (times the values' powers of two).
+// exponential wait for them).  An e4m3 code is an f16 number exactly: the products are mma.sync m16n8k16 of f16 numbers, float32 out, with the codes
+// as their first operand, so that all 16 rows of a product are keys (or entries) and its columns the heads.  (mma.sync takes e4m3 operands
+// too, but this GPU has no such instruction: 32 of them a step were 64 f16 products, 190 conversions and 150 additions, 80 us where this takes 60.)
+//     S^T = code_k . q^T                              s = S scale 2^e_k
+//     O^T = code_v^T . (p 2^(e_v - R))^T              R: the largest exponent of the values so far; the weights are at most 1 in f16
+// The order of a product's K, and of its rows, is free as long as both sides keep it: a lane's share of a key is HD / 4 neighbouring bytes and
+// of four value rows HD / 8 each (two keys' bytes side by side after a byte permute), 8- and 16-byte loads.  The weights turn from S^T's layout
+// into an operand by movmatrix.  Queries are brought to [2^7, 2^8) at their largest entry by a power of two: f16 keeps an entry's eight
+// bits down to 2^-21 of that.
 // Bound by DRAM: 2 (HD + 1) bytes a key.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
@@ -141,27 +141,19 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-// the codes nearest to lo and hi (in that order), and what they leave
-__device__ __forceinline__ uint32_t first_part(float& lo, float& hi) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-    const float2 f = __half22float2(*(const __half2*)&h);
-    lo -= f.x;
-    hi -= f.y;
-    return c;
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {      // an 8 x 8 matrix of f16, two of a row a lane
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
-__device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(hi), "f"(lo));
-    return c;
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *(const uint32_t*)&v;
 }
 
 template <int HD, int ROWS>
@@ -171,11 +163,10 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
     const int* __restrict__ req_start, const int* __restrict__ req_prior, int n_requests, const int* __restrict__ table, int table_stride,
     int page_tokens, int page_shift, int n_pages, int n_heads, int n_kv, int head_batches, int window, float scale_log2, int splits,
     float* __restrict__ part_acc, float* __restrict__ part_ml) {
-    constexpr int NR = ROWS / 8;           // heads a lane's fragments hold: g (and g + 8)
-    constexpr int QS = HD / 32;            // steps of 32 of the head's entries
-    constexpr int KW = HD / 16;            // words of a key that are a lane's
-    constexpr int VW = HD / 32;            // words of a value row a lane holds
-    constexpr int NT = HD / 8;             // column tiles of the output
+    constexpr int NB = ROWS / 8;           // column tiles of eight heads
+    constexpr int QS = HD / 16;            // steps of 16 of the head's entries, and words of a key that are a lane's
+    constexpr int VW = HD / 32;            // words of a value row that are a lane's
+    constexpr int NT = HD / 16;            // row tiles of the output
     cj::after_predecessor();
     cj::release_successor();
     extern __shared__ __align__(128) uint8_t ring[];                   // [WARPS][STAGES][keys, values][STEP][HD], then the warps' results
@@ -241,57 +232,47 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
     if (k0 < last) ask(k0, 0);
     ask_page(k0 + STRIDE);
 
-    // the queries' two parts; qa[i]: heads g and g + 8 (or g's second parts), entries t4 HD / 4 + 8 i + {0 .. 3} and {4 .. 7}
-    uint32_t qa[NR][QS][4];
-    float back[NR];                        // what undoes the queries' power of two, with the scale in units of log 2
-    {
-        uint32_t hi[NR][QS][2], lo[NR][QS][2];
+    // the queries of heads g (and g + 8), entries t4 HD / 4 + 4 i + {0, 1} and {2, 3}; of heads 2 t4 and 2 t4 + 1 (and 8 more), what undoes
+    // their power of two, with the scale in units of log 2
+    uint32_t qb[NB][QS][2];
+    float back[NB][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            uint32_t w[4 * QS];
-            const int head = g + 8 * r;
+    for (int n = 0; n < NB; ++n) {
+        uint32_t w[2 * QS];
+        const int head = g + 8 * n;
 #pragma unroll
-            for (int i = 0; i < QS; ++i) {
-                uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (head < n_h) u = *(const uint4*)(q + ((size_t)t * n_heads + h0 + head) * HD + t4 * (HD / 4) + i * 8);
-                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-            }
-            float most = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4 * QS; ++i) most = fmaxf(most, fmaxf(fabsf(bf16_low(w[i])), fabsf(bf16_high(w[i]))));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int e = query_exponent(most);
-            const float up = power_of_two(e);
-            back[r] = most < INFINITY ? scale_log2 * power_of_two(-e) : NAN;      // (a code would cut it to 448)
-#pragma unroll
-            for (int i = 0; i < QS; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float x0 = bf16_low(w[4 * i + 2 * j]) * up, x1 = bf16_high(w[4 * i + 2 * j]) * up;
-                    float x2 = bf16_low(w[4 * i + 2 * j + 1]) * up, x3 = bf16_high(w[4 * i + 2 * j + 1]) * up;
-                    hi[r][i][j] = first_part(x0, x1) | first_part(x2, x3) << 16;
-                    lo[r][i][j] = codes_of(x0 * 16.0f, x1 * 16.0f) | codes_of(x2 * 16.0f, x3 * 16.0f) << 16;
-                }
+        for (int i = 0; i < QS / 2; ++i) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (head < n_h) u = *(const uint4*)(q + ((size_t)t * n_heads + h0 + head) * HD + t4 * (HD / 4) + i * 8);
+            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
         }
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * QS; ++i) most = fmaxf(most, fmaxf(fabsf(bf16_low(w[i])), fabsf(bf16_high(w[i]))));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = query_exponent(most);
+        const float up = power_of_two(e), undo = scale_log2 * power_of_two(-e);
+        back[n][0] = __shfl_sync(0xffffffffu, undo, 8 * t4);
+        back[n][1] = __shfl_sync(0xffffffffu, undo, 8 * t4 + 4);
 #pragma unroll
         for (int i = 0; i < QS; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                qa[0][i][2 * j] = hi[0][i][j];
-                qa[0][i][2 * j + 1] = NR == 2 ? hi[NR - 1][i][j] : lo[0][i][j];
-                if (NR == 2) qa[NR - 1][i][2 * j] = lo[0][i][j], qa[NR - 1][i][2 * j + 1] = lo[NR - 1][i][j];
-            }
+            for (int j = 0; j < 2; ++j) qb[n][i][j] = pack_f16(bf16_low(w[2 * i + j]) * up, bf16_high(w[2 * i + j]) * up);
     }
 
-    float o[NT][4];
+    float o[NB][NT][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-    float m[NR], l[NR];
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+    float m[NB][2], l[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.0f;
     int R = 0;                             // + 127
 
     uint32_t phase = 0;
@@ -309,106 +290,99 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         const uint8_t* keys = ring + (warp * STAGES + stage) * 2 * STEP * HD;
         const uint8_t* values = keys + STEP * HD;
         const uint32_t there = __ballot_sync(0xffffffffu, v_exp >= 0);
-        // ---- scores: s[b][2 r + e] of head g + 8 r and key 8 b + 2 t4 + e
-        float s[4][2 * NR];
+        // ---- scores: s[n][u][2 k + e] of head 8 n + 2 t4 + e and key 16 u + 8 k + g
+        float s[NB][2][4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-            for (int i = 0; i < KW / 4; ++i) {
-                const uint4 k = *(const uint4*)(keys + (b * 8 + g) * HD + t4 * (HD / 4) + i * 16);
-                mma_e4m3(c, qa[0][2 * i], k.x, k.y);
-                mma_e4m3(c, qa[0][2 * i + 1], k.z, k.w);
-                if (NR == 2) {
-                    mma_e4m3(d, qa[NR - 1][2 * i], k.x, k.y);
-                    mma_e4m3(d, qa[NR - 1][2 * i + 1], k.z, k.w);
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][u][e] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QS / 4; ++i) {
+                const uint4 a = *(const uint4*)(keys + (16 * u + g) * HD + t4 * (HD / 4) + i * 16);
+                const uint4 b = *(const uint4*)(keys + (16 * u + 8 + g) * HD + t4 * (HD / 4) + i * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t a0, a1, a2, a3;
+                    e4m3x4_to_f16((&a.x)[j], a0, a2);
+                    e4m3x4_to_f16((&b.x)[j], a1, a3);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) mma_f16(s[n][u], a0, a1, a2, a3, qb[n][4 * i + j][0], qb[n][4 * i + j][1]);
                 }
             }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s[b][e] = fmaf(NR == 2 ? d[e] : c[2 + e], 0.0625f, c[e]);
-                if (NR == 2) s[b][2 * NR - 2 + e] = fmaf(d[2 + e], 0.0625f, c[2 + e]);
-            }
         }
-        // in units of the scores' own scale until the exponential: m is the largest so far times that scale
+        // scores in units of the queries' own until the exponential; m is the largest so far in units of log 2
         const float kf = __int_as_float(k_exp << 23);
-        float mx[NR];
+        float mx[NB][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) mx[r] = -INFINITY;
+        for (int n = 0; n < NB; ++n) mx[n][0] = mx[n][1] = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < 4; ++b) {
+            const float f = __shfl_sync(0xffffffffu, kf, b * 8 + g);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f = __shfl_sync(0xffffffffu, kf, b * 8 + 2 * t4 + e);
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int r = 0; r < NR; ++r) s[b][2 * r + e] *= f;
-            }
+                for (int e = 0; e < 2; ++e) s[n][b >> 1][2 * (b & 1) + e] *= f;
+        }
         if (there != 0xffffffffu) {
 #pragma unroll
             for (int b = 0; b < 4; ++b)
+                if (!(there >> (b * 8 + g) & 1))
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (!(there >> (b * 8 + 2 * t4 + e) & 1))
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) s[b][2 * r + e] = -INFINITY;
+                    for (int n = 0; n < NB; ++n) s[n][b >> 1][2 * (b & 1)] = s[n][b >> 1][2 * (b & 1) + 1] = -INFINITY;
         }
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int r = 0; r < NR; ++r) mx[r] = fmaxf(mx[r], s[b][2 * r + e]);
         const int most = max(R, __reduce_max_sync(0xffffffffu, v_exp));
         bool moved = most != R;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-            mx[r] = fmaxf(m[r], mx[r] * back[r]);
-            moved = moved || mx[r] != m[r];
-        }
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = fmaxf(fmaxf(s[n][0][e], s[n][0][2 + e]), fmaxf(s[n][1][e], s[n][1][2 + e]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                mx[n][e] = fmaxf(m[n][e], x * back[n][e]);
+                moved = moved || mx[n][e] != m[n][e];
+            }
         if (__any_sync(0xffffffffu, moved)) {
             const float down = power_of_two(max(R - most, -126));
-            float old[NR];
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                old[r] = mx[r] == -INFINITY ? 1.0f : ex2(m[r] - mx[r]);
-                l[r] *= old[r];
-                old[r] *= down;
-                m[r] = mx[r];
-            }
             R = most;
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int n = 0; n < NB; ++n) {
+                float old[2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] *= old[NR == 2 ? e >> 1 : 0];
-        }
-        // ---- weights: their parts as the first operand of one product (up to eight heads: both) or two.  (At most 2^8: a code goes to 448)
-        const float vf = power_of_two(max(v_exp - R + 8, -126));
-        uint32_t hi[NR][2], lo[NR][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = __shfl_sync(0xffffffffu, vf, (2 * u + (j >> 1)) * 8 + 2 * t4 + (j & 1));
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                const float sub = m[r] == -INFINITY ? 0.0f : -m[r];
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float w = ex2(fmaf(s[2 * u + (j >> 1)][2 * r + (j & 1)], back[r], sub));
-                    l[r] += w;
-                    x[j] = w * f[j];
+                for (int e = 0; e < 2; ++e) {
+                    old[e] = mx[n][e] == -INFINITY ? 1.0f : ex2(m[n][e] - mx[n][e]);
+                    l[n][e] *= old[e];
+                    old[e] *= down;
+                    m[n][e] = mx[n][e];
                 }
-                hi[r][u] = first_part(x[0], x[1]) | first_part(x[2], x[3]) << 16;
-                if (NR == 2) lo[r][u] = codes_of(x[0], x[1]) | codes_of(x[2], x[3]) << 16;
-                else lo[r][u] = codes_of(x[0] * 16.0f, x[1] * 16.0f) | codes_of(x[2] * 16.0f, x[3] * 16.0f) << 16;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][i][e] *= old[e & 1];
             }
         }
-        const uint32_t pa[4] = {hi[0][0], NR == 2 ? hi[NR - 1][0] : lo[0][0], hi[0][1], NR == 2 ? hi[NR - 1][1] : lo[0][1]};
-        const uint32_t pb[4] = {lo[0][0], lo[NR - 1][0], lo[0][1], lo[NR - 1][1]};
-        // ---- values: column tile i holds entries g HD / 8 + i of the eight g; four keys of an entry to a word
+        // ---- weights: pb[n][b] of head 8 n + g and keys 8 b + 2 t4 + {0, 1}
+        const float vf = power_of_two(max(v_exp - R, -126));
+        uint32_t pb[NB][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float f = __shfl_sync(0xffffffffu, vf, b * 8 + g);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float w = ex2(fmaf(s[n][b >> 1][2 * (b & 1) + e], back[n][e], m[n][e] == -INFINITY ? 0.0f : -m[n][e]));
+                    l[n][e] += w;
+                    x[e] = w * f;
+                }
+                pb[n][b] = transposed(pack_f16(x[0], x[1]));
+            }
+        }
+        // ---- values: row tile i holds entries g HD / 8 + 2 i (rows 0 .. 7) and + 2 i + 1 (8 .. 15) of the eight g
         uint32_t vw[2][4][VW];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -422,35 +396,22 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
                     const uint2 x = *(const uint2*)(values + row * HD + g * 8);
                     vw[u][i][0] = x.x, vw[u][i][1] = x.y;
                 }
-            }
-        if (there != 0xffffffffu) {
-            // rows of no key hold what was there before
+                if (there != 0xffffffffu && !(there >> row & 1))      // (a row of no key holds what was there before)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!(there >> (u * 16 + (i >> 1) * 8 + 2 * t4 + (i & 1)) & 1))
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) vw[u][i][w] = 0;
-        }
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            uint32_t b[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t x01 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x5140), x23 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x5140);
-                const uint32_t y01 = __byte_perm(vw[u][0][w], vw[u][1][w], 0x7362), y23 = __byte_perm(vw[u][2][w], vw[u][3][w], 0x7362);
-                b[u][0] = __byte_perm(x01, x23, 0x5410);
-                b[u][1] = __byte_perm(x01, x23, 0x7632);
-                b[u][2] = __byte_perm(y01, y23, 0x5410);
-                b[u][3] = __byte_perm(y01, y23, 0x7632);
+                    for (int w = 0; w < VW; ++w) vw[u][i][w] = 0;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                mma_e4m3(o[4 * w + i], pa, b[0][i], b[1][i]);
-                if (NR == 2) mma_e4m3(o[4 * w + i], pb, b[0][i], b[1][i]);
-            }
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < VW; ++w)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t a0, a1, a2, a3;
+                    e4m3x4_to_f16(__byte_perm(vw[u][0][w], vw[u][1][w], j ? 0x7362 : 0x5140), a0, a1);
+                    e4m3x4_to_f16(__byte_perm(vw[u][2][w], vw[u][3][w], j ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) mma_f16(o[n][2 * w + j], a0, a1, a2, a3, pb[n][2 * u], pb[n][2 * u + 1]);
+                }
         __syncwarp();                      // (every lane has read this step's stage)
         phase ^= stage;
         stage ^= 1;
@@ -459,17 +420,18 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
 
     // ---- the four warps' results, added in their order
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (t4 == 0) sm[warp][g + 8 * r] = m[r], sl[warp][g + 8 * r] = l[r];
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            red[warp][g + 8 * r][2 * t4 * NT + i] = NR == 2 ? o[i][2 * r] : fmaf(o[i][2], 0.0625f, o[i][0]);
-            red[warp][g + 8 * r][(2 * t4 + 1) * NT + i] = NR == 2 ? o[i][2 * r + 1] : fmaf(o[i][3], 0.0625f, o[i][1]);
+        for (int e = 0; e < 2; ++e) {
+            const int head = 8 * n + 2 * t4 + e;
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+            if (g == 0) sm[warp][head] = m[n][e], sl[warp][head] = l[n][e];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) *(float2*)&red[warp][head][g * (HD / 8) + 2 * i] = make_float2(o[n][i][e], o[n][i][2 + e]);
         }
-    }
-    if (lane == 0) sr[warp] = R - 127 - 8;
+    if (lane == 0) sr[warp] = R - 127;
     __syncthreads();
     for (int i = tid; i < n_h * (HD / 2); i += WARPS * 32) {
         const int row = i / (HD / 2), d = 2 * (i % (HD / 2));
@@ -514,18 +476,24 @@ __global__ void __launch_bounds__(128) decode_e4m3_merge_kernel(__nv_bfloat16* _
     float L = 0.0f, a[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) a[j] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float2 ml = *(const float2*)(part_ml + (s0 + s) * 2);
-        const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-        L = fmaf(ml.y, f, L);
+    for (int c = 0; c < splits; c += 32) {
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (c + lane < splits) ml = *(const float2*)(part_ml + (s0 + c + lane) * 2);
+        const float mine = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        L = fmaf(ml.y, mine, L);
+        const int n = min(32, splits - c);
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) {
+            const float f = __shfl_sync(0xffffffffu, mine, s);
 #pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-            const float2 v = *(const float2*)(part_acc + (s0 + s) * HD + lane * VEC + j);
-            a[j] = fmaf(v.x, f, a[j]);
-            a[j + 1] = fmaf(v.y, f, a[j + 1]);
+            for (int j = 0; j < VEC; j += 2) {
+                const float2 v = *(const float2*)(part_acc + (s0 + c + s) * HD + lane * VEC + j);
+                a[j] = fmaf(v.x, f, a[j]);
+                a[j + 1] = fmaf(v.y, f, a[j + 1]);
+            }
         }
     }
+    L = warp_sum(L);
     const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int j = 0; j < VEC; j += 2)

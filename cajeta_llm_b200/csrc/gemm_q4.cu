@@ -41,8 +41,9 @@ struct Args {
     int rows, x_rows, features, K, groups, half_out, accumulate;
 };
 
-// NTOK: rows of x a block takes at a time; WM: pieces of 16 features a block takes of each weight; HALF: groups of 32
-template <int NTOK, int WM, bool GATED, bool HALF>
+// NTOK: rows of x a block takes at a time; WM: pieces of 16 features a block takes of each weight; HALF: groups of 32; AHEAD: tiles along K whose codes
+// a warp has asked for before it multiplies the first
+template <int NTOK, int WM, bool GATED, bool HALF, int AHEAD>
 __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
     constexpr int NB = NTOK / 8, W = GATED ? 2 : 1, PIECE = q4::piece_bytes(HALF);
     constexpr int GRP = HALF ? 2 : 1;                      // groups of a tile
@@ -56,7 +57,11 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
     if (GATED) wp[W - 1] = a.w_up + (size_t)grp * tiles_f * tiles_k * q4::tile_bytes(HALF);
     // piece i of K tile kt
     auto piece = [&](int i, int kt) { return ((size_t)((piece0 + i) >> 3) * tiles_k + kt) * q4::tile_bytes(HALF) + ((piece0 + i) & 7) * PIECE; };
-    auto fetch = [&](int kt, uint4 (&c)[W][WM], uint32_t (&s)[W][WM][GRP]) {
+    struct Codes {
+        uint4 c[W][WM];
+        uint32_t s[W][WM][GRP];
+    };
+    auto fetch = [&](int kt, Codes& to) {
 #pragma unroll
         for (int i = 0; i < WM; ++i)
 #pragma unroll
@@ -64,19 +69,23 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
                 // (pieces past the last tile of features are not there; the last tile's are, filled with zeros)
                 const bool in = kt < tiles_k && ((piece0 + i) >> 3) < tiles_f;
                 const uint8_t* p = wp[u] + (in ? piece(i, kt) : 0);
-                c[u][i] = in ? q4::ldg_codes(p + lane * 16) : make_uint4(0, 0, 0, 0);
+                to.c[u][i] = in ? q4::ldg_codes(p + lane * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int h = 0; h < GRP; ++h) s[u][i][h] = in ? __ldg((const uint32_t*)(p + 512 + (h * 8 + g) * 4)) : 0u;
+                for (int h = 0; h < GRP; ++h) to.s[u][i][h] = in ? __ldg((const uint32_t*)(p + 512 + (h * 8 + g) * 4)) : 0u;
             }
     };
-    uint4 code[W][WM];
-    uint32_t scale[W][WM][GRP];
-    fetch(warp, code, scale);
+    Codes ring[AHEAD];
+    auto fetch_first = [&]() {
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) fetch(warp + d * WARPS, ring[d]);
+    };
+    // (a group's rows are known only after the wait, and most groups of a few rows' step have none)
+    if (!a.offsets) fetch_first();
     cj::after_predecessor();
     cj::release_successor();
     const int lo = a.offsets ? max(0, a.offsets[grp]) : 0, hi = a.offsets ? min(a.rows, a.offsets[grp + 1]) : a.rows;
     for (int row0 = lo + blockIdx.z * NTOK; row0 < hi; row0 += gridDim.z * NTOK) {
-        if (row0 != lo + (int)blockIdx.z * NTOK) fetch(warp, code, scale);
+        if (a.offsets || row0 != (int)blockIdx.z * NTOK) fetch_first();
         const __nv_bfloat16* xr[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -94,12 +103,7 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[u][i][n][e] = 0.0f;
-#pragma unroll 1
-        for (int kt = warp; kt < tiles_k; kt += WARPS) {
-            uint4 next[W][WM];
-            uint32_t next_scale[W][WM][GRP];
-            fetch(kt + WARPS, next, next_scale);
-            uint2 xb[NB][4];
+        auto fetch_x = [&](int kt, uint2 (&xb)[NB][4]) {
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -107,6 +111,23 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
                     const int k = kt * 64 + j * 16 + t4 * 4;
                     xb[n][j] = xr[n] && k < a.K ? __ldg((const uint2*)(xr[n] + k)) : make_uint2(0u, 0u);
                 }
+        };
+        uint2 x_next[NB][4];
+        fetch_x(warp, x_next);
+#pragma unroll 1
+        for (int kt0 = warp; kt0 < tiles_k; kt0 += WARPS * AHEAD)
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) {
+            const int kt = kt0 + d * WARPS;
+            if (kt >= tiles_k) break;
+            const Codes now = ring[d];
+            uint2 xb[NB][4];
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) xb[n][j] = x_next[n][j];
+            fetch(kt + WARPS * AHEAD, ring[d]);
+            fetch_x(kt + WARPS, x_next);
 #pragma unroll
             for (int u = 0; u < W; ++u)
 #pragma unroll
@@ -120,7 +141,7 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) part[n][e] = 0.0f;
                         }
-                        const uint32_t wa = j < 2 ? code[u][i].x : code[u][i].y, wb = j < 2 ? code[u][i].z : code[u][i].w;
+                        const uint32_t wa = j < 2 ? now.c[u][i].x : now.c[u][i].y, wb = j < 2 ? now.c[u][i].z : now.c[u][i].w;
                         uint32_t f[4];
                         f[0] = q4::pair(wa >> (8 * (j & 1)));
                         f[1] = q4::pair(wb >> (8 * (j & 1)));
@@ -129,7 +150,7 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
 #pragma unroll
                         for (int n = 0; n < NB; ++n) mma_bf16(part[n], f, xb[n][j].x, xb[n][j].y);
                         if (j % (4 / GRP) == 4 / GRP - 1) {
-                            const uint32_t s = scale[u][i][j / (4 / GRP)];
+                            const uint32_t s = now.s[u][i][j / (4 / GRP)];
                             const float s0 = __uint_as_float(s << 16), s1 = __uint_as_float(s & 0xffff0000u);
 #pragma unroll
                             for (int n = 0; n < NB; ++n) {
@@ -140,14 +161,6 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
                             }
                         }
                     }
-                }
-#pragma unroll
-            for (int u = 0; u < W; ++u)
-#pragma unroll
-                for (int i = 0; i < WM; ++i) {
-                    code[u][i] = next[u][i];
-#pragma unroll
-                    for (int h = 0; h < GRP; ++h) scale[u][i][h] = next_scale[u][i][h];
                 }
         }
         // ---- the warps' sums: feature i * 16 + g (+ 8), row n * 8 + 2 t4 (+ 1)
@@ -286,24 +299,25 @@ CJ_EXPORT int cj_gemm_q4(const void* x, long long ldx, int x_rows, const void* w
     const Args a{(const __nv_bfloat16*)x, (const uint8_t*)w, (const uint8_t*)w_up, bias, out, offsets, index, ldx, ldo, rows, x_rows,
                  features, K, groups, out_dtype == CJ_BF16 ? 1 : 0, accumulate};
     const int all = (features + 15) / 16;
-    const int row_tiles = min((rows + n_tok - 1) / n_tok, offsets ? 8 : 65535);
-#define LAUNCH(NTOK, WM, GATED, HALF)                                                                                     \
+    // (the blocks of a group take its rows tile by tile: how many it has is not known here)
+    const int row_tiles = offsets ? 1 : min((rows + n_tok - 1) / n_tok, 65535);
+#define LAUNCH(NTOK, WM, GATED, HALF, AHEAD)                                                                                     \
     {                                                                                                                     \
         constexpr int smem = WARPS * (GATED ? 2 : 1) * WM * 16 * (NTOK + 1) * 4;                                          \
-        cudaError_t e = cudaFuncSetAttribute(gemm_q4_kernel<NTOK, WM, GATED, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
+        cudaError_t e = cudaFuncSetAttribute(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
         if (e != cudaSuccess) return (int)e;                                                                              \
-        cj::launch(gemm_q4_kernel<NTOK, WM, GATED, HALF>, dim3((all + WM - 1) / WM, groups, row_tiles), dim3(WARPS * 32), smem, stream, a); \
+        cj::launch(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, dim3((all + WM - 1) / WM, groups, row_tiles), dim3(WARPS * 32), smem, stream, a); \
         return launch_status();                                                                                           \
     }
-#define PICK(NTOK, WM)                                                                                                    \
+#define PICK(NTOK, WM, AHEAD)                                                                                                    \
     if (n_tok == NTOK && pieces == WM) {                                                                                  \
-        if (w_up) { if (half) LAUNCH(NTOK, WM, true, true) else LAUNCH(NTOK, WM, true, false) }                           \
-        else { if (half) LAUNCH(NTOK, WM, false, true) else LAUNCH(NTOK, WM, false, false) }                              \
+        if (w_up) { if (half) LAUNCH(NTOK, WM, true, true, AHEAD) else LAUNCH(NTOK, WM, true, false, AHEAD) }                           \
+        else { if (half) LAUNCH(NTOK, WM, false, true, AHEAD) else LAUNCH(NTOK, WM, false, false, AHEAD) }                              \
     }
-    PICK(8, 1)
-    PICK(8, 2)
-    PICK(16, 2)
-    PICK(32, 2)
+    PICK(8, 1, 4)
+    PICK(8, 2, 2)
+    PICK(16, 2, 2)
+    PICK(32, 2, 1)
 #undef PICK
 #undef LAUNCH
     return CJ_ERR_SIZE;

@@ -1778,11 +1778,18 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tok
 
 @functools.lru_cache(maxsize=4096)
 def e4m3_splits(rows: int, n_heads: int, n_kv: int, span: int, sms: int) -> int:
-    """Blocks that share a row's keys in ``decode_attention_e4m3``: as many as it takes to put three blocks on every SM, of at
-    least 128 keys (a step of each of a block's warps)."""
+    """Blocks that share a row's keys in ``decode_attention_e4m3``."""
     group = n_heads // n_kv
-    blocks = rows * n_kv * -(-group // (16 if group > 8 else 8))
-    return max(1, min(-(-3 * sms // blocks), -(-span // 128), 64))
+    blocks, steps = rows * n_kv * -(-group // (16 if group > 8 else 8)), -(-span // 128)
+
+    # rounds of three blocks an SM, each a start and steps of 128 keys that take a chain of waits alone (1.1 us) and their bytes' time
+    # together; and the merge.  (us, fitted; measured at 1, 4, 12 or 14 and 32 blocks a row: 32 rows x 4,096 keys of 16 heads 120, 100, 116, 168; eight
+    # rows of up to 32,768, 4 kv heads, 297, 84, 51 or 53, 57; one of 32,768 278, 79, 33, 21; eight of 576, 16 heads, 9, 12, 16, 31)
+    def cost(n):
+        rounds = -(-blocks * n // (3 * sms))
+        return rounds * (3 + -(-steps // n) * max(1.1, 0.72 * min(3.0, blocks * n / sms))) + (2 + 0.12 * n if n > 1 else 0)
+
+    return min(range(1, min(steps, 128) + 1), key=cost)
 
 
 def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor,

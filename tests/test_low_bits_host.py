@@ -152,8 +152,10 @@ def test_the_cache_holds_codes_and_exponents():
 
 
 def test_blocks_a_row():
-    """Rows of few blocks are dealt out until every SM has three, in pieces of at least 128 keys."""
-    assert K.e4m3_splits(1, 16, 16, 576, 148) == 5
-    assert K.e4m3_splits(64, 16, 16, 2048, 148) == 1
-    assert K.e4m3_splits(1, 28, 4, 32768, 148) == 64
+    """Few rows are dealt out to many blocks, many or short ones are not; never to more than a step of 128 keys each."""
+    assert K.e4m3_splits(1, 16, 16, 576, 148) > 2
+    assert K.e4m3_splits(8, 16, 16, 576, 148) == 1
+    assert 20 <= K.e4m3_splits(1, 28, 4, 32768, 148) <= 64
     assert K.e4m3_splits(1, 40, 2, 1, 148) == 1
+    for rows, span in ((1, 1), (3, 200), (64, 2048), (1000, 9), (1, 100_000)):
+        assert 1 <= K.e4m3_splits(rows, 28, 4, span, 148) <= max(1, -(-span // 128))
