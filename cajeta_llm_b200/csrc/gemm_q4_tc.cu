@@ -22,8 +22,8 @@ using namespace tc;
 
 namespace {
 
-constexpr int LOAD0 = 0, PRODUCT = 1, EPI0 = 2, CONV0 = 6, LOAD1 = 14;      // warps
-constexpr int THREADS = 15 * 32;
+constexpr int LOAD0 = 0, PRODUCT = 1, EPI0 = 2, CONV0 = 6, CONV_SETS = 2, LOAD1 = CONV0 + 8 * CONV_SETS;      // warps
+constexpr int THREADS = (LOAD1 + 1) * 32;
 constexpr int MAX_STAGES = 8, MAX_SLOTS = 8, MAX_GROUPS = 1024;
 constexpr int SLOT_COLS = 32;                 // 128 rows x 64 bfloat16
 constexpr int SMEM_LIMIT = 222 * 1024;        // (with the groups' table, 4 KB, what a block can have)
@@ -217,13 +217,16 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         }
     } else if (warp >= CONV0) {
         // ---- codes to bfloat16: a piece of 16 features a warp, into the 16 lanes of tensor memory that are the piece's rows
-        const int q = warp & 3, upper = (warp - CONV0) >> 2;       // the quarter of the lanes this warp may touch, and which half of it
+        // (two sets of eight warps take turns: one waits, loads and stores while the other computes)
+        const int q = warp & 3, upper = (warp - CONV0) >> 2 & 1;   // the quarter of the lanes this warp may touch, and which half of it
+        const uint32_t set = (warp - CONV0) >> 3;
         const int piece = GATED ? upper * 4 + q : q * 2 + upper;
         const uint32_t lanes = (uint32_t)(q * 32 + upper * 16) << 16;
         uint32_t it = 0;
         bool ok = true;
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
             for (int kb = 0; kb < n_kb; ++kb, ++it) {
+                if (it % CONV_SETS != set) continue;
                 const int s = it % p.stages, slot = it % p.slots;
                 ok = mbar_wait_warp(&full[s], (it / p.stages) & 1, 5);
                 if (!ok) break;

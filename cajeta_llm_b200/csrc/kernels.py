@@ -1698,16 +1698,36 @@ def wait_errors() -> Dict[str, int]:
 
 # ---- the 8-bit cache ------------------------------------------------------------------------------------------------------
 
+_SIGNS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+
+
+def _entry(lib: str, name: str, signs: str):
+    """A library's function that takes Python's numbers as they are (a letter of ``signs`` an argument: an object made of each argument, of two
+    dozen, takes as long as the launch)."""
+    fn = getattr(library(lib), name)
+    if fn.argtypes is None:
+        fn.argtypes = [_SIGNS[c] for c in signs]
+    return fn
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _raw() -> int:
+    return _raw_stream(_raw_device()) if _raw_stream is not None and _raw_device is not None else torch.cuda.current_stream().cuda_stream
+
+
 def _need_e4m3_cache(k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor, page_tokens: int, n_kv: int,
                      head_dim: int, what: str) -> None:
     shape = (k_plane.shape[0], n_kv, page_tokens, head_dim)
     for n, t in (("k_plane", k_plane), ("v_plane", v_plane)):
         _need(t, n, torch.float8_e4m3fn)
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise KernelError(f"{what}: {n} {tuple(t.shape)} is not [pages, {n_kv}, {page_tokens}, {head_dim}]")
     for n, t in (("k_exp", k_exp), ("v_exp", v_exp)):
         _need(t, n, torch.uint8)
-        if tuple(t.shape) != shape[:3]:
+        if t.shape != shape[:3]:
             raise KernelError(f"{what}: {n} {tuple(t.shape)} is not [pages, {n_kv}, {page_tokens}]")
 
 
@@ -1717,9 +1737,9 @@ def _on_device(t: torch.Tensor) -> bool:
 
 def _need_same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The kernels launch on the current device's current stream: every tensor lies there."""
-    here = torch.cuda.current_device()
+    here = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != here:
+        if t is not None and t.get_device() != here:
             raise KernelError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{here}")
 
 
@@ -1736,7 +1756,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     if not _on_device(qkv) or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError("rope_kv_write_e4m3: qkv must be a float32 CUDA matrix whose rows are contiguous")
     T = qkv.shape[0]
-    if tuple(q_out.shape) != (T, n_heads, head_dim) or positions.numel() != T:
+    if q_out.shape != (T, n_heads, head_dim) or positions.numel() != T:
         raise KernelError(f"rope_kv_write_e4m3: q_out {tuple(q_out.shape)} and positions {tuple(positions.shape)} do not fit {T} rows")
     ends = [q_off + n_heads * head_dim] + ([k_off + n_kv * head_dim, v_off + n_kv * head_dim] if write_kv else [])
     if max(ends) > qkv.shape[1] or min(q_off, *(o for o in (k_off, v_off) if write_kv), 1 << 30) < 0:
@@ -1753,10 +1773,10 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
         if row_req.numel() != T or table.dim() != 2:
             raise KernelError("rope_kv_write_e4m3: row_req must name each row's request, table must be [requests, pages]")
     _need_same_device("rope_kv_write_e4m3", qkv, q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
-    st = library("cache_e4m3").cj_append_e4m3(
-        _ptr(qkv), _i(qkv.stride(0)), _i(q_off), _i(k_off if write_kv else 0), _i(v_off if write_kv else 0), _ptr(q_out), _ptr(k_plane), _ptr(v_plane),
-        _ptr(k_exp), _ptr(v_exp), _ptr(positions), _ptr(row_req), _ptr(table), _i(table.shape[0] if write_kv else 0), _i(table.stride(0) if write_kv else 0),
-        _i(page_tokens), _i(k_plane.shape[0] if write_kv else 0), _i(T), _i(n_heads), _i(n_kv), _i(head_dim), _i(rotary_dim), _ptr(inv_freq), _i(1 if write_kv else 0), _stream())
+    st = _entry("cache_e4m3", "cj_append_e4m3", "piiiippppppppiiiiiiiiipip")(
+        qkv.data_ptr(), qkv.stride(0), q_off, k_off if write_kv else 0, v_off if write_kv else 0, q_out.data_ptr(), _at(k_plane), _at(v_plane),
+        _at(k_exp), _at(v_exp), positions.data_ptr(), _at(row_req), _at(table), table.shape[0] if write_kv else 0, table.stride(0) if write_kv else 0,
+        page_tokens, k_plane.shape[0] if write_kv else 0, T, n_heads, n_kv, head_dim, rotary_dim, _at(inv_freq), 1 if write_kv else 0, _raw())
     _check(st, "rope_kv_write_e4m3")
 
 
@@ -1766,7 +1786,7 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tok
         raise KernelError(f"{what} takes heads of 64 or 128, not {head_dim}")
     if n_kv <= 0 or n_heads % n_kv != 0:
         raise KernelError(f"{what}: {n_heads} heads are not a multiple of {n_kv} kv heads")
-    if tuple(q.shape[-2:]) != (n_heads, head_dim) or q.dim() != 3 or out.shape != q.shape:
+    if q.dim() != 3 or q.shape[1:] != (n_heads, head_dim) or out.shape != q.shape:
         raise KernelError(f"{what}: q {tuple(q.shape)} and out {tuple(out.shape)} are not [rows, {n_heads}, {head_dim}]")
     if table.dim() != 2:
         raise KernelError(f"{what}: table must be [requests, pages]")
@@ -1813,10 +1833,10 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
     if splits > 1:
         acc = torch.empty((T, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
         ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
-    st = library("cache_e4m3").cj_decode_e4m3(
-        _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(positions), _ptr(row_req),
-        _ptr(None), _ptr(None), _i(table.shape[0]), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(T), _i(n_heads), _i(n_kv), _i(head_dim), _i(window),
-        _f(scale), _i(splits), _ptr(acc), _ptr(ml), _stream())
+    st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
+        q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
+        positions.data_ptr(), row_req.data_ptr(), None, None, table.shape[0], table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv,
+        head_dim, window, scale, splits, _at(acc), _at(ml), _raw())
     _check(st, "decode_attention_e4m3")
     if splits > 1:
         global launches
@@ -1842,16 +1862,16 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     if T == 0 or R == 0:
         return
     if T > E4M3_ROW_BY_ROW:
-        st = library("attention_e4m3_tc").cj_prefill_e4m3_tc(
-            _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(req_start), _ptr(req_prior),
-            _i(R), _i(T), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(n_heads), _i(n_kv), _i(head_dim), _i(window), _f(scale), _i(0),
-            _i(_sm_count()), _stream())
+        st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifiip")(
+            q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
+            req_start.data_ptr(), req_prior.data_ptr(), R, T, table.data_ptr(), table.stride(0), page_tokens, n_heads, n_kv, head_dim, window,
+            scale, 0, _sm_count(), _raw())
         _check(st, "prefill_attention_e4m3")
         return
-    st = library("cache_e4m3").cj_decode_e4m3(
-        _ptr(q), _ptr(out), _ptr(k_plane), _ptr(v_plane), _ptr(k_exp), _ptr(v_exp), _i(k_plane.shape[0]), _ptr(None), _ptr(None),
-        _ptr(req_start), _ptr(req_prior), _i(R), _ptr(table), _i(table.stride(0)), _i(page_tokens), _i(T), _i(n_heads), _i(n_kv), _i(head_dim),
-        _i(window), _f(scale), _i(1), _ptr(None), _ptr(None), _stream())
+    st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
+        q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0], None, None,
+        req_start.data_ptr(), req_prior.data_ptr(), R, table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv, head_dim, window, scale, 1,
+        None, None, _raw())
     _check(st, "prefill_attention_e4m3")
 
 
@@ -2012,20 +2032,18 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
         x, x_rows = a, a.shape[0]
         if a_row_index is not None:
             x = torch.empty((M, w.k), dtype=torch.bfloat16, device=a.device)
-            st = library("gemm_q4_tc").cj_q4_gather(_ptr(a), _ll(a.stride(0)), _i(x_rows), _ptr(a_row_index), _ptr(x), _i(M), _i(w.k), _stream())
+            st = _entry("gemm_q4_tc", "cj_q4_gather", "plippiip")(a.data_ptr(), a.stride(0), x_rows, a_row_index.data_ptr(), x.data_ptr(), M, w.k, _raw())
             _check(st, "gemm_q4")
             x_rows = M
         tok = q4_tile_rows(M, w.features, w.groups if group_offsets is not None else 0, w_up is not None, _sm_count())
-        st = library("gemm_q4_tc").cj_gemm_q4_tc(
-            _ptr(x), _ll(x.stride(0)), _i(x_rows), _ptr(w.data), _ptr(w_up.data if w_up is not None else None), _ptr(bias), _ptr(out), _i(_code(out)),
-            _ll(out.stride(0)), _i(M), _i(w.features), _i(w.k), _i(w.groups), _i(half), _ptr(group_offsets), _i(1 if accumulate else 0), _i(tok),
-            _i(_sm_count()), _stream())
+        st = _entry("gemm_q4_tc", "cj_gemm_q4_tc", "plippppiliiiiipiiip")(
+            x.data_ptr(), x.stride(0), x_rows, w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
+            out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), 1 if accumulate else 0, tok, _sm_count(), _raw())
         _check(st, "gemm_q4")
         return
     n_tok = 8 if M <= 8 or group_offsets is not None and M <= 4 * w.groups else 16 if M <= 16 else 32
     pieces = 1 if n_tok == 8 else 2
-    st = library("gemm_q4").cj_gemm_q4(
-        _ptr(a), _ll(a.stride(0)), _i(a.shape[0]), _ptr(w.data), _ptr(w_up.data if w_up is not None else None), _ptr(bias), _ptr(out),
-        _i(_code(out)), _ll(out.stride(0)), _i(M), _i(w.features), _i(w.k), _i(w.groups), _i(half), _ptr(group_offsets),
-        _ptr(a_row_index), _i(1 if accumulate else 0), _i(n_tok), _i(pieces), _stream())
+    st = _entry("gemm_q4", "cj_gemm_q4", "plippppiliiiiippiiip")(
+        a.data_ptr(), a.stride(0), a.shape[0], w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
+        out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), _at(a_row_index), 1 if accumulate else 0, n_tok, pieces, _raw())
     _check(st, "gemm_q4")

@@ -159,3 +159,18 @@ def test_blocks_a_row():
     assert K.e4m3_splits(1, 40, 2, 1, 148) == 1
     for rows, span in ((1, 1), (3, 200), (64, 2048), (1000, 9), (1, 100_000)):
         assert 1 <= K.e4m3_splits(rows, 28, 4, span, 148) <= max(1, -(-span // 128))
+
+
+def test_what_a_call_hands_over_is_what_the_function_takes():
+    """The letters of every entry point's arguments against the declaration in its source."""
+    import os
+    import re
+    from cajeta_llm_b200.csrc import build
+    with open(K.__file__) as f:
+        calls = set(re.findall(r'_entry\("(\w+)", "(\w+)", "(\w+)"\)', f.read()))
+    assert len(calls) >= 6
+    for lib, name, signs in calls:
+        with open(os.path.join(build.HERE, build.LIBRARIES[lib])) as f:
+            declared = re.search(r"CJ_EXPORT int " + name + r"\(([^)]*)\)", f.read()).group(1)
+        kinds = "".join("p" if "*" in a or "cudaStream_t" in a else "l" if "long long" in a else "f" if "float" in a else "i" for a in declared.split(","))
+        assert kinds == signs, name
