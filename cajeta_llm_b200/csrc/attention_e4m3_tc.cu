@@ -5,7 +5,7 @@
 //     P = exp2(S scale - m)           four warps a query tile, a row a thread; P as bfloat16 over the columns of its scores
 //     O += P . (code_v 2^e_v)         O in tensor memory
 // A code times its power of two is a bfloat16 number exactly, whatever the exponents of the tokens beside it (f16 would keep more bits of P,
-// but only values within 22 octaves of each other: a row's values could vanish beside larger ones that it does not even see).  So three warps
+// but only values within 22 octaves of each other: a row's values could vanish beside larger ones that it does not even see).  So seven warps
 // turn codes into the bfloat16 tiles in shared memory that both products read, and the rest is attention over a bfloat16 cache: P, as there, is
 // the one rounding.  The codes come with plain 16-byte loads, pages of any size, a tile's keys in registers while its predecessor's values are
 // converted (half the bytes of a bfloat16 cache: 16 KB a tile).  The two query tiles take turns between the exponential unit and the tensor
@@ -22,8 +22,8 @@ namespace {
 
 constexpr int BM = 128, QT = 2, BN = 128;         // query rows a tile, tiles a block, keys a tile
 constexpr int STAGES = 2;
-constexpr int CONV_WARPS = 3, PRODUCT = 3, SOFT0 = 4;
-constexpr int THREADS = 12 * 32;                  // three warps a scheduler: 168 registers a thread
+constexpr int CONV_WARPS = 7, PRODUCT = 7, SOFT0 = 8;
+constexpr int THREADS = 16 * 32;
 constexpr int HALF_BYTES = 128 * 64 * 2;          // [128 x 64] f16, swizzled: 16 KB
 constexpr float RESCALE_THRESHOLD = 8.0f;         // in log2 units
 constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;

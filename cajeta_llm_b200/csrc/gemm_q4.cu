@@ -52,26 +52,30 @@ __global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
     const int tiles_k = (a.K + 63) / 64, tiles_f = (a.features + 127) / 128;
     const int piece0 = blockIdx.x * WM;                    // of all pieces of 16 features
     const int grp = blockIdx.y;
-    const uint8_t* wp[W];
-    wp[0] = a.w + (size_t)grp * tiles_f * tiles_k * q4::tile_bytes(HALF);
-    if (GATED) wp[W - 1] = a.w_up + (size_t)grp * tiles_f * tiles_k * q4::tile_bytes(HALF);
-    // piece i of K tile kt
-    auto piece = [&](int i, int kt) { return ((size_t)((piece0 + i) >> 3) * tiles_k + kt) * q4::tile_bytes(HALF) + ((piece0 + i) & 7) * PIECE; };
+    // where this lane's codes and this lane's scales of a piece lie in the first tile along K (pieces past the last tile of features are not there; the
+    // last tile's are, filled with zeros)
+    const uint8_t* at[W][WM];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) {
+        const int pc = piece0 + i, ft = min(pc >> 3, tiles_f - 1);
+        const size_t off = ((size_t)grp * tiles_f + ft) * tiles_k * q4::tile_bytes(HALF) + (pc & 7) * PIECE;
+        at[0][i] = a.w + off;
+        if (GATED) at[W - 1][i] = a.w_up + off;
+    }
     struct Codes {
         uint4 c[W][WM];
         uint32_t s[W][WM][GRP];
     };
     auto fetch = [&](int kt, Codes& to) {
+        if (kt >= tiles_k) return;
+        const size_t off = (size_t)kt * q4::tile_bytes(HALF);
 #pragma unroll
         for (int i = 0; i < WM; ++i)
 #pragma unroll
             for (int u = 0; u < W; ++u) {
-                // (pieces past the last tile of features are not there; the last tile's are, filled with zeros)
-                const bool in = kt < tiles_k && ((piece0 + i) >> 3) < tiles_f;
-                const uint8_t* p = wp[u] + (in ? piece(i, kt) : 0);
-                to.c[u][i] = in ? q4::ldg_codes(p + lane * 16) : make_uint4(0, 0, 0, 0);
+                to.c[u][i] = q4::ldg_codes(at[u][i] + off + lane * 16);
 #pragma unroll
-                for (int h = 0; h < GRP; ++h) to.s[u][i][h] = in ? __ldg((const uint32_t*)(p + 512 + (h * 8 + g) * 4)) : 0u;
+                for (int h = 0; h < GRP; ++h) to.s[u][i][h] = __ldg((const uint32_t*)(at[u][i] + off + 512 + (h * 8 + g) * 4));
             }
     };
     Codes ring[AHEAD];

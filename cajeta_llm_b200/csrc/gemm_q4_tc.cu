@@ -83,6 +83,17 @@ __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_
         : "memory");
 }
 
+// A place in a ring and the parity of the round it is in, for what comes `by` places further each time (a division by a ring's length, which is not a
+// constant, costs a converting warp as much as the conversion).
+struct Ring {
+    int at;
+    uint32_t phase;
+    __device__ __forceinline__ void move(int by, int length) {
+        at += by;
+        while (at >= length) at -= length, phase ^= 1;
+    }
+};
+
 __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t s) {
     const __nv_bfloat162 r = __hmul2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&s);
     return *(const uint32_t*)&r;
@@ -169,15 +180,18 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                 cj::after_predecessor();
             }
             uint32_t it = 0;
+            Ring st_ring{(int)mine, 0};
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 const Tile t = tile_of(p, tile, feat_tiles, before);
                 for (int kb = 0; kb < n_kb; ++kb, ++it) {
                     if ((it & 1) != mine) continue;
-                    const int s = it % p.stages;
+                    const int s = st_ring.at;
+                    const uint32_t phase = st_ring.phase;
+                    st_ring.move(2, p.stages);
                     uint8_t* st = smem + (size_t)s * p.stage_bytes;
                     if (it >= early) {
-                        ok = mbar_wait(&empty[s], ((it / p.stages) & 1) ^ 1, 1);
+                        ok = mbar_wait(&empty[s], phase ^ 1, 1);
                         if (!ok) break;
                         mbar_expect_tx(&full[s], p.x_bytes + TILE);
                         codes(t, kb, st, &full[s]);
@@ -189,20 +203,20 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     } else if (warp == PRODUCT) {
         // ---- products
         if (elect_one()) {
-            uint32_t it = 0, at = 0;
+            Ring st{0, 0}, sl{0, 0}, ac{0, 0};
             bool ok = true;
-            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++at) {
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ac.move(1, p.accs)) {
                 const Tile t = tile_of(p, tile, feat_tiles, before);
-                const int as = at % p.accs;
-                ok = mbar_wait(&acc_empty[as], ((at / p.accs) & 1) ^ 1, 2);
+                const int as = ac.at;
+                ok = mbar_wait(&acc_empty[as], ac.phase ^ 1, 2);
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint32_t acc = tmem + acc0 + as * p.tok;
                 const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
-                for (int kb = 0; kb < n_kb; ++kb, ++it) {
-                    const int s = it % p.stages, slot = it % p.slots;
+                for (int kb = 0; kb < n_kb; ++kb, st.move(1, p.stages), sl.move(1, p.slots)) {
+                    const int s = st.at, slot = sl.at;
                     // (the slot's weights came out of the stage: x lies there too)
-                    ok = mbar_wait(&a_full[slot], (it / p.slots) & 1, 3) && mbar_wait(&full[s], (it / p.stages) & 1, 4);
+                    ok = mbar_wait(&a_full[slot], sl.phase, 3) && mbar_wait(&full[s], st.phase, 4);
                     if (!ok) break;
                     tcgen05_fence_after();
                     const uint64_t dx = umma_desc_sw128(smem + (size_t)s * p.stage_bytes);
@@ -222,48 +236,45 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         const uint32_t set = (warp - CONV0) >> 3;
         const int piece = GATED ? upper * 4 + q : q * 2 + upper;
         const uint32_t lanes = (uint32_t)(q * 32 + upper * 16) << 16;
-        uint32_t it = 0;
-        bool ok = true;
-        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-            for (int kb = 0; kb < n_kb; ++kb, ++it) {
-                if (it % CONV_SETS != set) continue;
-                const int s = it % p.stages, slot = it % p.slots;
-                ok = mbar_wait_warp(&full[s], (it / p.stages) & 1, 5);
-                if (!ok) break;
-                const uint8_t* src = smem + (size_t)s * p.stage_bytes + p.x_bytes + piece * PIECE;
-                const uint4 c = *(const uint4*)(src + lane * 16);
-                uint32_t sc[HALF ? 2 : 1];
+        const int my_tiles = (int)blockIdx.x < total ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+        const uint8_t* codes = smem + p.x_bytes + piece * PIECE;
+        Ring st{(int)set, 0}, sl{(int)set, 0};
+        for (int it = set; it < my_tiles * n_kb; it += CONV_SETS, st.move(CONV_SETS, p.stages), sl.move(CONV_SETS, p.slots)) {
+            bool ok = mbar_wait_warp(&full[st.at], st.phase, 5);
+            if (!ok) break;
+            const uint8_t* src = codes + st.at * p.stage_bytes;
+            const uint4 c = *(const uint4*)(src + lane * 16);
+            uint32_t sc[HALF ? 2 : 1];
 #pragma unroll
-                for (int h = 0; h < (HALF ? 2 : 1); ++h) sc[h] = *(const uint32_t*)(src + 512 + (h * 8 + (lane >> 2)) * 4);
-                uint32_t v[16];
+            for (int h = 0; h < (HALF ? 2 : 1); ++h) sc[h] = *(const uint32_t*)(src + 512 + (h * 8 + (lane >> 2)) * 4);
+            uint32_t v[16];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t a = (j < 2 ? c.x : c.y) >> (8 * (j & 1)), b = (j < 2 ? c.z : c.w) >> (8 * (j & 1));
-                    const uint32_t s2 = sc[HALF ? j >> 1 : 0], lo = __byte_perm(s2, 0, 0x1010), hi = __byte_perm(s2, 0, 0x3232);
-                    v[4 * j] = times(q4::pair(a), lo);
-                    v[4 * j + 1] = times(q4::pair(a >> 4), lo);
-                    v[4 * j + 2] = times(q4::pair(b), hi);
-                    v[4 * j + 3] = times(q4::pair(b >> 4), hi);
-                }
-                ok = mbar_wait_warp(&a_empty[slot], ((it / p.slots) & 1) ^ 1, 6);
-                if (!ok) break;
-                tcgen05_fence_after();
-                tmem_st_16x256b_x4(tmem + slot * SLOT_COLS + lanes, v);
-                tmem_st_wait();
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[slot]);
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t a = (j < 2 ? c.x : c.y) >> (8 * (j & 1)), b = (j < 2 ? c.z : c.w) >> (8 * (j & 1));
+                const uint32_t s2 = sc[HALF ? j >> 1 : 0], lo = __byte_perm(s2, 0, 0x1010), hi = __byte_perm(s2, 0, 0x3232);
+                v[4 * j] = times(q4::pair(a), lo);
+                v[4 * j + 1] = times(q4::pair(a >> 4), lo);
+                v[4 * j + 2] = times(q4::pair(b), hi);
+                v[4 * j + 3] = times(q4::pair(b >> 4), hi);
             }
+            ok = mbar_wait_warp(&a_empty[sl.at], sl.phase ^ 1, 6);
+            if (!ok) break;
+            tcgen05_fence_after();
+            tmem_st_16x256b_x4(tmem + sl.at * SLOT_COLS + lanes, v);
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[sl.at]);
         }
     } else {
         // ---- epilogue: warps 2 .. 5, a quarter of the lanes each; a lane is a feature, columns are rows of x
         if (!p.offsets) cj::after_predecessor();
         const int q = warp & 3;
-        uint32_t at = 0;
-        for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++at) {
+        Ring ac{0, 0};
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ac.move(1, p.accs)) {
             const Tile t = tile_of(p, tile, feat_tiles, before);
-            const int as = at % p.accs;
-            if (!mbar_wait_warp(&acc_full[as], (at / p.accs) & 1, 7)) break;
+            const int as = ac.at;
+            if (!mbar_wait_warp(&acc_full[as], ac.phase, 7)) break;
             tcgen05_fence_after();
             const uint32_t src = tmem + acc0 + as * p.tok + ((uint32_t)(q * 32) << 16);
             const int n = t.tok_end - t.tok0;
