@@ -31,9 +31,7 @@ constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
 template <int HD>
 struct Smem {
     static constexpr int TILE = HALF_BYTES * (HD / 64);
-    static constexpr int Q = 0, K = QT * TILE, V = K + STAGES * TILE, TAB = V + STAGES * TILE;
-    // a converting warp's look-ups of two tiles: rows of the planes, the keys' and the values' powers of two
-    static constexpr int TAB_WARP = 2 * BN * (4 + 4 + 4), BAR = TAB + CONV_WARPS * TAB_WARP;
+    static constexpr int Q = 0, K = QT * TILE, V = K + STAGES * TILE, BAR = V + STAGES * TILE;
     static constexpr int TOTAL = BAR + 256 + 1024;
 };
 
@@ -42,7 +40,7 @@ struct Args {
     __nv_bfloat16* out;
     const uint8_t *kplane, *vplane, *kexp, *vexp;
     const int *req_start, *req_prior, *table;
-    int n_requests, table_stride, page_tokens, n_pages, n_heads, n_kv, window;
+    int n_requests, table_stride, page_tokens, page_shift, n_pages, n_heads, n_kv, window;      // page_shift: -1 for a page of no power of two
     float scale_log2;
     int total_rows, block_rows;
 };
@@ -154,56 +152,47 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         constexpr int PIECES = HD / 16;                    // of 16 codes a row
         constexpr int ROWS_WARP = 32 / PIECES, ROWS_PASS = CONV_WARPS * ROWS_WARP, PASSES = (BN + ROWS_PASS - 1) / ROWS_PASS;
         const int piece = lane % PIECES, r0 = warp * ROWS_WARP + lane / PIECES;
-        // This warp's look-ups of tiles i and i + 1 (every warp makes them all: four keys a lane, and no barrier between the warps)
-        int* rows_w = (int*)(smem + S::TAB + warp * S::TAB_WARP);
-        float* kf_w = (float*)(rows_w + 2 * BN);
-        float* vf_w = kf_w + 2 * BN;
-        int page[4], ek[4], ev[4];
-        auto ask_pages = [&](int i) {                      // pages of tile i's keys lane, lane + 32, ...
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = (kt_begin + i) * BN + j * 32 + lane;
-                page[j] = key >= key_from && key <= p_last ? __ldg(tab + key / p.page_tokens) : -1;
-            }
-        };
-        auto ask_exponents = [&](int i) {                  // their rows in the planes (-1: none), exponents on the way
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = (kt_begin + i) * BN + j * 32 + lane;
-                const int row = page[j] >= 0 && page[j] < p.n_pages ? (page[j] * p.n_kv + kvh) * p.page_tokens + key % p.page_tokens : -1;
-                rows_w[(i & 1) * BN + j * 32 + lane] = row;
-                ek[j] = row >= 0 ? (int)p.kexp[row] : 0;
-                ev[j] = row >= 0 ? (int)p.vexp[row] : 0;
-            }
-            __syncwarp();
-        };
-        auto factors = [&](int i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                kf_w[(i & 1) * BN + j * 32 + lane] = __uint_as_float((uint32_t)ek[j] << 23);
-                vf_w[(i & 1) * BN + j * 32 + lane] = __uint_as_float((uint32_t)ev[j] << 23);
-            }
-            __syncwarp();
-        };
-        uint4 kc[PASSES], vc[PASSES];
-        auto load = [&](int i, const uint8_t* plane, uint4 (&c)[PASSES]) {
+        // Every lane looks its own rows of a tile up (the eight or four lanes of a row the same): pages two tiles ahead, exponents and codes one
+        int page[PASSES], at_page[PASSES], row[PASSES];
+        uint32_t ek[PASSES], ev[PASSES];
+        auto ask_pages = [&](int i) {
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
-                const int row = r0 + j * ROWS_PASS < BN ? rows_w[(i & 1) * BN + r0 + j * ROWS_PASS] : -1;
-                c[j] = row >= 0 ? __ldg((const uint4*)(plane + (size_t)row * HD + piece * 16)) : make_uint4(0u, 0u, 0u, 0u);
+                const int r = r0 + j * ROWS_PASS, key = (kt_begin + i) * BN + r;
+                const int n = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_tokens;
+                at_page[j] = key - n * p.page_tokens;
+                page[j] = r < BN && key >= key_from && key <= p_last ? __ldg(tab + n) : -1;
             }
         };
-        auto put = [&](int i, bool values, const uint4 (&c)[PASSES]) -> bool {
+        uint4 kc[PASSES], vc[PASSES];
+        auto load = [&](const uint8_t* plane, uint4 (&c)[PASSES]) {
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j)
+                c[j] = row[j] >= 0 ? __ldg((const uint4*)(plane + (size_t)row[j] * HD + piece * 16)) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        auto ask_keys = [&]() {                            // of the tile whose pages were asked for last; its exponents too
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) row[j] = page[j] >= 0 && page[j] < p.n_pages ? (page[j] * p.n_kv + kvh) * p.page_tokens + at_page[j] : -1;
+            load(p.kplane, kc);
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) ek[j] = row[j] >= 0 ? p.kexp[row[j]] : 0;
+        };
+        auto ask_values = [&]() {
+            load(p.vplane, vc);
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) ev[j] = row[j] >= 0 ? p.vexp[row[j]] : 0;
+        };
+        auto put = [&](int i, bool values, const uint4 (&c)[PASSES], const uint32_t (&exps)[PASSES]) -> bool {
             const int s = i % STAGES;
             if (!mbar_wait_warp(values ? &v_empty[s] : &k_empty[s], ((i / STAGES) & 1) ^ 1, 11)) return false;
             uint8_t* half = smem + (values ? S::V : S::K) + s * TILE + (piece >> 2) * HALF_BYTES;
-            const float* factor = (values ? vf_w : kf_w) + (i & 1) * BN;
             const int chunk = (piece & 3) * 2;
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
                 const int r = r0 + j * ROWS_PASS;
                 if (r >= BN) break;
-                const f32x2 f = pack2(factor[r], factor[r]);
+                const float scale = __uint_as_float(exps[j] << 23);
+                const f32x2 f = pack2(scale, scale);
                 const uint2 a = scaled_codes(c[j].x, f), b = scaled_codes(c[j].y, f), d = scaled_codes(c[j].z, f), e = scaled_codes(c[j].w, f);
                 *(uint4*)(half + r * 128 + ((chunk ^ (r & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
                 *(uint4*)(half + r * 128 + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
@@ -215,24 +204,23 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         // in the order the products want them: K0, V0, K1, V1, ...  While the values of a tile are converted the next tile's keys and
         // exponents and the pages of the one after are on their way; while those keys are, their values
         ask_pages(0);
-        ask_exponents(0);
-        load(0, p.kplane, kc);
-        load(0, p.vplane, vc);
-        if (n_tiles > 1) ask_pages(1);
-        factors(0);
-        bool ok = put(0, false, kc);
+        ask_keys();
+        ask_values();
+        ask_pages(1);
+        bool ok = put(0, false, kc, ek);
         for (int i = 0; i < n_tiles && ok; ++i) {
             const bool next = i + 1 < n_tiles;
+            uint32_t ev_now[PASSES];
+#pragma unroll
+            for (int j = 0; j < PASSES; ++j) ev_now[j] = ev[j];
             if (next) {
-                ask_exponents(i + 1);
-                load(i + 1, p.kplane, kc);
-                if (i + 2 < n_tiles) ask_pages(i + 2);
+                ask_keys();
+                ask_pages(i + 2);
             }
-            ok = put(i, true, vc);
+            ok = put(i, true, vc, ev_now);
             if (!ok || !next) break;
-            factors(i + 1);
-            load(i + 1, p.vplane, vc);
-            ok = put(i + 1, false, kc);
+            ask_values();
+            ok = put(i + 1, false, kc, ek);
         }
     } else if (warp == PRODUCT) {
         // ---- products, in the order S_a(0) S_b(0), then per key tile i: PV_a(i) S_a(i + 1) PV_b(i) S_b(i + 1), each PV in two halves of
@@ -451,7 +439,8 @@ CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, c
     CUtensorMap map_q;
     if (!make_map_bf16(&map_q, q, total_rows, (long long)n_heads * hd, (long long)n_heads * hd, BM)) return CJ_ERR_ARG;
     const Args a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane, (const uint8_t*)vplane, (const uint8_t*)kexp,
-                 (const uint8_t*)vexp, req_start, req_prior, table, n_requests, table_stride, page_tokens, n_pages, n_heads, n_kv, window,
+                 (const uint8_t*)vexp, req_start, req_prior, table, n_requests, table_stride, page_tokens,
+                 (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, n_pages, n_heads, n_kv, window,
                  scale * 1.4426950408889634f, total_rows, block_rows};
     auto kern = hd == 128 ? prefill_e4m3_tc_kernel<128> : prefill_e4m3_tc_kernel<64>;
     const int smem = hd == 128 ? Smem<128>::TOTAL : Smem<64>::TOTAL;
