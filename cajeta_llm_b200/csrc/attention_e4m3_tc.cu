@@ -5,10 +5,11 @@
 //     P = exp2(S scale - m)           four warps a query tile, a row a thread; P as bfloat16 over the columns of its scores
 //     O += P . (code_v 2^e_v)         O in tensor memory
 // A code times its power of two is a bfloat16 number exactly, whatever the exponents of the tokens beside it (f16 would keep more bits of P,
-// but only values within 22 octaves of each other: a row's values could vanish beside larger ones that it does not even see).  So seven warps
+// but only values within 22 octaves of each other: a row's values could vanish beside larger ones that it does not even see).  So six warps
 // turn codes into the bfloat16 tiles in shared memory that both products read, and the rest is attention over a bfloat16 cache: P, as there, is
-// the one rounding.  The codes come with plain 16-byte loads, pages of any size, a tile's keys in registers while its predecessor's values are
-// converted (half the bytes of a bfloat16 cache: 16 KB a tile).  The two query tiles take turns between the exponential unit and the tensor
+// the one rounding.  The codes come by bulk copies of a page's run of rows, pages of any size, one warp's work: a tile's keys travel while its
+// predecessor's values are converted (half the bytes of a bfloat16 cache: 16 KB a tile; plain loads into registers, tried first, held the
+// conversions of the tile before up: 290 us where this takes 215).  The two query tiles take turns between the exponential unit and the tensor
 // core, each key tile is worked on as two halves of 64 keys, and the reference maximum moves only when it grows by more than 2^8.
 // Every wait is bounded (tc_common.cuh).
 #define CJ_LIB "attention_e4m3_tc"
@@ -22,7 +23,7 @@ namespace {
 
 constexpr int BM = 128, QT = 2, BN = 128;         // query rows a tile, tiles a block, keys a tile
 constexpr int STAGES = 2;
-constexpr int CONV_WARPS = 7, PRODUCT = 7, SOFT0 = 8;
+constexpr int CONV_WARPS = 6, LOADER = 6, PRODUCT = 7, SOFT0 = 8;
 constexpr int THREADS = 16 * 32;
 constexpr int HALF_BYTES = 128 * 64 * 2;          // [128 x 64] f16, swizzled: 16 KB
 constexpr float RESCALE_THRESHOLD = 8.0f;         // in log2 units
@@ -31,7 +32,8 @@ constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
 template <int HD>
 struct Smem {
     static constexpr int TILE = HALF_BYTES * (HD / 64);
-    static constexpr int Q = 0, K = QT * TILE, V = K + STAGES * TILE, BAR = V + STAGES * TILE;
+    static constexpr int Q = 0, K = QT * TILE, V = K + STAGES * TILE;
+    static constexpr int CODES = V + STAGES * TILE, FACTORS = CODES + 2 * BN * HD, BAR = FACTORS + 2 * BN * 4;      // a tile's keys, and its values
     static constexpr int TOTAL = BAR + 256 + 1024;
 };
 
@@ -48,6 +50,11 @@ struct Args {
 struct QueryTile {
     int rows, p0, begin, end;      // rows of the step (0: empty), position of the first, key tiles [begin, end] of the block's
 };
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
 
 // four codes times a power of two, as bfloat16
 __device__ __forceinline__ uint2 scaled_codes(uint32_t w, f32x2 f) {
@@ -125,11 +132,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     uint64_t* p_full = s_full + QT;               // [QT][2] the weights of a tile's first / last 64 keys are written
     uint64_t* half_done = p_full + 2 * QT;        // [QT] the output product over a tile's first 64 keys is done
     uint64_t* o_done = half_done + QT;            // [QT] the last output product is done
-    uint32_t* tmem_slot = (uint32_t*)(o_done + QT);
+    uint64_t* c_full = o_done + QT;               // [2] a tile's codes (of keys, of values) have landed, their powers of two are written
+    uint64_t* c_empty = c_full + 2;               // [2] they are converted
+    uint32_t* tmem_slot = (uint32_t*)(c_empty + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
+        for (int s = 0; s < 2; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], CONV_WARPS);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&k_full[s], CONV_WARPS * 32), mbar_init(&k_empty[s], 1);
             mbar_init(&v_full[s], CONV_WARPS * 32), mbar_init(&v_empty[s], 1);
@@ -148,80 +158,93 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp < CONV_WARPS) {
-        // ---- codes -> f16 tiles ----------------------------------------------------------------------
-        constexpr int PIECES = HD / 16;                    // of 16 codes a row
-        constexpr int ROWS_WARP = 32 / PIECES, ROWS_PASS = CONV_WARPS * ROWS_WARP, PASSES = (BN + ROWS_PASS - 1) / ROWS_PASS;
-        const int piece = lane % PIECES, r0 = warp * ROWS_WARP + lane / PIECES;
-        // Every lane looks its own rows of a tile up (the eight or four lanes of a row the same): pages two tiles ahead, exponents and codes one
-        int page[PASSES], at_page[PASSES], row[PASSES];
-        uint32_t ek[PASSES], ev[PASSES];
-        auto ask_pages = [&](int i) {
+        // ---- codes -> bfloat16 tiles: 16 codes of a row a lane, in the order the products want the tiles: K0, V0, K1, V1, ...
+        constexpr int PIECES = HD / 16, ROWS_WARP = 32 / PIECES, ROWS_PASS = CONV_WARPS * ROWS_WARP, PASSES = (BN + ROWS_PASS - 1) / ROWS_PASS;
+        // (eight lanes that are served together take two rows and, of eight pieces, other halves of them: no two in one bank, coming or going)
+        const int in_warp = PIECES == 8 ? lane >> 2 & 3 : lane >> 2;
+        const int piece = PIECES == 8 ? ((lane & 3) | (lane >> 4 << 2)) ^ ((in_warp & 1) << 2) : lane & 3;
+        const int chunk = (piece & 3) * 2, r0 = warp * ROWS_WARP + in_warp;
+        const float* factors = (const float*)(smem + S::FACTORS);
+        bool ok = true;
+        for (int i = 0; i < 2 * n_tiles && ok; ++i) {
+            const int values = i & 1, t = i >> 1, s = t % STAGES;
+            ok = mbar_wait_warp(&c_full[values], t & 1, 10) && mbar_wait_warp(values ? &v_empty[s] : &k_empty[s], ((t / STAGES) & 1) ^ 1, 11);
+            if (!ok) break;
+            const uint8_t* codes = smem + S::CODES + values * BN * HD + piece * 16;
+            uint8_t* dst = smem + (values ? S::V : S::K) + s * TILE + (piece >> 2) * HALF_BYTES;
+            // (the passes' chains side by side: all loads first, and only the last pass may have no row)
+            uint4 c[PASSES];
+            float scale[PASSES];
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
-                const int r = r0 + j * ROWS_PASS, key = (kt_begin + i) * BN + r;
-                const int n = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_tokens;
-                at_page[j] = key - n * p.page_tokens;
-                page[j] = r < BN && key >= key_from && key <= p_last ? __ldg(tab + n) : -1;
+                const int r = min(r0 + j * ROWS_PASS, BN - 1);
+                c[j] = *(const uint4*)(codes + r * HD);
+                scale[j] = factors[values * BN + r];
             }
-        };
-        uint4 kc[PASSES], vc[PASSES];
-        auto load = [&](const uint8_t* plane, uint4 (&c)[PASSES]) {
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j)
-                c[j] = row[j] >= 0 ? __ldg((const uint4*)(plane + (size_t)row[j] * HD + piece * 16)) : make_uint4(0u, 0u, 0u, 0u);
-        };
-        auto ask_keys = [&]() {                            // of the tile whose pages were asked for last; its exponents too
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) row[j] = page[j] >= 0 && page[j] < p.n_pages ? (page[j] * p.n_kv + kvh) * p.page_tokens + at_page[j] : -1;
-            load(p.kplane, kc);
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) ek[j] = row[j] >= 0 ? p.kexp[row[j]] : 0;
-        };
-        auto ask_values = [&]() {
-            load(p.vplane, vc);
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) ev[j] = row[j] >= 0 ? p.vexp[row[j]] : 0;
-        };
-        auto put = [&](int i, bool values, const uint4 (&c)[PASSES], const uint32_t (&exps)[PASSES]) -> bool {
-            const int s = i % STAGES;
-            if (!mbar_wait_warp(values ? &v_empty[s] : &k_empty[s], ((i / STAGES) & 1) ^ 1, 11)) return false;
-            uint8_t* half = smem + (values ? S::V : S::K) + s * TILE + (piece >> 2) * HALF_BYTES;
-            const int chunk = (piece & 3) * 2;
 #pragma unroll
             for (int j = 0; j < PASSES; ++j) {
                 const int r = r0 + j * ROWS_PASS;
-                if (r >= BN) break;
-                const float scale = __uint_as_float(exps[j] << 23);
-                const f32x2 f = pack2(scale, scale);
+                if (scale[j] == 0.0f) c[j] = make_uint4(0u, 0u, 0u, 0u);    // (no key: the codes are what was there before)
+                const f32x2 f = pack2(scale[j], scale[j]);
                 const uint2 a = scaled_codes(c[j].x, f), b = scaled_codes(c[j].y, f), d = scaled_codes(c[j].z, f), e = scaled_codes(c[j].w, f);
-                *(uint4*)(half + r * 128 + ((chunk ^ (r & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
-                *(uint4*)(half + r * 128 + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+                if (j < PASSES - 1 || r < BN) {
+                    *(uint4*)(dst + r * 128 + ((chunk ^ (r & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+                    *(uint4*)(dst + r * 128 + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+                }
             }
             fence_async_shared();
             mbar_arrive(values ? &v_full[s] : &k_full[s]);
-            return true;
-        };
-        // in the order the products want them: K0, V0, K1, V1, ...  While the values of a tile are converted the next tile's keys and
-        // exponents and the pages of the one after are on their way; while those keys are, their values
-        ask_pages(0);
-        ask_keys();
-        ask_values();
-        ask_pages(1);
-        bool ok = put(0, false, kc, ek);
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            const bool next = i + 1 < n_tiles;
-            uint32_t ev_now[PASSES];
-#pragma unroll
-            for (int j = 0; j < PASSES; ++j) ev_now[j] = ev[j];
-            if (next) {
-                ask_keys();
-                ask_pages(i + 2);
-            }
-            ok = put(i, true, vc, ev_now);
-            if (!ok || !next) break;
-            ask_values();
-            ok = put(i + 1, false, kc, ek);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c_empty[values]);
         }
+    } else if (warp == LOADER) {
+        // ---- look-ups and copies: lane l has keys l, l + 32, ... of a tile; the first key of a page's run (within 32) copies it
+        float* factors = (float*)(smem + S::FACTORS);
+        int page[4], at_page[4];
+        auto ask_pages = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = (kt_begin + i) * BN + j * 32 + lane;
+                const int n = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_tokens;
+                at_page[j] = key - n * p.page_tokens;
+                page[j] = key >= key_from && key <= p_last ? __ldg(tab + n) : -1;
+            }
+        };
+        ask_pages(0);
+        bool ok = true;
+        for (int i = 0; i < n_tiles && ok; ++i) {
+            int row[4], run[4], have = 0;
+            uint32_t ek[4], ev[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = (kt_begin + i) * BN + j * 32 + lane;
+                row[j] = page[j] >= 0 && page[j] < p.n_pages ? (page[j] * p.n_kv + kvh) * p.page_tokens + at_page[j] : -1;
+                ek[j] = row[j] >= 0 ? p.kexp[row[j]] : 0;
+                ev[j] = row[j] >= 0 ? p.vexp[row[j]] : 0;
+                const bool first = row[j] >= 0 && (lane == 0 || at_page[j] == 0 || key == key_from);
+                run[j] = first ? min(min(p.page_tokens - at_page[j], 32 - lane), p_last + 1 - key) : 0;
+                have += __popc(__ballot_sync(0xffffffffu, row[j] >= 0));
+            }
+            if (i + 1 < n_tiles) ask_pages(i + 1);
+#pragma unroll
+            for (int values = 0; values < 2; ++values) {
+                if (ok) ok = mbar_wait_warp(&c_empty[values], (i & 1) ^ 1, 12);
+                if (!ok) break;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) factors[values * BN + j * 32 + lane] = __uint_as_float((values ? ev[j] : ek[j]) << 23);
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(&c_full[values], have * HD);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (run[j] > 0)
+                        bulk_load(smem + S::CODES + (values * BN + j * 32 + lane) * HD, (values ? p.vplane : p.kplane) + (size_t)row[j] * HD,
+                                  run[j] * HD, &c_full[values]);
+            }
+        }
+        // (the copies under way end before the block does: the converting warps wait for each, unless a wait ran out)
+        if (!ok)
+            for (int values = 0; values < 2; ++values) mbar_wait_warp(&c_full[values], 0, 14), mbar_wait_warp(&c_full[values], 1, 14);
     } else if (warp == PRODUCT) {
         // ---- products, in the order S_a(0) S_b(0), then per key tile i: PV_a(i) S_a(i + 1) PV_b(i) S_b(i + 1), each PV in two halves of
         // 64 keys.  S_g(i + 1) overwrites the columns PV_g(i) reads P from; one thread's products run in the order they were issued
@@ -326,40 +349,35 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
                     for (int c = 0; c < HC; ++c)
                         if (!((unsigned)(half * HC + c - lo) <= (unsigned)span && span >= 0)) v[c] = 0xff800000u;       // -inf
                 }
-                // one pass with the reference maximum so far; again only where these keys raise it by more than the threshold
-                float m_use = m_ref, factor = 1.0f, sum;
-                bool rescale = false;
-                uint32_t packed[HC];                   // only [0, 32) is used
-#pragma unroll 1
-                for (int attempt = 0;; ++attempt) {
-                    const float neg_sub = m_use == -INFINITY ? 0.0f : -m_use;
-                    const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2), sub2 = pack2(neg_sub, neg_sub);
-                    f32x2 sum2a = pack2(0.0f, 0.0f), sum2b = sum2a;
-                    float mx0 = -INFINITY, mx1 = -INFINITY;
+                // The largest score first, in four chains of three-way maxima, then one pass of exponentials.  (One pass with the reference
+                // maximum so far, which finds the largest on its way and is repeated where that moves the reference, is shorter by the wait for
+                // the maximum, but a warp repeats it for any of its 32 rows: keys of uneven lengths, 2,048 rows behind 4,096, took 300 us.)
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < HC; c += 4) {
-                        const float2 t0 = unpack2(fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, sub2));
-                        const float2 t1 = unpack2(fma2(pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, sub2));
-                        const float e0 = ex2(t0.x), e1 = ex2(t0.y), e2 = ex2(t1.x), e3 = ex2(t1.y);
-                        sum2a = add2(sum2a, pack2(e0, e1));
-                        sum2b = add2(sum2b, pack2(e2, e3));
-                        const __nv_bfloat162 b0 = __floats2bfloat162_rn(e0, e1), b1 = __floats2bfloat162_rn(e2, e3);
-                        packed[c >> 1] = *(const uint32_t*)&b0;
-                        packed[(c >> 1) + 1] = *(const uint32_t*)&b1;
-                        mx0 = max3(mx0, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-                        mx1 = max3(mx1, __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
-                    }
-                    const float2 sa = unpack2(sum2a), sb = unpack2(sum2b);
-                    sum = (sa.x + sa.y) + (sb.x + sb.y);
-                    if (attempt == 1) break;
-                    const float mx = fmaxf(mx0, mx1) * p.scale_log2;
-                    float m_new = m_ref;
-                    if (mx > m_ref + RESCALE_THRESHOLD || m_ref == -INFINITY) m_new = fmaxf(m_ref, mx);
-                    if (!__any_sync(0xffffffffu, m_new != m_ref)) break;
-                    rescale = m_new != m_ref && m_ref != -INFINITY;
-                    factor = rescale ? exp2f(m_ref - m_new) : 1.0f;
-                    m_use = m_new;
+                for (int c = 0; c < HC; c += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1]));
+                const float largest = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
+                const bool rescale = largest > m_ref + RESCALE_THRESHOLD && m_ref != -INFINITY;
+                const float m_use = rescale || m_ref == -INFINITY ? fmaxf(m_ref, largest) : m_ref;
+                const float factor = rescale ? exp2f(m_ref - m_use) : 1.0f;
+                const float neg_sub = m_use == -INFINITY ? 0.0f : -m_use;
+                const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2), sub2 = pack2(neg_sub, neg_sub);
+                f32x2 sum2a = pack2(0.0f, 0.0f), sum2b = sum2a;
+                uint32_t packed[HC / 2];
+#pragma unroll
+                for (int c = 0; c < HC; c += 4) {
+                    const float2 t0 = unpack2(fma2(pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, sub2));
+                    const float2 t1 = unpack2(fma2(pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, sub2));
+                    const float e0 = ex2(t0.x), e1 = ex2(t0.y), e2 = ex2(t1.x), e3 = ex2(t1.y);
+                    sum2a = add2(sum2a, pack2(e0, e1));
+                    sum2b = add2(sum2b, pack2(e2, e3));
+                    const __nv_bfloat162 b0 = __floats2bfloat162_rn(e0, e1), b1 = __floats2bfloat162_rn(e2, e3);
+                    packed[c >> 1] = *(const uint32_t*)&b0;
+                    packed[(c >> 1) + 1] = *(const uint32_t*)&b1;
                 }
+                const float2 sa = unpack2(sum2a), sb = unpack2(sum2b);
+                const float sum = (sa.x + sa.y) + (sb.x + sb.y);
                 tmem_st32<0>(s_addr + half * (HC / 2), packed);
                 l = l * factor + sum;
                 m_ref = m_use;
