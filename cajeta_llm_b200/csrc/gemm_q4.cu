@@ -44,7 +44,7 @@ struct Args {
 // NTOK: rows of x a block takes at a time; WM: pieces of 16 features a block takes of each weight; HALF: groups of 32; AHEAD: tiles along K whose codes
 // a warp has asked for before it multiplies the first
 template <int NTOK, int WM, bool GATED, bool HALF, int AHEAD>
-__global__ void __launch_bounds__(WARPS * 32) gemm_q4_kernel(const Args a) {
+__global__ void __launch_bounds__(WARPS * 32, NTOK == 8 && AHEAD == 1 ? 4 : 0) gemm_q4_kernel(const Args a) {
     constexpr int NB = NTOK / 8, W = GATED ? 2 : 1, PIECE = q4::piece_bytes(HALF);
     constexpr int GRP = HALF ? 2 : 1;                      // groups of a tile
     extern __shared__ float red[];                         // [WARPS][W][WM * 16][NTOK + 1]
@@ -289,9 +289,10 @@ CJ_EXPORT int cj_q4_quantise(const void* w, int dtype, void* codes, float* scale
 
 // x bf16 [x_rows, ldx], w (w_up) in the layout; out float32 or bf16 [rows, ldo].  offsets: null or int32 [groups + 1]; index: null
 // or int32 [rows] (an index outside x reads zeros).  K a multiple of four, x and ldx of 8 bytes.  w_up: out = silu(x w) (x w_up).
+// n_tok: rows of x a block takes at a time, 8, 16 or 32; ahead: tiles along K whose codes are asked for ahead, 4 or 1 (plain products of eight rows).
 CJ_EXPORT int cj_gemm_q4(const void* x, long long ldx, int x_rows, const void* w, const void* w_up, const float* bias, void* out, int out_dtype,
                          long long ldo, int rows, int features, int K, int groups, int half, const int* offsets, const int* index,
-                         int accumulate, int n_tok, int pieces, cudaStream_t stream) {
+                         int accumulate, int n_tok, int ahead, cudaStream_t stream) {
     if (rows <= 0) return 0;
     if (!x || !w || !out || features <= 0 || K <= 0 || groups <= 0 || x_rows <= 0) return CJ_ERR_ARG;
     if (out_dtype != CJ_F32 && out_dtype != CJ_BF16) return CJ_ERR_DTYPE;
@@ -313,16 +314,21 @@ CJ_EXPORT int cj_gemm_q4(const void* x, long long ldx, int x_rows, const void* w
         cj::launch(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, dim3((all + WM - 1) / WM, groups, row_tiles), dim3(WARPS * 32), smem, stream, a); \
         return launch_status();                                                                                           \
     }
-#define PICK(NTOK, WM, AHEAD)                                                                                                    \
-    if (n_tok == NTOK && pieces == WM) {                                                                                  \
-        if (w_up) { if (half) LAUNCH(NTOK, WM, true, true, AHEAD) else LAUNCH(NTOK, WM, true, false, AHEAD) }                           \
-        else { if (half) LAUNCH(NTOK, WM, false, true, AHEAD) else LAUNCH(NTOK, WM, false, false, AHEAD) }                              \
+#define PLAIN(NTOK, WM, AHEAD) { if (half) LAUNCH(NTOK, WM, false, true, AHEAD) else LAUNCH(NTOK, WM, false, false, AHEAD) }
+#define GATED(NTOK, WM, AHEAD) { if (half) LAUNCH(NTOK, WM, true, true, AHEAD) else LAUNCH(NTOK, WM, true, false, AHEAD) }
+    // rows at a time, pieces of 16 features, tiles ahead
+    if (w_up) {
+        if (n_tok == 8) GATED(8, 1, 1)
+        if (n_tok == 16) GATED(16, 2, 2)
+        if (n_tok == 32) GATED(32, 2, 1)
+    } else {
+        if (n_tok == 8 && ahead == 4) PLAIN(8, 1, 4)
+        if (n_tok == 8) PLAIN(8, 1, 1)
+        if (n_tok == 16) PLAIN(16, 2, 2)
+        if (n_tok == 32) PLAIN(32, 2, 1)
     }
-    PICK(8, 1, 4)
-    PICK(8, 2, 2)
-    PICK(16, 2, 2)
-    PICK(32, 2, 1)
-#undef PICK
+#undef GATED
+#undef PLAIN
 #undef LAUNCH
     return CJ_ERR_SIZE;
 }

@@ -1831,12 +1831,12 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
     splits = splits or e4m3_splits(T, n_heads, n_kv, min(window, max_context) if window > 0 else max(1, max_context), _sm_count())
     acc = ml = None
     if splits > 1:
-        acc = torch.empty((T, n_heads, splits, head_dim), dtype=torch.float32, device=q.device)
-        ml = torch.empty((T, n_heads, splits, 2), dtype=torch.float32, device=q.device)
+        acc = q.new_empty((T * n_heads * splits * (head_dim + 2),), dtype=torch.float32)       # the blocks' sums, then their maxima and divisors
+        ml = acc.data_ptr() + 4 * T * n_heads * splits * head_dim
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
         q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
         positions.data_ptr(), row_req.data_ptr(), None, None, table.shape[0], table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv,
-        head_dim, window, scale, splits, _at(acc), _at(ml), _raw())
+        head_dim, window, scale, splits, _at(acc), ml, _raw())
     _check(st, "decode_attention_e4m3")
     if splits > 1:
         global launches
@@ -2042,8 +2042,11 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
         _check(st, "gemm_q4")
         return
     n_tok = 8 if M <= 8 or group_offsets is not None and M <= 4 * w.groups else 16 if M <= 16 else 32
-    pieces = 1 if n_tok == 8 else 2
+    # Few blocks hide their own loads' time, four tiles ahead; where there are more than four an SM they hide each other's, with registers for that many
+    # (us, four tiles and one: 1 row x 2,048 x 6,144 4.3 and 5.1; 8 rows' experts of 1,408 x 2,048, gated, 28.9 and 21.6, one row's 14.1 and 11.1)
+    blocks = (min(M, w.groups) if group_offsets is not None else -(-M // 8)) * -(-w.features // 16)
+    ahead = 4 if blocks < 4 * _sm_count() else 1
     st = _entry("gemm_q4", "cj_gemm_q4", "plippppiliiiiippiiip")(
         a.data_ptr(), a.stride(0), a.shape[0], w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
-        out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), _at(a_row_index), 1 if accumulate else 0, n_tok, pieces, _raw())
+        out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), _at(a_row_index), 1 if accumulate else 0, n_tok, ahead, _raw())
     _check(st, "gemm_q4")
