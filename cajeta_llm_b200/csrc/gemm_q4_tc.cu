@@ -40,6 +40,10 @@ struct Args {
     int tok;                   // rows of x a tile takes
     int stages, slots, accs;   // ring of shared memory, ring of tensor memory, accumulators
     int x_bytes, stage_bytes;
+    // A float32 result's K goes in parts of so many blocks of 64, each summed from zero and added to what the parts before left: tcgen05 cuts its sums off
+    // rather than rounding them, and an error that grows with their length stays that of 2,560 entries (2,048 x 3,584 x 3,584: 1.2e-6 of the result
+    // in one part, 7e-7 in two).
+    int part_kb;
 };
 
 struct Tile {
@@ -205,15 +209,17 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         if (elect_one()) {
             Ring st{0, 0}, sl{0, 0}, ac{0, 0};
             bool ok = true;
-            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ac.move(1, p.accs)) {
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 const Tile t = tile_of(p, tile, feat_tiles, before);
-                const int as = ac.at;
-                ok = mbar_wait(&acc_empty[as], ac.phase ^ 1, 2);
-                if (!ok) break;
-                tcgen05_fence_after();
-                const uint32_t acc = tmem + acc0 + as * p.tok;
+                uint32_t acc = 0;
+                int part = 0;                 // blocks of K in the accumulator
                 const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
                 for (int kb = 0; kb < n_kb; ++kb, st.move(1, p.stages), sl.move(1, p.slots)) {
+                    if (part == 0) {
+                        ok = mbar_wait(&acc_empty[ac.at], ac.phase ^ 1, 2);
+                        if (!ok) break;
+                        acc = tmem + acc0 + ac.at * p.tok;
+                    }
                     const int s = st.at, slot = sl.at;
                     // (the slot's weights came out of the stage: x lies there too)
                     ok = mbar_wait(&a_full[slot], sl.phase, 3) && mbar_wait(&full[s], st.phase, 4);
@@ -222,11 +228,15 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                     const uint64_t dx = umma_desc_sw128(smem + (size_t)s * p.stage_bytes);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        umma_bf16_a_tmem(acc, tmem + slot * SLOT_COLS + 8 * k, dx + 2 * k, idesc, (kb | k) ? 1u : 0u);
+                        umma_bf16_a_tmem(acc, tmem + slot * SLOT_COLS + 8 * k, dx + 2 * k, idesc, (part | k) ? 1u : 0u);
                     umma_commit(&empty[s]);
                     umma_commit(&a_empty[slot]);
+                    if (++part == p.part_kb || kb == n_kb - 1) {
+                        umma_commit(&acc_full[ac.at]);
+                        ac.move(1, p.accs);
+                        part = 0;
+                    }
                 }
-                if (ok) umma_commit(&acc_full[as]);
             }
         }
     } else if (warp >= CONV0) {
@@ -271,16 +281,20 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         if (!p.offsets) cj::after_predecessor();
         const int q = warp & 3;
         Ring ac{0, 0};
-        for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ac.move(1, p.accs)) {
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x)
+        for (int kb = 0; kb < n_kb; kb += p.part_kb, ac.move(1, p.accs)) {
             const Tile t = tile_of(p, tile, feat_tiles, before);
             const int as = ac.at;
-            if (!mbar_wait_warp(&acc_full[as], ac.phase, 7)) break;
+            const bool add = p.accumulate || kb > 0;
+            ok = mbar_wait_warp(&acc_full[as], ac.phase, 7);
+            if (!ok) break;
             tcgen05_fence_after();
             const uint32_t src = tmem + acc0 + as * p.tok + ((uint32_t)(q * 32) << 16);
             const int n = t.tok_end - t.tok0;
             const int feature = GATED ? t.f * 64 + q * 16 + (lane & 15) : t.f * 128 + q * 32 + lane;
             const bool in = feature < p.features;
-            const float bias = !GATED && p.bias && in ? p.bias[feature] : 0.0f;
+            const float bias = !GATED && p.bias && in && kb == 0 ? p.bias[feature] : 0.0f;
 #pragma unroll 1
             for (int c0 = 0; c0 < n; c0 += 16) {
                 uint32_t v[16];
@@ -303,22 +317,25 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                         }
                     }
                 } else if (in) {
-                    const size_t o = (size_t)(t.tok0 + c0) * p.ldo + feature;
+                    // (adding by a reduction in L2: nobody else writes these entries, so the sums are those of a load, an addition and a store in
+                    // their order, without the wait for the load)
+                    const int left = n - c0;
                     if (p.half_out) {
+                        __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)(t.tok0 + c0) * p.ldo + feature;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (c0 + j < n) ((__nv_bfloat16*)p.out)[o + (size_t)j * p.ldo] = __float2bfloat16_rn(__uint_as_float(v[j]) + bias);
-                    } else if (p.accumulate) {
-                        float old[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) old[j] = c0 + j < n ? ((const float*)p.out)[o + (size_t)j * p.ldo] : 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (c0 + j < n) ((float*)p.out)[o + (size_t)j * p.ldo] = old[j] + (__uint_as_float(v[j]) + bias);
+                        for (int j = 0; j < 16; ++j, dst += p.ldo)
+                            if (j < left) *dst = __float2bfloat16_rn(__uint_as_float(v[j]) + bias);
                     } else {
+                        float* dst = (float*)p.out + (size_t)(t.tok0 + c0) * p.ldo + feature;
+                        if (add) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (c0 + j < n) ((float*)p.out)[o + (size_t)j * p.ldo] = __uint_as_float(v[j]) + bias;
+                            for (int j = 0; j < 16; ++j, dst += p.ldo)
+                                if (j < left) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(dst), "f"(__uint_as_float(v[j]) + bias) : "memory");
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j, dst += p.ldo)
+                                if (j < left) *dst = __uint_as_float(v[j]) + bias;
+                        }
                     }
                 }
             }
@@ -375,7 +392,9 @@ CJ_EXPORT int cj_gemm_q4_tc(const void* x, long long ldx, int x_rows, const void
     CUtensorMap map;
     if (!make_map_bf16(&map, x, x_rows, K, ldx, tok)) return CJ_ERR_ARG;
     Args a{(const uint8_t*)w, (const uint8_t*)w_up, bias, out, offsets, ldo, rows, features, K, groups, out_dtype == CJ_BF16 ? 1 : 0, accumulate,
-           tok, 0, 0, 0, tok * 128, 0};
+           tok, 0, 0, 0, tok * 128, 0, 0};
+    const int n_kb = (K + 63) / 64, parts = out_dtype == CJ_F32 && !w_up ? (n_kb + 39) / 40 : 1;
+    a.part_kb = (n_kb + parts - 1) / parts;
     a.stage_bytes = a.x_bytes + (q4::tile_bytes(half != 0) + 1023) / 1024 * 1024;
     a.stages = min(MAX_STAGES, (SMEM_LIMIT - 1024 - BAR_BYTES) / a.stage_bytes);
     // two accumulators where at least three slots of weights fit beside them

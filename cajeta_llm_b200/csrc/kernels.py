@@ -1969,7 +1969,12 @@ class Q4Weight:
         return math.prod(self.shape)
 
 
-Q4_TC_ROWS = 32      # rows (of a group, on average) from which on a product with 4-bit weights runs on tcgen05
+def q4_on_tcgen05(rows: int, features: int, groups: int) -> bool:
+    """Whether a product with 4-bit weights has rows enough for the form that puts them on the columns of tcgen05 products (``groups`` 0: dense)."""
+    # Its tiles take 12 us at K 2,048 whatever their rows, the other form's work grows with them.  (us, tcgen05 and the other: dense, 6,144 features x 2,048,
+    # 24 rows 12.4 and 11.4, 32 rows 12.4 and 12.9, 64 rows 12.9 and 18.8; 2,048 features, 64 rows 11.8 and 7.2, 128 rows 12.7 and 12.1; 60 gated
+    # experts of 1,408 x 2,048, two rows each 60 and 40, four 69 and 84, seventeen 92 and 136)
+    return rows > 4 * groups if groups else rows > 8 and rows * features > 190_000
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2026,8 +2031,7 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
     if a.shape[0] == 0:
         raise KernelError("gemm_q4: a has no rows")
     half = 1 if w.group == 32 else 0
-    per_group = M / w.groups
-    if per_group > Q4_TC_ROWS and a.stride(0) % 8 == 0 and a.data_ptr() % 16 == 0:
+    if q4_on_tcgen05(M, w.features, w.groups if group_offsets is not None else 0) and a.stride(0) % 8 == 0 and a.data_ptr() % 16 == 0:
         global launches
         x, x_rows = a, a.shape[0]
         if a_row_index is not None:
@@ -2041,7 +2045,7 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
             out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), 1 if accumulate else 0, tok, _sm_count(), _raw())
         _check(st, "gemm_q4")
         return
-    n_tok = 8 if M <= 8 or group_offsets is not None and M <= 4 * w.groups else 16 if M <= 16 else 32
+    n_tok = 8 if M <= 8 or group_offsets is not None else 16 if M <= 16 else 32
     # Few blocks hide their own loads' time, four tiles ahead; where there are more than four an SM they hide each other's, with registers for that many
     # (us, four tiles and one: 1 row x 2,048 x 6,144 4.3 and 5.1; 8 rows' experts of 1,408 x 2,048, gated, 28.9 and 21.6, one row's 14.1 and 11.1)
     blocks = (min(M, w.groups) if group_offsets is not None else -(-M // 8)) * -(-w.features // 16)

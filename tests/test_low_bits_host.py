@@ -161,6 +161,15 @@ def test_blocks_a_row():
         assert 1 <= K.e4m3_splits(rows, 28, 4, span, 148) <= max(1, -(-span // 128))
 
 
+def test_which_form_a_4_bit_product_takes():
+    assert not K.q4_on_tcgen05(1, 151_936, 0) and not K.q4_on_tcgen05(8, 151_936, 0) and not K.q4_on_tcgen05(64, 2048, 0)
+    assert K.q4_on_tcgen05(64, 6144, 0) and K.q4_on_tcgen05(2048, 512, 0)
+    assert not K.q4_on_tcgen05(32, 1408, 60) and K.q4_on_tcgen05(8192, 1408, 60)
+    for rows, features, groups, gated in ((2048, 3584, 0, False), (100, 70, 0, True), (8192, 1408, 60, True), (300, 9, 4, False)):
+        tok = K.q4_tile_rows(rows, features, groups, gated, 148)
+        assert tok % 16 == 0 and 16 <= tok <= 256
+
+
 def test_what_a_call_hands_over_is_what_the_function_takes():
     """The letters of every entry point's arguments against the declaration in its source."""
     import os
