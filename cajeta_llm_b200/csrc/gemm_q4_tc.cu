@@ -4,12 +4,12 @@
 //
 // with the weights and their layout of gemm_q4.cu.  A code times its scale is a bfloat16 number, so the weights are turned into
 // bfloat16 on their way and the product is that of the unpacked weights to the bit.  They are the product's 128 rows and are read from
-// tensor memory: eight warps take a tile of 128 features x 64 of K out of shared memory, each a piece of 16 features (a 16-byte load a
+// tensor memory: eight warps take a tile of 128 features x 64 of K, each a piece of 16 features (a 16-byte load a
 // lane), and put it there with one 16x256b store, whose lanes hold what the layout gave them; nothing is written back to shared
 // memory, whose bandwidth the other operand needs.  The rows of x are the product's columns, up to 256 of them, so that the codes'
 // conversion (140 issue slots a scheduler and tile of 128 x 64) hides behind the product (256 clocks for 128 rows, 512 for 256).
 //
-// Persistent blocks, one an SM: two warps load (x by TMA, the codes of a tile by one bulk copy), one thread issues the products, four
+// Persistent blocks, one an SM: two warps load x by TMA, the converting warps their codes, one thread issues the products, eight
 // warps drain an accumulator while the next fills where tensor memory has room for two.  The gated form puts 16 features of the gate and 16
 // of the other weight on each warp's 32 lanes, so that their sums meet by a shuffle.  Bound by the tensor core for many rows; for a
 // mixture whose groups have a few dozen rows by the weights' bytes and by the groups' last, part-filled tiles.
@@ -22,10 +22,12 @@ using namespace tc;
 
 namespace {
 
-constexpr int LOAD0 = 0, PRODUCT = 1, EPI0 = 2, CONV0 = 6, CONV_SETS = 2, LOAD1 = CONV0 + 8 * CONV_SETS;      // warps
-constexpr int THREADS = (LOAD1 + 1) * 32;
-constexpr int MAX_STAGES = 8, MAX_SLOTS = 8, MAX_GROUPS = 1024;
-constexpr int SLOT_COLS = 32;                 // 128 rows x 64 bfloat16
+constexpr int LOAD_X = 0, LOAD_CODES = 2, PRODUCT = 3, EPI0 = 4, EPI_WARPS = 8, CONV0 = EPI0 + EPI_WARPS, CONV_SETS = 2;      // warps
+constexpr int THREADS = (CONV0 + 8 * CONV_SETS) * 32;
+// (a converting set sees every other pair: an even number of stages of codes are its own, and no wait takes a round for another)
+constexpr int MAX_STAGES = 6, CODE_STAGES = 6, MAX_SLOTS = 4, MAX_GROUPS = 1024;
+static_assert(CODE_STAGES % CONV_SETS == 0, "a set's stages of codes are its own");
+constexpr int HALF_COLS = 32, SLOT_COLS = 2 * HALF_COLS;      // a pair of blocks of K: twice 128 rows x 64 bfloat16
 constexpr int SMEM_LIMIT = 222 * 1024;        // (with the groups' table, 4 KB, what a block can have)
 constexpr int BAR_BYTES = 512;
 
@@ -38,12 +40,12 @@ struct Args {
     long long ldo;
     int rows, features, K, groups, half_out, accumulate;
     int tok;                   // rows of x a tile takes
-    int stages, slots, accs;   // ring of shared memory, ring of tensor memory, accumulators
-    int x_bytes, stage_bytes;
-    // A float32 result's K goes in parts of so many blocks of 64, each summed from zero and added to what the parts before left: tcgen05 cuts its sums off
+    int stages, slots, accs;   // rings of x and of tensor memory, accumulators
+    int x_bytes;               // of a block of 64 of K; a stage has two
+    // A float32 result's K goes in parts of so many pairs of blocks of 64, each summed from zero and added to what the parts before left: tcgen05 cuts its sums off
     // rather than rounding them, and an error that grows with their length stays that of 2,560 entries (2,048 x 3,584 x 3,584: 1.2e-6 of the result
     // in one part, 7e-7 in two).
-    int part_kb;
+    int part_pairs;
 };
 
 struct Tile {
@@ -98,9 +100,36 @@ struct Ring {
     }
 };
 
-__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t s) {
-    const __nv_bfloat162 r = __hmul2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&s);
-    return *(const uint32_t*)&r;
+// Where a tile of features begins along K: each elsewhere, so that the blocks that share rows of x do not all read the same lines of L2 at the same
+// time (2,048 rows, 3,584 x 3,584: 55 us where all begin at 0, 48 with this).
+__device__ __forceinline__ int first_pair(int f, int feat_tiles, int n_pairs) { return (int)((long long)f * n_pairs / feat_tiles); }
+__device__ __forceinline__ int turned(int pair, int turn, int n_pairs) { return pair + turn < n_pairs ? pair + turn : pair + turn - n_pairs; }
+
+__device__ __forceinline__ void commit_at(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// A lane's 16 bytes of codes (features g and g + 8) times their scales, in the order of a 16x256b store.  A code + 8 in the upper four of a
+// bfloat16's seven fraction bits, behind the exponent of 16, is the number 24 + code; one multiplication and addition brings
+// (24 + code) s - 24 s, in which both products are exact (24 has two significant bits, s five) and so is the sum.
+template <bool HALF>
+__device__ __forceinline__ void unpack(uint32_t (&v)[16], const uint4& c, const uint32_t* sc) {
+    const __nv_bfloat162 minus24(__ushort_as_bfloat16(0xc1c0), __ushort_as_bfloat16(0xc1c0));
+    auto of = [](uint32_t w, uint32_t s, __nv_bfloat162 off) {
+        const uint32_t n = (w & 0x00780078u) | 0x41804180u;
+        const __nv_bfloat162 r = __hfma2(*(const __nv_bfloat162*)&n, *(const __nv_bfloat162*)&s, off);
+        return *(const uint32_t*)&r;
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t s2 = sc[HALF ? h : 0], lo = __byte_perm(s2, 0, 0x1010), hi = __byte_perm(s2, 0, 0x3232);
+        const __nv_bfloat162 lo24 = __hmul2(*(const __nv_bfloat162*)&lo, minus24), hi24 = __hmul2(*(const __nv_bfloat162*)&hi, minus24);
+        const uint32_t a = h ? c.y : c.x, b = h ? c.w : c.z;
+        v[8 * h] = of(a << 3, lo, lo24), v[8 * h + 1] = of(a >> 1, lo, lo24);
+        v[8 * h + 2] = of(b << 3, hi, hi24), v[8 * h + 3] = of(b >> 1, hi, hi24);
+        v[8 * h + 4] = of(a >> 5, lo, lo24), v[8 * h + 5] = of(a >> 9, lo, lo24);
+        v[8 * h + 6] = of(b >> 5, hi, hi24), v[8 * h + 7] = of(b >> 9, hi, hi24);
+    }
 }
 
 template <bool GATED, bool HALF>
@@ -109,10 +138,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     constexpr int PIECE = q4::piece_bytes(HALF), TILE = q4::tile_bytes(HALF);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
-    uint64_t* full = bars;                        // [stages] x and codes have landed
-    uint64_t* empty = full + MAX_STAGES;          // [stages] the products have read x (and the codes were converted before)
-    uint64_t* a_full = empty + MAX_STAGES;        // [slots] the weights lie in tensor memory
+    uint8_t* code_ring = smem + (size_t)p.stages * 2 * p.x_bytes;
+    uint64_t* full = (uint64_t*)(code_ring + CODE_STAGES * 2 * TILE);       // [stages] x has landed
+    uint64_t* empty = full + MAX_STAGES;          // [stages] the products have read it
+    uint64_t* code_full = empty + MAX_STAGES;     // [CODE_STAGES] codes have landed
+    uint64_t* code_empty = code_full + CODE_STAGES;                         // [CODE_STAGES] a set has read them
+    uint64_t* a_full = code_empty + CODE_STAGES;        // [slots] the weights lie in tensor memory
     uint64_t* a_empty = a_full + MAX_SLOTS;       // [slots] the products have read them
     uint64_t* acc_full = a_empty + MAX_SLOTS;     // [accs]
     uint64_t* acc_empty = acc_full + 2;
@@ -121,8 +152,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < CODE_STAGES; ++s) mbar_init(&code_full[s], 1), mbar_init(&code_empty[s], 8);
         for (int s = 0; s < p.slots; ++s) mbar_init(&a_full[s], 8), mbar_init(&a_empty[s], 1);
-        for (int s = 0; s < p.accs; ++s) mbar_init(&acc_full[s], 1), mbar_init(&acc_empty[s], 4);
+        for (int s = 0; s < p.accs; ++s) mbar_init(&acc_full[s], 1), mbar_init(&acc_empty[s], EPI_WARPS);
         fence_barrier_init();
     }
     if (warp == PRODUCT) tmem_alloc(tmem_slot, 512);
@@ -153,140 +185,157 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     cj::release_successor();
     const uint32_t tmem = *tmem_slot;
     const int feat_tiles = (p.features + FEAT - 1) / FEAT, tiles_f = (p.features + 127) / 128, n_kb = (p.K + 63) / 64;
+    const int n_pairs = (n_kb + 1) / 2;
     const int total = (p.offsets ? before[p.groups] : (p.rows + p.tok - 1) / p.tok) * feat_tiles;
     const uint32_t acc0 = p.slots * SLOT_COLS;
 
-    if (warp == LOAD0 || warp == LOAD1) {
-        // ---- loads: one warp the even blocks of K, one the odd (what one thread has under way in bulk loads is bounded)
+    if (warp < LOAD_CODES) {
+        // ---- x: one warp the even pairs of blocks of K, one the odd (what one thread has under way in bulk loads is bounded)
         if (elect_one()) {
-            const uint32_t mine = warp == LOAD0 ? 0 : 1;
-            if (!mine) tma_prefetch_descriptor(&map_x);
-            auto codes = [&](const Tile& t, int kb, uint8_t* st, uint64_t* bar) {
-                if (GATED) {
-                    // the gate's four pieces and the other weight's
-                    const size_t at = (((size_t)t.group * tiles_f + (t.f >> 1)) * n_kb + kb) * TILE + (t.f & 1) * 4 * PIECE;
-                    bulk_load(st + p.x_bytes, p.w + at, 4 * PIECE, bar);
-                    bulk_load(st + p.x_bytes + 4 * PIECE, p.w_up + at, 4 * PIECE, bar);
-                } else
-                    bulk_load(st + p.x_bytes, p.w + (((size_t)t.group * tiles_f + t.f) * n_kb + kb) * TILE, TILE, bar);
-            };
-            // weights are written by no kernel of a step: the first ring of codes leaves before the wait for the kernel that makes x
-            uint32_t early = 0;
-            if (!p.offsets) {
-                if ((int)blockIdx.x < total) {
-                    const Tile t = tile_of(p, blockIdx.x, feat_tiles, before);
-                    for (; (int)early < min(n_kb, p.stages); ++early) {
-                        if ((early & 1) != mine) continue;
-                        mbar_expect_tx(&full[early], p.x_bytes + TILE);
-                        codes(t, early, smem + (size_t)early * p.stage_bytes, &full[early]);
-                    }
-                }
-                cj::after_predecessor();
-            }
-            uint32_t it = 0;
-            Ring st_ring{(int)mine, 0};
+            if (warp == LOAD_X) tma_prefetch_descriptor(&map_x);
+            if (!p.offsets) cj::after_predecessor();
+            int pair = warp - LOAD_X;
+            Ring st{0, 0};
+            st.move(pair, p.stages);
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 const Tile t = tile_of(p, tile, feat_tiles, before);
-                for (int kb = 0; kb < n_kb; ++kb, ++it) {
-                    if ((it & 1) != mine) continue;
-                    const int s = st_ring.at;
-                    const uint32_t phase = st_ring.phase;
-                    st_ring.move(2, p.stages);
-                    uint8_t* st = smem + (size_t)s * p.stage_bytes;
-                    if (it >= early) {
-                        ok = mbar_wait(&empty[s], phase ^ 1, 1);
-                        if (!ok) break;
-                        mbar_expect_tx(&full[s], p.x_bytes + TILE);
-                        codes(t, kb, st, &full[s]);
-                    }
-                    tma_load_2d(st, &map_x, &full[s], kb * 64, t.tok0);
+                const int turn = first_pair(t.f, feat_tiles, n_pairs);
+                for (; pair < n_pairs; pair += 2, st.move(2, p.stages)) {
+                    const int at = turned(pair, turn, n_pairs);
+                    uint8_t* dst = smem + (size_t)st.at * 2 * p.x_bytes;
+                    ok = mbar_wait(&empty[st.at], st.phase ^ 1, 1);
+                    if (!ok) break;
+                    const bool two = 2 * at + 1 < n_kb;
+                    mbar_expect_tx(&full[st.at], two ? 2 * p.x_bytes : p.x_bytes);
+                    tma_load_2d(dst, &map_x, &full[st.at], at * 128, t.tok0);
+                    if (two) tma_load_2d(dst + p.x_bytes, &map_x, &full[st.at], at * 128 + 64, t.tok0);
+                }
+                pair -= n_pairs;
+            }
+        }
+    } else if (warp == LOAD_CODES) {
+        // ---- codes: weights are written by no kernel of a step, so that a dense product's leave before the wait for the kernel that makes x
+        if (elect_one()) {
+            Ring st{0, 0};
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                const Tile t = tile_of(p, tile, feat_tiles, before);
+                const int turn = first_pair(t.f, feat_tiles, n_pairs);
+                for (int pair = 0; pair < n_pairs; ++pair, st.move(1, CODE_STAGES)) {
+                    const int kb = 2 * turned(pair, turn, n_pairs), blocks = min(2, n_kb - kb);
+                    uint8_t* dst = code_ring + st.at * 2 * TILE;
+                    uint64_t* bar = &code_full[st.at];
+                    ok = mbar_wait(&code_empty[st.at], st.phase ^ 1, 8);
+                    if (!ok) break;
+                    mbar_expect_tx(bar, blocks * TILE);
+                    if (GATED) {
+                        // of each block the gate's four pieces and the other weight's
+                        const size_t at = (((size_t)t.group * tiles_f + (t.f >> 1)) * n_kb + kb) * TILE + (t.f & 1) * 4 * PIECE;
+                        for (int b = 0; b < blocks; ++b) {
+                            bulk_load(dst + b * TILE, p.w + at + b * TILE, 4 * PIECE, bar);
+                            bulk_load(dst + b * TILE + 4 * PIECE, p.w_up + at + b * TILE, 4 * PIECE, bar);
+                        }
+                    } else
+                        bulk_load(dst, p.w + (((size_t)t.group * tiles_f + t.f) * n_kb + kb) * TILE, blocks * TILE, bar);
                 }
             }
         }
     } else if (warp == PRODUCT) {
         // ---- products
         if (elect_one()) {
-            Ring st{0, 0}, sl{0, 0}, ac{0, 0};
+            // One thread's instructions come one after the other, four clocks and more each, beside those of the warps that share its scheduler: waits, commits and
+            // sums are for two blocks of K at a time, and the loop keeps addresses and descriptors instead of working them out of a place in a ring.
+            const uint32_t full0 = smem_u32(full), a_full0 = smem_u32(a_full), to_empty = smem_u32(empty) - full0, to_a_empty = smem_u32(a_empty) - a_full0;
+            const uint64_t desc0 = umma_desc_sw128(smem);
+            const uint32_t desc_half = (uint32_t)p.x_bytes >> 4, desc_step = 2 * desc_half;
+            const uint32_t full_end = full0 + 8 * p.stages, a_full_end = a_full0 + 8 * p.slots;
+            uint32_t at_full = full0, at_a = a_full0, phase = 0, a_phase = 0, at_tmem = tmem;
+            uint64_t desc = desc0;
+            Ring ac{0, 0};
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 const Tile t = tile_of(p, tile, feat_tiles, before);
-                uint32_t acc = 0;
-                int part = 0;                 // blocks of K in the accumulator
                 const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
-                for (int kb = 0; kb < n_kb; ++kb, st.move(1, p.stages), sl.move(1, p.slots)) {
-                    if (part == 0) {
-                        ok = mbar_wait(&acc_empty[ac.at], ac.phase ^ 1, 2);
-                        if (!ok) break;
-                        acc = tmem + acc0 + ac.at * p.tok;
-                    }
-                    const int s = st.at, slot = sl.at;
-                    // (the slot's weights came out of the stage: x lies there too)
-                    ok = mbar_wait(&a_full[slot], sl.phase, 3) && mbar_wait(&full[s], st.phase, 4);
+                // the pair, counted from where the tile begins, that has one block of K only
+                const int lone = n_kb & 1 ? n_pairs - 1 - first_pair(t.f, feat_tiles, n_pairs) : -1;
+                for (int pair0 = 0; pair0 < n_pairs && ok; pair0 += p.part_pairs) {
+                    ok = mbar_wait(&acc_empty[ac.at], ac.phase ^ 1, 2);
                     if (!ok) break;
-                    tcgen05_fence_after();
-                    const uint64_t dx = umma_desc_sw128(smem + (size_t)s * p.stage_bytes);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_bf16_a_tmem(acc, tmem + slot * SLOT_COLS + 8 * k, dx + 2 * k, idesc, (part | k) ? 1u : 0u);
-                    umma_commit(&empty[s]);
-                    umma_commit(&a_empty[slot]);
-                    if (++part == p.part_kb || kb == n_kb - 1) {
-                        umma_commit(&acc_full[ac.at]);
-                        ac.move(1, p.accs);
-                        part = 0;
+                    const uint32_t acc = tmem + acc0 + ac.at * p.tok;
+                    const int end = min(pair0 + p.part_pairs, n_pairs);
+                    for (int pair = pair0; pair < end; ++pair) {
+                        if (!mbar_try_wait_at(at_a, a_phase)) ok = mbar_wait_slow(a_full + ((at_a - a_full0) >> 3), a_phase, 3);
+                        if (!mbar_try_wait_at(at_full, phase)) ok = ok && mbar_wait_slow(full + ((at_full - full0) >> 3), phase, 4);
+                        if (!ok) break;
+                        tcgen05_fence_after();
+                        umma_bf16_a_tmem(acc, at_tmem, desc, idesc, pair > pair0 ? 1u : 0u);
+                        umma_bf16_a_tmem(acc, at_tmem + 8, desc + 2, idesc, 1);
+                        umma_bf16_a_tmem(acc, at_tmem + 16, desc + 4, idesc, 1);
+                        umma_bf16_a_tmem(acc, at_tmem + 24, desc + 6, idesc, 1);
+                        if (pair != lone) {
+                            umma_bf16_a_tmem(acc, at_tmem + 32, desc + desc_half, idesc, 1);
+                            umma_bf16_a_tmem(acc, at_tmem + 40, desc + desc_half + 2, idesc, 1);
+                            umma_bf16_a_tmem(acc, at_tmem + 48, desc + desc_half + 4, idesc, 1);
+                            umma_bf16_a_tmem(acc, at_tmem + 56, desc + desc_half + 6, idesc, 1);
+                        }
+                        commit_at(at_full + to_empty);
+                        commit_at(at_a + to_a_empty);
+                        at_full += 8, desc += desc_step, at_a += 8, at_tmem += SLOT_COLS;
+                        if (at_full == full_end) at_full = full0, desc = desc0, phase ^= 1;
+                        if (at_a == a_full_end) at_a = a_full0, at_tmem = tmem, a_phase ^= 1;
                     }
+                    if (!ok) break;
+                    umma_commit(&acc_full[ac.at]);
+                    ac.move(1, p.accs);
                 }
             }
         }
     } else if (warp >= CONV0) {
-        // ---- codes to bfloat16: a piece of 16 features a warp, into the 16 lanes of tensor memory that are the piece's rows
-        // (two sets of eight warps take turns: one waits, loads and stores while the other computes)
+        // ---- codes to bfloat16: of a pair of blocks of K two pieces of 16 features a warp, into the 16 lanes of tensor memory that are the
+        // pieces' rows (two sets of eight warps take the pairs in turn: one waits, loads and stores while the other computes)
         const int q = warp & 3, upper = (warp - CONV0) >> 2 & 1;   // the quarter of the lanes this warp may touch, and which half of it
-        const uint32_t set = (warp - CONV0) >> 3;
-        const int piece = GATED ? upper * 4 + q : q * 2 + upper;
+        const int set = (warp - CONV0) >> 3;
         const uint32_t lanes = (uint32_t)(q * 32 + upper * 16) << 16;
+        const uint8_t* mine = code_ring + (GATED ? upper * 4 + q : q * 2 + upper) * PIECE;
         const int my_tiles = (int)blockIdx.x < total ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-        const uint8_t* codes = smem + p.x_bytes + piece * PIECE;
-        Ring st{(int)set, 0}, sl{(int)set, 0};
-        for (int it = set; it < my_tiles * n_kb; it += CONV_SETS, st.move(CONV_SETS, p.stages), sl.move(CONV_SETS, p.slots)) {
-            bool ok = mbar_wait_warp(&full[st.at], st.phase, 5);
-            if (!ok) break;
-            const uint8_t* src = codes + st.at * p.stage_bytes;
-            const uint4 c = *(const uint4*)(src + lane * 16);
-            uint32_t sc[HALF ? 2 : 1];
+        Ring st{set, 0}, sl{0, 0};
+        sl.move(set, p.slots);
+        for (int left = my_tiles * n_pairs - set; left > 0; left -= CONV_SETS, st.move(CONV_SETS, CODE_STAGES), sl.move(CONV_SETS, p.slots)) {
+            if (!mbar_wait_warp(&code_full[st.at], st.phase, 5)) break;
+            // (where a pair has one block, what lies there is put down for the other and nobody reads it)
+            const uint8_t* src = mine + st.at * 2 * TILE;
+            const uint4 c0 = *(const uint4*)(src + lane * 16), c1 = *(const uint4*)(src + TILE + lane * 16);
+            constexpr int SCALES = HALF ? 2 : 1;
+            uint32_t sc[2 * SCALES];
 #pragma unroll
-            for (int h = 0; h < (HALF ? 2 : 1); ++h) sc[h] = *(const uint32_t*)(src + 512 + (h * 8 + (lane >> 2)) * 4);
+            for (int h = 0; h < 2 * SCALES; ++h)
+                sc[h] = *(const uint32_t*)(src + (h / SCALES) * TILE + 512 + (h % SCALES * 8 + (lane >> 2)) * 4);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&code_empty[st.at]);
             uint32_t v[16];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t a = (j < 2 ? c.x : c.y) >> (8 * (j & 1)), b = (j < 2 ? c.z : c.w) >> (8 * (j & 1));
-                const uint32_t s2 = sc[HALF ? j >> 1 : 0], lo = __byte_perm(s2, 0, 0x1010), hi = __byte_perm(s2, 0, 0x3232);
-                v[4 * j] = times(q4::pair(a), lo);
-                v[4 * j + 1] = times(q4::pair(a >> 4), lo);
-                v[4 * j + 2] = times(q4::pair(b), hi);
-                v[4 * j + 3] = times(q4::pair(b >> 4), hi);
-            }
-            ok = mbar_wait_warp(&a_empty[sl.at], sl.phase ^ 1, 6);
-            if (!ok) break;
+            unpack<HALF>(v, c0, sc);
+            if (!mbar_wait_warp(&a_empty[sl.at], sl.phase ^ 1, 6)) break;
             tcgen05_fence_after();
             tmem_st_16x256b_x4(tmem + sl.at * SLOT_COLS + lanes, v);
+            unpack<HALF>(v, c1, sc + SCALES);
+            tmem_st_16x256b_x4(tmem + sl.at * SLOT_COLS + HALF_COLS + lanes, v);
             tmem_st_wait();
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&a_full[sl.at]);
         }
     } else {
-        // ---- epilogue: warps 2 .. 5, a quarter of the lanes each; a lane is a feature, columns are rows of x
+        // ---- epilogue: two warps a quarter of the lanes, 16 columns in turn; a lane is a feature, columns are rows of x
         if (!p.offsets) cj::after_predecessor();
         const int q = warp & 3;
         Ring ac{0, 0};
         bool ok = true;
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x)
-        for (int kb = 0; kb < n_kb; kb += p.part_kb, ac.move(1, p.accs)) {
+        for (int pair = 0; pair < n_pairs; pair += p.part_pairs, ac.move(1, p.accs)) {
             const Tile t = tile_of(p, tile, feat_tiles, before);
             const int as = ac.at;
-            const bool add = p.accumulate || kb > 0;
+            const bool add = p.accumulate || pair > 0;
             ok = mbar_wait_warp(&acc_full[as], ac.phase, 7);
             if (!ok) break;
             tcgen05_fence_after();
@@ -294,9 +343,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             const int n = t.tok_end - t.tok0;
             const int feature = GATED ? t.f * 64 + q * 16 + (lane & 15) : t.f * 128 + q * 32 + lane;
             const bool in = feature < p.features;
-            const float bias = !GATED && p.bias && in && kb == 0 ? p.bias[feature] : 0.0f;
+            const float bias = !GATED && p.bias && in && pair == 0 ? p.bias[feature] : 0.0f;
 #pragma unroll 1
-            for (int c0 = 0; c0 < n; c0 += 16) {
+            for (int c0 = ((warp - EPI0) >> 2) * 16; c0 < n; c0 += 4 * EPI_WARPS) {
                 uint32_t v[16];
                 tmem_ld16(src + c0, v);
                 tmem_ld_wait();
@@ -392,15 +441,15 @@ CJ_EXPORT int cj_gemm_q4_tc(const void* x, long long ldx, int x_rows, const void
     CUtensorMap map;
     if (!make_map_bf16(&map, x, x_rows, K, ldx, tok)) return CJ_ERR_ARG;
     Args a{(const uint8_t*)w, (const uint8_t*)w_up, bias, out, offsets, ldo, rows, features, K, groups, out_dtype == CJ_BF16 ? 1 : 0, accumulate,
-           tok, 0, 0, 0, tok * 128, 0, 0};
-    const int n_kb = (K + 63) / 64, parts = out_dtype == CJ_F32 && !w_up ? (n_kb + 39) / 40 : 1;
-    a.part_kb = (n_kb + parts - 1) / parts;
-    a.stage_bytes = a.x_bytes + (q4::tile_bytes(half != 0) + 1023) / 1024 * 1024;
-    a.stages = min(MAX_STAGES, (SMEM_LIMIT - 1024 - BAR_BYTES) / a.stage_bytes);
-    // two accumulators where at least three slots of weights fit beside them
-    a.accs = 2 * tok + 3 * SLOT_COLS <= 512 ? 2 : 1;
+           tok, 0, 0, 0, tok * 128, 0};
+    const int n_pairs = (K + 127) / 128, parts = out_dtype == CJ_F32 && !w_up ? (n_pairs + 19) / 20 : 1;
+    a.part_pairs = (n_pairs + parts - 1) / parts;
+    const int code_ring = CODE_STAGES * 2 * q4::tile_bytes(half != 0);
+    a.stages = min(MAX_STAGES, (SMEM_LIMIT - 1024 - BAR_BYTES - code_ring) / (2 * a.x_bytes));
+    // two accumulators where two slots of weights fit beside them
+    a.accs = 2 * tok + 2 * SLOT_COLS <= 512 ? 2 : 1;
     a.slots = min(MAX_SLOTS, (512 - a.accs * tok) / SLOT_COLS);
-    const int smem = a.stages * a.stage_bytes + BAR_BYTES + 1024;
+    const int smem = a.stages * 2 * a.x_bytes + code_ring + BAR_BYTES + 1024;
     const long long most = offsets ? sms : (long long)feat_tiles * ((rows + tok - 1) / tok);
     auto kern = w_up ? (half ? gemm_q4_tc_kernel<true, true> : gemm_q4_tc_kernel<true, false>)
                      : (half ? gemm_q4_tc_kernel<false, true> : gemm_q4_tc_kernel<false, false>);
