@@ -1974,19 +1974,20 @@ def q4_on_tcgen05(rows: int, features: int, groups: int) -> bool:
     # Its tiles take 12 us at K 2,048 whatever their rows, the other form's work grows with them.  (us, tcgen05 and the other: dense, 6,144 features x 2,048,
     # 24 rows 12.4 and 11.4, 32 rows 12.4 and 12.9, 64 rows 12.9 and 18.8; 2,048 features, 64 rows 11.8 and 7.2, 128 rows 12.7 and 12.1; 60 gated
     # experts of 1,408 x 2,048, two rows each 60 and 40, four 69 and 84, seventeen 92 and 136)
-    return rows > 4 * groups if groups else rows > 8 and rows * features > 190_000
+    return rows > 3 * groups if groups else rows > 8 and rows * features > 140_000
 
 
 @functools.lru_cache(maxsize=4096)
 def q4_tile_rows(rows: int, features: int, groups: int, gated: bool, sms: int) -> int:
     """Rows of x that a tile of the tensor-core product with 4-bit weights takes."""
     if groups:
-        # tiles that most groups of an even split fill once (mean and two standard deviations)
-        mean = rows / groups
-        return min(256, -(-int(mean + 2.0 * mean ** 0.5) // 16) * 16)
+        # A tile of up to 160 rows takes as long as its weights' conversion, and 160 is the most that tensor memory has room for twice: a group
+        # that needs two tiles converts its weights twice (60 experts of 1,408 x 2,048, 34 rows each on average: 32 rows a tile 106 us, 48 88,
+        # 96 76, 160 72; nine rows each: 16 71 us, 80 55, 160 56)
+        return min(160, -(-rows // 16) * 16)
     feature_tiles = -(-features // (64 if gated else 128))
-    # rounds of the machine times what a tile of that many rows takes (its columns, and some for its start)
-    return min(range(256, 15, -16), key=lambda n: -(-feature_tiles * -(-rows // n) // sms) * (n + 16))
+    # rounds of the machine times what a tile of that many rows takes (its weights' conversion or its columns, and some for its start)
+    return min(range(min(256, -(-rows // 16) * 16), 15, -16), key=lambda n: -(-feature_tiles * -(-rows // n) // sms) * (max(n, 160) + 16))
 
 
 def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torch.Tensor] = None, accumulate: bool = False,
