@@ -244,9 +244,15 @@ __global__ void q4_quantise_kernel(const T* __restrict__ w, int8_t* __restrict__
     const long long row = idx / groups_k;
     const int k0 = (int)(idx % groups_k) * group, n = min(group, K - k0);
     float most = 0.0f;
-    for (int i = lane; i < n; i += 32) most = fmaxf(most, fabsf(to_f32(w[row * K + k0 + i])));
+    bool finite = true;
+    for (int i = lane; i < n; i += 32) {
+        const float v = fabsf(to_f32(w[row * K + k0 + i]));
+        most = fmaxf(most, v);
+        finite = finite && v < INFINITY;
+    }
     most = warp_max(most);
-    const float s = q4::scale_up(most / 7.0f);
+    // (a group with an entry that is no number has no scale: the caller is told)
+    const float s = __all_sync(0xffffffffu, finite) ? q4::scale_up(most / 7.0f) : INFINITY;
     for (int i = lane; i < n; i += 32) {
         const float v = s > 0.0f ? rintf(to_f32(w[row * K + k0 + i]) / s) : 0.0f;
         codes[row * K + k0 + i] = (int8_t)fminf(fmaxf(v, -8.0f), 7.0f);

@@ -132,6 +132,19 @@ __device__ __forceinline__ void unpack(uint32_t (&v)[16], const uint4& c, const 
     }
 }
 
+// each(j) for the 16 columns of a step of the epilogue, or for the first `left` of them: none of the whole ones asks for its place
+template <typename F>
+__device__ __forceinline__ void columns(int left, F&& each) {
+    if (left >= 16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) each(j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 15; ++j)
+            if (j < left) each(j);
+    }
+}
+
 template <bool GATED, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const Args p) {
     constexpr int FEAT = GATED ? 64 : 128;                         // features a tile takes
@@ -371,20 +384,13 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                     const int left = n - c0;
                     if (p.half_out) {
                         __nv_bfloat16* dst = (__nv_bfloat16*)p.out + (size_t)(t.tok0 + c0) * p.ldo + feature;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j, dst += p.ldo)
-                            if (j < left) *dst = __float2bfloat16_rn(__uint_as_float(v[j]) + bias);
+                        columns(left, [&](int j) { dst[j * p.ldo] = __float2bfloat16_rn(__uint_as_float(v[j]) + bias); });
                     } else {
                         float* dst = (float*)p.out + (size_t)(t.tok0 + c0) * p.ldo + feature;
-                        if (add) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j, dst += p.ldo)
-                                if (j < left) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(dst), "f"(__uint_as_float(v[j]) + bias) : "memory");
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j, dst += p.ldo)
-                                if (j < left) *dst = __uint_as_float(v[j]) + bias;
-                        }
+                        if (add) columns(left, [&](int j) {
+                            asm volatile("red.global.add.f32 [%0], %1;" ::"l"(dst + j * p.ldo), "f"(__uint_as_float(v[j]) + bias) : "memory");
+                        });
+                        else columns(left, [&](int j) { dst[j * p.ldo] = __uint_as_float(v[j]) + bias; });
                     }
                 }
             }

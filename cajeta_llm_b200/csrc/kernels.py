@@ -1884,6 +1884,8 @@ class Q4Weight:
 
     ``quantise`` makes one from a float32 or bfloat16 weight, ``from_codes`` from codes and scales; both wait until it lies there."""
 
+    MOST_SCALE = 2.0 ** 123        # scales lie below it: the products' 24 scales and more stay finite numbers
+
     def __init__(self, data: torch.Tensor, shape, group: int, features: int = 0, groups: int = 0):
         self.data = data                       # uint8, the layout
         self.shape = tuple(shape)
@@ -1910,8 +1912,8 @@ class Q4Weight:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, group: int = 64) -> "Q4Weight":
-        """``codes``: int8 [.., features, K] from -8 to 7; ``scales``: [.., features, ceil(K / group)], finite numbers of at most five
-        significant bits (float32 or bfloat16); group: 32 or a multiple of 64."""
+        """``codes``: int8 [.., features, K] from -8 to 7; ``scales``: [.., features, ceil(K / group)], numbers of at most five
+        significant bits below 2^123 (float32 or bfloat16); group: 32 or a multiple of 64."""
         cls._fits(codes.shape, group)
         _need(codes, "codes", torch.int8)
         cls._steady("Q4Weight.from_codes")
@@ -1921,14 +1923,14 @@ class Q4Weight:
         scales = scales.to(torch.float32).contiguous()
         if int(codes.amin()) < -8 or int(codes.amax()) > 7:
             raise KernelError("Q4Weight: codes lie between -8 and 7")
-        if not bool(((scales.view(torch.int32) & 0x7ffff) == 0).all()) or not bool(torch.isfinite(scales).all()):
-            raise KernelError("Q4Weight: scales must be finite and have at most five significant bits")
+        if not bool(((scales.view(torch.int32) & 0x7ffff) == 0).all()) or not bool((scales.abs() < cls.MOST_SCALE).all()):
+            raise KernelError("Q4Weight: scales must have at most five significant bits and lie below 2^123")
         return cls._lay_out(codes, scales, group)
 
     @classmethod
     def quantise(cls, w: torch.Tensor, group: int = 64) -> "Q4Weight":
         """The scale of a group is the smallest number of five significant bits that is at least max|w| / 7, a code w / scale rounded
-        to the nearest integer (of two, the even one)."""
+        to the nearest integer (of two, the even one).  Entries must be finite and smaller than 7 2^122."""
         return cls._lay_out(*cls.codes_of(w, group), group)
 
     @classmethod
@@ -1943,6 +1945,8 @@ class Q4Weight:
         scales = torch.empty(tuple(w.shape[:-1]) + (-(-K // group),), dtype=torch.float32, device=w.device)
         st = library("gemm_q4").cj_q4_quantise(_ptr(w), _i(_code(w)), _ptr(codes), _ptr(scales), _ll(w.numel() // K), _i(K), _i(group), _stream())
         _check(st, "Q4Weight.quantise")
+        if not bool((scales < cls.MOST_SCALE).all()):
+            raise KernelError("Q4Weight.quantise: entries must be finite and smaller than 7 2^122")
         return codes, scales
 
     @classmethod
@@ -1971,10 +1975,10 @@ class Q4Weight:
 
 def q4_on_tcgen05(rows: int, features: int, groups: int) -> bool:
     """Whether a product with 4-bit weights has rows enough for the form that puts them on the columns of tcgen05 products (``groups`` 0: dense)."""
-    # Its tiles take 12 us at K 2,048 whatever their rows, the other form's work grows with them.  (us, tcgen05 and the other: dense, 6,144 features x 2,048,
-    # 24 rows 12.4 and 11.4, 32 rows 12.4 and 12.9, 64 rows 12.9 and 18.8; 2,048 features, 64 rows 11.8 and 7.2, 128 rows 12.7 and 12.1; 60 gated
-    # experts of 1,408 x 2,048, two rows each 60 and 40, four 69 and 84, seventeen 92 and 136)
-    return rows > 3 * groups if groups else rows > 8 and rows * features > 140_000
+    # Its tiles take 8 us at K 2,048 whatever their rows, the other form's work grows with them.  (us, tcgen05 and the other: dense, 6,144 features x 2,048,
+    # 16 rows 7.9 and 6.8, 24 rows 8.0 and 11.4, 64 rows 8.5 and 18.8; 2,048 features, 64 rows 8.4 and 7.2, 80 rows 8.8 and 11.1; 60 gated
+    # experts of 1,408 x 2,048, two rows each 45 and 40, four 52 and 59, seventeen 62 and 170.  It has room for the places of 1,024 groups.)
+    return 3 * groups < rows and groups <= 1024 if groups else rows > 8 and rows * features > 140_000
 
 
 @functools.lru_cache(maxsize=4096)

@@ -180,3 +180,71 @@ def test_captured_and_replayed():
         got = out.clone()
         K.gemm_q4(x, w, out)
         assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("rows,features,k,group,form", [
+    (2048, 640, 2048, 64, "plain"), (700, 1920, 4032, 64, "accumulate"), (1000, 3584, 3584, 32, "plain"), (130, 5000, 64, 64, "bias"), (24, 6144, 200, 64, "half"),
+    (300, 20000, 136, 32, "gated"), (520, 704, 2752, 64, "gated32"), (65, 9000, 1032, 64, "accumulate"), (257, 4096, 8, 64, "plain"), (300, 1000, 1984, 32, "half")])
+def test_dense_of_many_rows(rows, features, k, group, form):
+    """Several tiles a block, an odd number of blocks of 64 along K, K in parts, rows and features that end inside a tile; twice over."""
+    assert K.q4_on_tcgen05(rows, features, 0)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows + k)
+    w, full = weight((features, k), group, seed=features)
+    x = torch.randn((rows, k + 8), generator=g, device=DEV).to(torch.bfloat16)[:, :k]
+    xd = x.to(F64)
+    want, size = xd @ full.T, xd.abs() @ full.abs().T
+    for _ in range(2):
+        if form.startswith("gated"):
+            up, full_up = weight((features, k), group, seed=features + 1)
+            out = torch.empty((rows, features), dtype=torch.float32 if form == "gated32" else torch.bfloat16, device=DEV)
+            K.gemm_q4(x, w, out, w_up=up)
+            u, usize = xd @ full_up.T, xd.abs() @ full_up.abs().T
+            gate = want * torch.sigmoid(want)
+            check(out, gate * u, 1.1 * sums(k, size) * u.abs() + sums(k, usize) * gate.abs() + 2.0 ** -20 * (1 + want.abs()) * (gate * u).abs())
+            continue
+        bias = torch.randn(features, generator=g, device=DEV) if form == "bias" else None
+        before = torch.randn((rows, features), generator=g, device=DEV)
+        out = before.to(torch.bfloat16) if form == "half" else before.clone()
+        K.gemm_q4(x, w, out, bias=bias, accumulate=form == "accumulate")
+        exact = want + (bias.to(F64) if bias is not None else before.to(F64) if form == "accumulate" else 0.0)
+        # (a part's sum joins the others and what was there by one float32 addition each)
+        check(out, exact, sums(k, size) + 2.0 ** -22 * (before.abs() if form == "accumulate" else bias.abs() if bias is not None else 0.0))
+
+
+def test_scales_and_entries_out_of_range_are_refused():
+    codes = torch.zeros((16, 64), dtype=torch.int8, device=DEV)
+    for s in (2.0 ** 123, float("inf"), float("nan"), -(2.0 ** 123)):
+        with pytest.raises(K.KernelError, match="below 2\\^123"):
+            K.Q4Weight.from_codes(codes, torch.full((16, 1), s, device=DEV))
+    for bad in (float("inf"), float("nan"), 3.0e38):
+        w = torch.ones((16, 128), device=DEV)
+        w[3, 70] = bad
+        with pytest.raises(K.KernelError, match="finite"):
+            K.Q4Weight.quantise(w)
+
+
+def test_the_largest_and_smallest_scales():
+    """Products of few rows and of many read the same numbers at both ends of the scales' range."""
+    codes = (torch.arange(256 * 64, device=DEV) % 16 - 8).to(torch.int8).view(256, 64)
+    for s in (31.0 * 2.0 ** 118, 2.0 ** -126):
+        w = K.Q4Weight.from_codes(codes, torch.full((256, 1), s, device=DEV))
+        x = torch.zeros((1024, 64), dtype=torch.bfloat16, device=DEV)
+        x[torch.arange(1024), torch.arange(1024) % 64] = 1.0
+        for rows in (1, 8, 1024):
+            out = torch.empty((rows, 256), device=DEV)
+            K.gemm_q4(x[:rows], w, out)
+            assert torch.equal(out.to(F64), codes.to(F64).T[torch.arange(rows, device=DEV) % 64] * s)
+
+
+def test_more_groups_than_the_tensor_core_form_has_places_for():
+    groups, k = 1500, 64
+    w, full = weight((groups, 16, k), 64, seed=5)
+    rows = 4 * groups
+    x = torch.randn((rows, k), device=DEV).to(torch.bfloat16)
+    offsets = torch.arange(0, rows + 1, 4, dtype=torch.int32, device=DEV)
+    out = torch.empty((rows, 16), device=DEV)
+    K.gemm_q4(x, w, out, group_offsets=offsets)
+    of = full.repeat_interleave(4, dim=0)
+    want = torch.einsum("sk,sfk->sf", x.to(F64), of)
+    check(out, want, sums(k, torch.einsum("sk,sfk->sf", x.to(F64).abs(), of.abs())))
