@@ -25,10 +25,10 @@ namespace {
 constexpr int LOAD_X = 0, LOAD_CODES = 2, PRODUCT = 3, EPI0 = 4, EPI_WARPS = 8, CONV0 = EPI0 + EPI_WARPS, CONV_SETS = 2;      // warps
 constexpr int THREADS = (CONV0 + 8 * CONV_SETS) * 32;
 // (a converting set sees every other pair: an even number of stages of codes are its own, and no wait takes a round for another)
-constexpr int MAX_STAGES = 6, CODE_STAGES = 6, MAX_SLOTS = 4, MAX_GROUPS = 1024;
+constexpr int MAX_STAGES = 4, CODE_STAGES = 6, MAX_GROUPS = 1024;
 static_assert(CODE_STAGES % CONV_SETS == 0, "a set's stages of codes are its own");
 constexpr int HALF_COLS = 32, SLOT_COLS = 2 * HALF_COLS;      // a pair of blocks of K: twice 128 rows x 64 bfloat16
-constexpr int SMEM_LIMIT = 222 * 1024;        // (with the groups' table, 4 KB, what a block can have)
+constexpr int SMEM_LIMIT = 218 * 1024;        // (with the groups' tables, 8 KB, what a block can have)
 constexpr int BAR_BYTES = 512;
 
 struct Args {
@@ -40,7 +40,7 @@ struct Args {
     long long ldo;
     int rows, features, K, groups, half_out, accumulate;
     int tok;                   // rows of x a tile takes
-    int stages, slots, accs;   // rings of x and of tensor memory, accumulators
+    int stages, accs;          // pairs of blocks of K that x and the weights in tensor memory have room for; accumulators
     int x_bytes;               // of a block of 64 of K; a stage has two
     // A float32 result's K goes in parts of so many pairs of blocks of 64, each summed from zero and added to what the parts before left: tcgen05 cuts its sums off
     // rather than rounding them, and an error that grows with their length stays that of 2,560 entries (2,048 x 3,584 x 3,584: 1.2e-6 of the result
@@ -53,7 +53,7 @@ struct Tile {
 };
 
 // dense: features run fastest (neighbouring blocks share the rows of x); grouped: rows run fastest (they share weights)
-__device__ __forceinline__ Tile tile_of(const Args& p, int tile, int feat_tiles, const int* before) {
+__device__ __forceinline__ Tile tile_of(const Args& p, int tile, int feat_tiles, const int* before, const int* edge) {
     Tile t;
     if (!p.offsets) {
         t.group = 0;
@@ -70,8 +70,8 @@ __device__ __forceinline__ Tile tile_of(const Args& p, int tile, int feat_tiles,
     const int n = before[lo + 1] - before[lo], local = tile - before[lo] * feat_tiles;
     t.group = lo;
     t.f = local / n;
-    t.tok0 = max(0, p.offsets[lo]) + local % n * p.tok;
-    t.tok_end = min(min(p.rows, p.offsets[lo + 1]), t.tok0 + p.tok);
+    t.tok0 = edge[lo] + local % n * p.tok;
+    t.tok_end = min(edge[lo + 1], t.tok0 + p.tok);
     return t;
 }
 
@@ -152,21 +152,19 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* code_ring = smem + (size_t)p.stages * 2 * p.x_bytes;
-    uint64_t* full = (uint64_t*)(code_ring + CODE_STAGES * 2 * TILE);       // [stages] x has landed
-    uint64_t* empty = full + MAX_STAGES;          // [stages] the products have read it
+    uint64_t* full = (uint64_t*)(code_ring + CODE_STAGES * 2 * TILE);       // [stages] x has landed and the weights lie in tensor memory
+    uint64_t* empty = full + MAX_STAGES;          // [stages] the products have read both
     uint64_t* code_full = empty + MAX_STAGES;     // [CODE_STAGES] codes have landed
     uint64_t* code_empty = code_full + CODE_STAGES;                         // [CODE_STAGES] a set has read them
-    uint64_t* a_full = code_empty + CODE_STAGES;        // [slots] the weights lie in tensor memory
-    uint64_t* a_empty = a_full + MAX_SLOTS;       // [slots] the products have read them
-    uint64_t* acc_full = a_empty + MAX_SLOTS;     // [accs]
+    uint64_t* acc_full = code_empty + CODE_STAGES;     // [accs]
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
     __shared__ int before[MAX_GROUPS + 1];        // tiles of rows of the groups before
+    __shared__ int edge[MAX_GROUPS + 1];          // where the groups' rows begin
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1 + 8), mbar_init(&empty[s], 1);
         for (int s = 0; s < CODE_STAGES; ++s) mbar_init(&code_full[s], 1), mbar_init(&code_empty[s], 8);
-        for (int s = 0; s < p.slots; ++s) mbar_init(&a_full[s], 8), mbar_init(&a_empty[s], 1);
         for (int s = 0; s < p.accs; ++s) mbar_init(&acc_full[s], 1), mbar_init(&acc_empty[s], EPI_WARPS);
         fence_barrier_init();
     }
@@ -178,7 +176,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             for (int g0 = 0; g0 < p.groups; g0 += 32) {
                 const int g = g0 + lane;
                 int n = 0;
-                if (g < p.groups) n = max(0, (min(p.rows, p.offsets[g + 1]) - max(0, p.offsets[g]) + p.tok - 1) / p.tok);
+                if (g < p.groups) {
+                    const int begin = min(max(0, p.offsets[g]), p.rows), end = min(max(0, p.offsets[g + 1]), p.rows);
+                    n = (max(0, end - begin) + p.tok - 1) / p.tok;
+                    edge[g] = begin;
+                    if (g + 1 == p.groups) edge[p.groups] = end;
+                }
                 int inc = n;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     const int feat_tiles = (p.features + FEAT - 1) / FEAT, tiles_f = (p.features + 127) / 128, n_kb = (p.K + 63) / 64;
     const int n_pairs = (n_kb + 1) / 2;
     const int total = (p.offsets ? before[p.groups] : (p.rows + p.tok - 1) / p.tok) * feat_tiles;
-    const uint32_t acc0 = p.slots * SLOT_COLS;
+    const uint32_t acc0 = p.stages * SLOT_COLS;
 
     if (warp < LOAD_CODES) {
         // ---- x: one warp the even pairs of blocks of K, one the odd (what one thread has under way in bulk loads is bounded)
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             st.move(pair, p.stages);
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-                const Tile t = tile_of(p, tile, feat_tiles, before);
+                const Tile t = tile_of(p, tile, feat_tiles, before, edge);
                 const int turn = first_pair(t.f, feat_tiles, n_pairs);
                 for (; pair < n_pairs; pair += 2, st.move(2, p.stages)) {
                     const int at = turned(pair, turn, n_pairs);
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             Ring st{0, 0};
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-                const Tile t = tile_of(p, tile, feat_tiles, before);
+                const Tile t = tile_of(p, tile, feat_tiles, before, edge);
                 const int turn = first_pair(t.f, feat_tiles, n_pairs);
                 for (int pair = 0; pair < n_pairs; ++pair, st.move(1, CODE_STAGES)) {
                     const int kb = 2 * turned(pair, turn, n_pairs), blocks = min(2, n_kb - kb);
@@ -259,16 +262,15 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         if (elect_one()) {
             // One thread's instructions come one after the other, four clocks and more each, beside those of the warps that share its scheduler: waits, commits and
             // sums are for two blocks of K at a time, and the loop keeps addresses and descriptors instead of working them out of a place in a ring.
-            const uint32_t full0 = smem_u32(full), a_full0 = smem_u32(a_full), to_empty = smem_u32(empty) - full0, to_a_empty = smem_u32(a_empty) - a_full0;
+            const uint32_t full0 = smem_u32(full), full_end = full0 + 8 * p.stages;
             const uint64_t desc0 = umma_desc_sw128(smem);
             const uint32_t desc_half = (uint32_t)p.x_bytes >> 4, desc_step = 2 * desc_half;
-            const uint32_t full_end = full0 + 8 * p.stages, a_full_end = a_full0 + 8 * p.slots;
-            uint32_t at_full = full0, at_a = a_full0, phase = 0, a_phase = 0, at_tmem = tmem;
+            uint32_t bar = full0, phase = 0, at_tmem = tmem;
             uint64_t desc = desc0;
             Ring ac{0, 0};
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-                const Tile t = tile_of(p, tile, feat_tiles, before);
+                const Tile t = tile_of(p, tile, feat_tiles, before, edge);
                 const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
                 // the pair, counted from where the tile begins, that has one block of K only
                 const int lone = n_kb & 1 ? n_pairs - 1 - first_pair(t.f, feat_tiles, n_pairs) : -1;
@@ -278,8 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                     const uint32_t acc = tmem + acc0 + ac.at * p.tok;
                     const int end = min(pair0 + p.part_pairs, n_pairs);
                     for (int pair = pair0; pair < end; ++pair) {
-                        if (!mbar_try_wait_at(at_a, a_phase)) ok = mbar_wait_slow(a_full + ((at_a - a_full0) >> 3), a_phase, 3);
-                        if (!mbar_try_wait_at(at_full, phase)) ok = ok && mbar_wait_slow(full + ((at_full - full0) >> 3), phase, 4);
+                        if (!mbar_try_wait_at(bar, phase)) ok = mbar_wait_slow(full + ((bar - full0) >> 3), phase, 3);
                         if (!ok) break;
                         tcgen05_fence_after();
                         umma_bf16_a_tmem(acc, at_tmem, desc, idesc, pair > pair0 ? 1u : 0u);
@@ -292,11 +293,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                             umma_bf16_a_tmem(acc, at_tmem + 48, desc + desc_half + 4, idesc, 1);
                             umma_bf16_a_tmem(acc, at_tmem + 56, desc + desc_half + 6, idesc, 1);
                         }
-                        commit_at(at_full + to_empty);
-                        commit_at(at_a + to_a_empty);
-                        at_full += 8, desc += desc_step, at_a += 8, at_tmem += SLOT_COLS;
-                        if (at_full == full_end) at_full = full0, desc = desc0, phase ^= 1;
-                        if (at_a == a_full_end) at_a = a_full0, at_tmem = tmem, a_phase ^= 1;
+                        commit_at(bar + 8 * MAX_STAGES);
+                        bar += 8, desc += desc_step, at_tmem += SLOT_COLS;
+                        if (bar == full_end) bar = full0, desc = desc0, at_tmem = tmem, phase ^= 1;
                     }
                     if (!ok) break;
                     umma_commit(&acc_full[ac.at]);
@@ -313,8 +312,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         const uint8_t* mine = code_ring + (GATED ? upper * 4 + q : q * 2 + upper) * PIECE;
         const int my_tiles = (int)blockIdx.x < total ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
         Ring st{set, 0}, sl{0, 0};
-        sl.move(set, p.slots);
-        for (int left = my_tiles * n_pairs - set; left > 0; left -= CONV_SETS, st.move(CONV_SETS, CODE_STAGES), sl.move(CONV_SETS, p.slots)) {
+        sl.move(set, p.stages);
+        for (int left = my_tiles * n_pairs - set; left > 0; left -= CONV_SETS, st.move(CONV_SETS, CODE_STAGES), sl.move(CONV_SETS, p.stages)) {
             if (!mbar_wait_warp(&code_full[st.at], st.phase, 5)) break;
             // (where a pair has one block, what lies there is put down for the other and nobody reads it)
             const uint8_t* src = mine + st.at * 2 * TILE;
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             if (lane == 0) mbar_arrive(&code_empty[st.at]);
             uint32_t v[16];
             unpack<HALF>(v, c0, sc);
-            if (!mbar_wait_warp(&a_empty[sl.at], sl.phase ^ 1, 6)) break;
+            if (!mbar_wait_warp(&empty[sl.at], sl.phase ^ 1, 6)) break;
             tcgen05_fence_after();
             tmem_st_16x256b_x4(tmem + sl.at * SLOT_COLS + lanes, v);
             unpack<HALF>(v, c1, sc + SCALES);
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             tmem_st_wait();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[sl.at]);
+            if (lane == 0) mbar_arrive(&full[sl.at]);
         }
     } else {
         // ---- epilogue: two warps a quarter of the lanes, 16 columns in turn; a lane is a feature, columns are rows of x
@@ -346,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         bool ok = true;
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x)
         for (int pair = 0; pair < n_pairs; pair += p.part_pairs, ac.move(1, p.accs)) {
-            const Tile t = tile_of(p, tile, feat_tiles, before);
+            const Tile t = tile_of(p, tile, feat_tiles, before, edge);
             const int as = ac.at;
             const bool add = p.accumulate || pair > 0;
             ok = mbar_wait_warp(&acc_full[as], ac.phase, 7);
@@ -447,14 +446,13 @@ CJ_EXPORT int cj_gemm_q4_tc(const void* x, long long ldx, int x_rows, const void
     CUtensorMap map;
     if (!make_map_bf16(&map, x, x_rows, K, ldx, tok)) return CJ_ERR_ARG;
     Args a{(const uint8_t*)w, (const uint8_t*)w_up, bias, out, offsets, ldo, rows, features, K, groups, out_dtype == CJ_BF16 ? 1 : 0, accumulate,
-           tok, 0, 0, 0, tok * 128, 0};
+           tok, 0, 0, tok * 128, 0};
     const int n_pairs = (K + 127) / 128, parts = out_dtype == CJ_F32 && !w_up ? (n_pairs + 19) / 20 : 1;
     a.part_pairs = (n_pairs + parts - 1) / parts;
     const int code_ring = CODE_STAGES * 2 * q4::tile_bytes(half != 0);
-    a.stages = min(MAX_STAGES, (SMEM_LIMIT - 1024 - BAR_BYTES - code_ring) / (2 * a.x_bytes));
-    // two accumulators where two slots of weights fit beside them
+    // two accumulators where the weights of two pairs fit beside them
     a.accs = 2 * tok + 2 * SLOT_COLS <= 512 ? 2 : 1;
-    a.slots = min(MAX_SLOTS, (512 - a.accs * tok) / SLOT_COLS);
+    a.stages = min(min(MAX_STAGES, (512 - a.accs * tok) / SLOT_COLS), (SMEM_LIMIT - 1024 - BAR_BYTES - code_ring) / (2 * a.x_bytes));
     const int smem = a.stages * 2 * a.x_bytes + code_ring + BAR_BYTES + 1024;
     const long long most = offsets ? sms : (long long)feat_tiles * ((rows + tok - 1) / tok);
     auto kern = w_up ? (half ? gemm_q4_tc_kernel<true, true> : gemm_q4_tc_kernel<true, false>)
