@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     uint64_t* code_empty = code_full + CODE_STAGES;                         // [CODE_STAGES] a set has read them
     uint64_t* acc_full = code_empty + CODE_STAGES;     // [accs]
     uint64_t* acc_empty = acc_full + 2;
-    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+    uint2* told = (uint2*)(acc_empty + 2);        // [stages] the loading warp's word to the products: their shape, and whether the pair has two blocks
+    uint32_t* tmem_slot = (uint32_t*)(told + MAX_STAGES);
     __shared__ int before[MAX_GROUPS + 1];        // tiles of rows of the groups before
     __shared__ int edge[MAX_GROUPS + 1];          // where the groups' rows begin
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
     const int feat_tiles = (p.features + FEAT - 1) / FEAT, tiles_f = (p.features + 127) / 128, n_kb = (p.K + 63) / 64;
     const int n_pairs = (n_kb + 1) / 2;
     const int total = (p.offsets ? before[p.groups] : (p.rows + p.tok - 1) / p.tok) * feat_tiles;
+    const int my_tiles = (int)blockIdx.x < total ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
     const uint32_t acc0 = p.stages * SLOT_COLS;
 
     if (warp < LOAD_CODES) {
@@ -217,12 +219,14 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 const Tile t = tile_of(p, tile, feat_tiles, before, edge);
                 const int turn = first_pair(t.f, feat_tiles, n_pairs);
+                const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
                 for (; pair < n_pairs; pair += 2, st.move(2, p.stages)) {
                     const int at = turned(pair, turn, n_pairs);
                     uint8_t* dst = smem + (size_t)st.at * 2 * p.x_bytes;
                     ok = mbar_wait(&empty[st.at], st.phase ^ 1, 1);
                     if (!ok) break;
                     const bool two = 2 * at + 1 < n_kb;
+                    told[st.at] = make_uint2(idesc, two);
                     mbar_expect_tx(&full[st.at], two ? 2 * p.x_bytes : p.x_bytes);
                     tma_load_2d(dst, &map_x, &full[st.at], at * 128, t.tok0);
                     if (two) tma_load_2d(dst + p.x_bytes, &map_x, &full[st.at], at * 128 + 64, t.tok0);
@@ -269,11 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             uint64_t desc = desc0;
             Ring ac{0, 0};
             bool ok = true;
-            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-                const Tile t = tile_of(p, tile, feat_tiles, before, edge);
-                const uint32_t idesc = umma_idesc_bf16(128, min(p.tok, (t.tok_end - t.tok0 + 15) & ~15));
-                // the pair, counted from where the tile begins, that has one block of K only
-                const int lone = n_kb & 1 ? n_pairs - 1 - first_pair(t.f, feat_tiles, n_pairs) : -1;
+            for (int left = my_tiles; left > 0 && ok; --left) {
                 for (int pair0 = 0; pair0 < n_pairs && ok; pair0 += p.part_pairs) {
                     ok = mbar_wait(&acc_empty[ac.at], ac.phase ^ 1, 2);
                     if (!ok) break;
@@ -283,11 +283,13 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                         if (!mbar_try_wait_at(bar, phase)) ok = mbar_wait_slow(full + ((bar - full0) >> 3), phase, 3);
                         if (!ok) break;
                         tcgen05_fence_after();
+                        const uint2 of = told[(bar - full0) >> 3];
+                        const uint32_t idesc = of.x;
                         umma_bf16_a_tmem(acc, at_tmem, desc, idesc, pair > pair0 ? 1u : 0u);
                         umma_bf16_a_tmem(acc, at_tmem + 8, desc + 2, idesc, 1);
                         umma_bf16_a_tmem(acc, at_tmem + 16, desc + 4, idesc, 1);
                         umma_bf16_a_tmem(acc, at_tmem + 24, desc + 6, idesc, 1);
-                        if (pair != lone) {
+                        if (of.y) {
                             umma_bf16_a_tmem(acc, at_tmem + 32, desc + desc_half, idesc, 1);
                             umma_bf16_a_tmem(acc, at_tmem + 40, desc + desc_half + 2, idesc, 1);
                             umma_bf16_a_tmem(acc, at_tmem + 48, desc + desc_half + 4, idesc, 1);
@@ -310,7 +312,6 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         const int set = (warp - CONV0) >> 3;
         const uint32_t lanes = (uint32_t)(q * 32 + upper * 16) << 16;
         const uint8_t* mine = code_ring + (GATED ? upper * 4 + q : q * 2 + upper) * PIECE;
-        const int my_tiles = (int)blockIdx.x < total ? (total - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
         Ring st{set, 0}, sl{0, 0};
         sl.move(set, p.stages);
         for (int left = my_tiles * n_pairs - set; left > 0; left -= CONV_SETS, st.move(CONV_SETS, CODE_STAGES), sl.move(CONV_SETS, p.stages)) {
