@@ -1772,7 +1772,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
         _need(row_req, "row_req", torch.int32), _need(table, "table", torch.int32)
         if row_req.numel() != T or table.dim() != 2:
             raise KernelError("rope_kv_write_e4m3: row_req must name each row's request, table must be [requests, pages]")
-    _need_same_device("rope_kv_write_e4m3", qkv, q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
+    _need_same_device("rope_kv_write_e4m3", qkv, q_out, positions, inv_freq, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
     st = _entry("cache_e4m3", "cj_append_e4m3", "piiiippppppppiiiiiiiiipip")(
         qkv.data_ptr(), qkv.stride(0), q_off, k_off if write_kv else 0, v_off if write_kv else 0, q_out.data_ptr(), _at(k_plane), _at(v_plane),
         _at(k_exp), _at(v_exp), positions.data_ptr(), _at(row_req), _at(table), table.shape[0] if write_kv else 0, table.stride(0) if write_kv else 0,
@@ -1822,6 +1822,7 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
     _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, "decode_attention_e4m3")
     _need(positions, "positions", torch.int32), _need(row_req, "row_req", torch.int32)
     T = q.shape[0]
+    _need_same_device("decode_attention_e4m3", positions, row_req)
     if positions.numel() != T or row_req.numel() != T:
         raise KernelError(f"decode_attention_e4m3: positions and row_req must hold one entry for each of {T} rows")
     if not 0 <= splits <= 65535:
@@ -1855,6 +1856,7 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     request are left as they were.  head_dim 64 or 128."""
     _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, "prefill_attention_e4m3")
     _need(req_start, "req_start", torch.int32), _need(req_prior, "req_prior", torch.int32)
+    _need_same_device("prefill_attention_e4m3", req_start, req_prior)
     R = req_prior.numel()
     if req_start.numel() != R + 1 or table.shape[0] < R:
         raise KernelError(f"prefill_attention_e4m3: req_start {tuple(req_start.shape)} and table {tuple(table.shape)} do not fit {R} requests")
@@ -2030,13 +2032,14 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
         _need(a_row_index, "a_row_index", torch.int32)
         if a_row_index.numel() != M:
             raise KernelError(f"gemm_q4: a_row_index must hold an entry for each of {M} rows")
-    _need_same_device("gemm_q4", a, w.data, out, bias, group_offsets, a_row_index)
+    _need_same_device("gemm_q4", a, w.data, w_up and w_up.data, out, bias, group_offsets, a_row_index)
     if M == 0:
         return
     if a.shape[0] == 0:
         raise KernelError("gemm_q4: a has no rows")
     half = 1 if w.group == 32 else 0
-    if q4_on_tcgen05(M, w.features, w.groups if group_offsets is not None else 0) and a.stride(0) % 8 == 0 and a.data_ptr() % 16 == 0:
+    if q4_on_tcgen05(M, w.features, w.groups if group_offsets is not None else 0) and a.stride(0) % 8 == 0 and a.data_ptr() % 16 == 0 \
+            and (a_row_index is not None or a.stride(0) >= w.k):
         global launches
         x, x_rows = a, a.shape[0]
         if a_row_index is not None:

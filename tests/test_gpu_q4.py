@@ -248,3 +248,13 @@ def test_more_groups_than_the_tensor_core_form_has_places_for():
     of = full.repeat_interleave(4, dim=0)
     want = torch.einsum("sk,sfk->sf", x.to(F64), of)
     check(out, want, sums(k, torch.einsum("sk,sfk->sf", x.to(F64).abs(), of.abs())))
+
+
+def test_rows_of_a_shared_in_memory():
+    """One row expanded to many, and rows that overlap."""
+    w, full = weight((6144, 128), 64, seed=9)
+    x = torch.randn(128 + 8 * 63, device=DEV).to(torch.bfloat16)
+    for a in (x[:128].view(1, 128).expand(64, 128), x.as_strided((64, 128), (8, 1))):
+        out = torch.empty((64, 6144), device=DEV)
+        K.gemm_q4(a, w, out)
+        check(out, a.to(F64) @ full.T, sums(128, a.to(F64).abs() @ full.abs().T))
