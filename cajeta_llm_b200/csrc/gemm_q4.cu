@@ -315,7 +315,8 @@ CJ_EXPORT int cj_gemm_q4(const void* x, long long ldx, int x_rows, const void* w
 #define LAUNCH(NTOK, WM, GATED, HALF, AHEAD)                                                                                     \
     {                                                                                                                     \
         constexpr int smem = WARPS * (GATED ? 2 : 1) * WM * 16 * (NTOK + 1) * 4;                                          \
-        cudaError_t e = cudaFuncSetAttribute(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
+        cudaError_t e = smem <= 48 * 1024 ? cudaSuccess                                                                    \
+            : cudaFuncSetAttribute(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
         if (e != cudaSuccess) return (int)e;                                                                              \
         cj::launch(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, dim3((all + WM - 1) / WM, groups, row_tiles), dim3(WARPS * 32), smem, stream, a); \
         return launch_status();                                                                                           \

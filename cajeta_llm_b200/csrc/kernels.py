@@ -1718,9 +1718,28 @@ def _raw() -> int:
     return _raw_stream(_raw_device()) if _raw_stream is not None and _raw_device is not None else torch.cuda.current_stream().cuda_stream
 
 
+def _plain(tensors, dtypes) -> bool:
+    """Whether all are contiguous, of their types and on the current device; where not, the checks one by one say which (a step's calls are bound by
+    the host: those take 0.5 us a tensor, this 0.2)."""
+    here = tensors[0].get_device()
+    if here < 0 or _raw_device is None or here != _raw_device():
+        return False
+    for t, dtype in zip(tensors, dtypes):
+        if t.dtype is not dtype or t.get_device() != here or not t.is_contiguous():
+            return False
+    return True
+
+
+_CACHE_TYPES = (torch.float8_e4m3fn, torch.float8_e4m3fn, torch.uint8, torch.uint8)
+_APPEND_TYPES = _CACHE_TYPES + (torch.bfloat16, torch.int32, torch.int32, torch.int32)
+_ATTEND_TYPES = _CACHE_TYPES + (torch.bfloat16, torch.bfloat16, torch.int32, torch.int32, torch.int32)
+
+
 def _need_e4m3_cache(k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor, page_tokens: int, n_kv: int,
-                     head_dim: int, what: str) -> None:
+                     head_dim: int, what: str, plain: bool) -> None:
     shape = (k_plane.shape[0], n_kv, page_tokens, head_dim)
+    if plain and k_plane.shape == shape and v_plane.shape == shape and k_exp.shape == shape[:3] and v_exp.shape == shape[:3]:
+        return
     for n, t in (("k_plane", k_plane), ("v_plane", v_plane)):
         _need(t, n, torch.float8_e4m3fn)
         if t.shape != shape:
@@ -1752,14 +1771,16 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     an entry is its code times 2^e.  Zeros, and what lies below 448 2^-100, take e = -100; what lies beyond 448 2^119 is cut to it.
     A row whose request (none of ``table``'s) or page (-1) is not there is rotated and not written.  q_out: bfloat16 [T, heads, head_dim];
     head_dim 64 or 128."""
-    _need(q_out, "q_out", torch.bfloat16), _need(positions, "positions", torch.int32)
+    plain = write_kv and _plain((k_plane, v_plane, k_exp, v_exp, q_out, positions, row_req, table), _APPEND_TYPES)
+    if not plain:
+        _need(q_out, "q_out", torch.bfloat16), _need(positions, "positions", torch.int32)
     if not _on_device(qkv) or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise KernelError("rope_kv_write_e4m3: qkv must be a float32 CUDA matrix whose rows are contiguous")
     T = qkv.shape[0]
     if q_out.shape != (T, n_heads, head_dim) or positions.numel() != T:
         raise KernelError(f"rope_kv_write_e4m3: q_out {tuple(q_out.shape)} and positions {tuple(positions.shape)} do not fit {T} rows")
-    ends = [q_off + n_heads * head_dim] + ([k_off + n_kv * head_dim, v_off + n_kv * head_dim] if write_kv else [])
-    if max(ends) > qkv.shape[1] or min(q_off, *(o for o in (k_off, v_off) if write_kv), 1 << 30) < 0:
+    first, last = (min(q_off, k_off, v_off), max(k_off, v_off) + n_kv * head_dim) if write_kv else (q_off, 0)
+    if first < 0 or max(last, q_off + n_heads * head_dim) > qkv.shape[1]:
         raise KernelError(f"rope_kv_write_e4m3: the heads' columns do not lie within the {qkv.shape[1]} of qkv")
     if rotary_dim > 0:
         if inv_freq is None:
@@ -1768,11 +1789,14 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
         if inv_freq.numel() < rotary_dim // 2:
             raise KernelError(f"rope_kv_write_e4m3: inv_freq holds {inv_freq.numel()} entries, the rotation needs {rotary_dim // 2}")
     if write_kv:
-        _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, "rope_kv_write_e4m3")
-        _need(row_req, "row_req", torch.int32), _need(table, "table", torch.int32)
+        _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, "rope_kv_write_e4m3", plain)
+        if not plain:
+            _need(row_req, "row_req", torch.int32), _need(table, "table", torch.int32)
         if row_req.numel() != T or table.dim() != 2:
             raise KernelError("rope_kv_write_e4m3: row_req must name each row's request, table must be [requests, pages]")
-    _need_same_device("rope_kv_write_e4m3", qkv, q_out, positions, inv_freq, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
+    _need_same_device("rope_kv_write_e4m3", qkv, inv_freq)
+    if not plain:
+        _need_same_device("rope_kv_write_e4m3", q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
     st = _entry("cache_e4m3", "cj_append_e4m3", "piiiippppppppiiiiiiiiipip")(
         qkv.data_ptr(), qkv.stride(0), q_off, k_off if write_kv else 0, v_off if write_kv else 0, q_out.data_ptr(), _at(k_plane), _at(v_plane),
         _at(k_exp), _at(v_exp), positions.data_ptr(), _at(row_req), _at(table), table.shape[0] if write_kv else 0, table.stride(0) if write_kv else 0,
@@ -1780,8 +1804,12 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     _check(st, "rope_kv_write_e4m3")
 
 
-def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, what) -> None:
-    _need(q, "q", torch.bfloat16), _need(out, "out", torch.bfloat16), _need(table, "table", torch.int32)
+def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, of_rows, of_requests, names, page_tokens, n_heads, n_kv, head_dim, window,
+                         scale, what) -> None:
+    plain = _plain((k_plane, v_plane, k_exp, v_exp, q, out, table, of_rows, of_requests), _ATTEND_TYPES)
+    if not plain:
+        _need(q, "q", torch.bfloat16), _need(out, "out", torch.bfloat16), _need(table, "table", torch.int32)
+        _need(of_rows, names[0], torch.int32), _need(of_requests, names[1], torch.int32)
     if head_dim not in (64, 128):
         raise KernelError(f"{what} takes heads of 64 or 128, not {head_dim}")
     if n_kv <= 0 or n_heads % n_kv != 0:
@@ -1792,8 +1820,9 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tok
         raise KernelError(f"{what}: table must be [requests, pages]")
     if window < 0 or not scale > 0.0:
         raise KernelError(f"{what}: window must be positive (or 0 for none) and scale positive, found {window} and {scale}")
-    _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, what)
-    _need_same_device(what, q, out, k_plane, v_plane, k_exp, v_exp, table)
+    _need_e4m3_cache(k_plane, v_plane, k_exp, v_exp, page_tokens, n_kv, head_dim, what, plain)
+    if not plain:
+        _need_same_device(what, q, out, k_plane, v_plane, k_exp, v_exp, table, of_rows, of_requests)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1819,10 +1848,9 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
     ``rope_kv_write_e4m3`` writes: row t sees the positions from ``positions[t] + 1 - window`` (0 without a window) to
     ``positions[t]``.  A row of none of ``table``'s requests (-1) sees none: zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
     that share a row's keys (0: by the size of the launch; the results' last bits depend on it).  head_dim 64 or 128."""
-    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, "decode_attention_e4m3")
-    _need(positions, "positions", torch.int32), _need(row_req, "row_req", torch.int32)
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, positions, row_req, ("positions", "row_req"), page_tokens, n_heads, n_kv,
+                         head_dim, window, scale, "decode_attention_e4m3")
     T = q.shape[0]
-    _need_same_device("decode_attention_e4m3", positions, row_req)
     if positions.numel() != T or row_req.numel() != T:
         raise KernelError(f"decode_attention_e4m3: positions and row_req must hold one entry for each of {T} rows")
     if not 0 <= splits <= 65535:
@@ -1854,9 +1882,8 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     ``req_start[r]`` to ``req_start[r + 1]`` of q [T, heads, head_dim] (bfloat16) are request r's tokens from position
     ``req_prior[r]`` on, each sees its request's keys up to its own position, under a window the last ``window`` of them.  Rows of no
     request are left as they were.  head_dim 64 or 128."""
-    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, page_tokens, n_heads, n_kv, head_dim, window, scale, "prefill_attention_e4m3")
-    _need(req_start, "req_start", torch.int32), _need(req_prior, "req_prior", torch.int32)
-    _need_same_device("prefill_attention_e4m3", req_start, req_prior)
+    _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, req_start, req_prior, ("req_start", "req_prior"), page_tokens, n_heads,
+                         n_kv, head_dim, window, scale, "prefill_attention_e4m3")
     R = req_prior.numel()
     if req_start.numel() != R + 1 or table.shape[0] < R:
         raise KernelError(f"prefill_attention_e4m3: req_start {tuple(req_start.shape)} and table {tuple(table.shape)} do not fit {R} requests")
