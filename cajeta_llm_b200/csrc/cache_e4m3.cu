@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 // own, filled by bulk copies of a page's run of rows a step ahead (registers that loads are on their way to would make every shuffle and
 // exponential wait for them).  An e4m3 code is an f16 number exactly: the products are mma.sync m16n8k16 of f16 numbers, float32 out, with the codes
 // as their first operand, so that all 16 rows of a product are keys (or entries) and its columns the heads.  (mma.sync takes e4m3 operands
-// too; with them 64 rows of up to 2,048 keys took 80 us where this takes 63.)
+// too; with them 64 rows of up to 2,048 keys took 80 us where this takes 61.)
 //     S^T = code_k . q^T                              s = S scale 2^e_k
 //     O^T = code_v^T . (p 2^(e_v - R))^T              R: the largest exponent of the values so far; the weights are at most 1 in f16
 // The order of a product's K, and of its rows, is free as long as both sides keep it: a lane's share of a key is HD / 4 neighbouring bytes and
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 // bits down to 2^-21 of that.
 // R is the row's, not the key's: values of a token that are more than 2^14 smaller than the largest the row has met keep fewer bits of their
 // weights, and none beyond 2^24.
-// Bound by DRAM: 2 (HD + 1) bytes a key (64 rows of up to 2,048 keys, 28 heads over 4: 63 us, 70 % of a copy's rate; 32 rows of 4,096: 100 us, 82 %).
+// Bound by DRAM: 2 (HD + 1) bytes a key (64 rows of up to 2,048 keys, 28 heads over 4: 61 us, 73 % of a copy's rate; 32 rows of 4,096: 101 us, 81 %).
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
 constexpr int STEP = 32;                   // keys of a warp's step
@@ -158,6 +158,20 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return *(const uint32_t*)&v;
 }
 
+// A row's blocks, up to eight, can be a cluster and add their results through each other's shared memory; otherwise they leave them to a kernel of its own.
+constexpr int MOST_CLUSTER = 8;
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 ld_of_block(const float* p, int rank) {      // what lies at p in the shared memory of the cluster's block `rank`
+    uint32_t a;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc::smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
 template <int HD, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4m3_kernel(
     const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const uint8_t* __restrict__ kplane, const uint8_t* __restrict__ vplane,
@@ -175,6 +189,8 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
     float (*red)[ROWS][HD + 4] = (float (*)[ROWS][HD + 4])ring;
     __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS];
     __shared__ int sr[WARPS];
+    float* together = (float*)(ring + sizeof(float) * WARPS * ROWS * (HD + 4));    // a cluster's block: its four warps' sums [ROWS][HD] ...
+    __shared__ float2 together_ml[ROWS];                                          // ... and maximum and divisor
     __shared__ uint64_t bars[WARPS][STAGES];
     const int t = blockIdx.x, split = blockIdx.z;
     const int kvh = blockIdx.y / head_batches, hb = blockIdx.y % head_batches;
@@ -454,11 +470,39 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         if (splits == 1) {
             const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
             *(__nv_bfloat162*)(out + head * HD + d) = __floats2bfloat162_rn(a.x * inv, a.y * inv);
-        } else {
+        } else if (part_acc) {
             *(float2*)(part_acc + (head * splits + split) * HD + d) = a;
             if (d == 0) *(float2*)(part_ml + (head * splits + split) * 2) = make_float2(M, L);
+        } else {
+            *(float2*)(together + row * HD + d) = a;
+            if (d == 0) together_ml[row] = make_float2(M, L);
         }
     }
+    if (splits == 1 || part_acc) return;
+    cluster_sync();
+    for (int i = split * WARPS * 32 + tid; i < n_h * (HD / 2); i += splits * WARPS * 32) {
+        const int row = i / (HD / 2), d = 2 * (i % (HD / 2));
+        float2 ml[MOST_CLUSTER], v[MOST_CLUSTER];
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int b = 0; b < MOST_CLUSTER; ++b) {
+            ml[b] = make_float2(-INFINITY, 0.0f);
+            if (b < splits) ml[b] = ld_of_block((const float*)&together_ml[row], b), v[b] = ld_of_block(together + row * HD + d, b);
+            M = fmaxf(M, ml[b].x);
+        }
+        float2 a = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int b = 0; b < MOST_CLUSTER; ++b) {
+            if (ml[b].x == -INFINITY) continue;
+            const float f = exp2f(ml[b].x - M);
+            L = fmaf(ml[b].y, f, L);
+            a.x = fmaf(v[b].x, f, a.x);
+            a.y = fmaf(v[b].y, f, a.y);
+        }
+        const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+        *(__nv_bfloat162*)(out + ((size_t)t * n_heads + h0 + row) * HD + d) = __floats2bfloat162_rn(a.x * inv, a.y * inv);
+    }
+    cluster_sync();                        // (the others may still read this block's shared memory)
 }
 
 // The stretches of every (row, head) added in their order: a warp each.
@@ -531,7 +575,7 @@ CJ_EXPORT int cj_append_e4m3(const float* qkv, int ld, int q_off, int k_off, int
 }
 
 // q, out: bf16 [T, n_heads, hd]; the cache as cj_append_e4m3 writes it.  splits > 1: every row's keys are dealt to that many
-// blocks; part_acc float32 [T, n_heads, splits, hd] and part_ml [T, n_heads, splits, 2] are scratch.  hd: 64 or 128.
+// blocks, which are a cluster (up to eight) or, with scratch given, leave their results to a second kernel: part_acc float32 [T, n_heads, splits, hd] and part_ml [T, n_heads, splits, 2].  hd: 64 or 128.
 // positions null: the rows are portions of requests, req_start int32 [n_requests + 1], req_prior [n_requests] (one split).
 // table: int32 [n_requests, table_stride]; a row of no request sees no key, and a page of no number below n_pages holds none.
 CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const void* vplane, const void* kexp, const void* vexp,
@@ -541,7 +585,7 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
     if (T <= 0) return 0;
     if (!q || !out || !kplane || !vplane || !kexp || !vexp || !table) return CJ_ERR_ARG;
     if (positions ? !row_req : (!req_start || !req_prior || splits != 1)) return CJ_ERR_ARG;
-    if (splits < 1 || (splits > 1 && (!part_acc || !part_ml))) return CJ_ERR_ARG;
+    if (splits < 1 || (splits > MOST_CLUSTER && !part_acc) || (part_acc && !part_ml)) return CJ_ERR_ARG;
     if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || window < 0 || n_requests <= 0 || n_pages <= 0 || !(scale > 0.0f)) return CJ_ERR_SIZE;
     if (hd != 64 && hd != 128) return CJ_ERR_SIZE;
     if (((uintptr_t)q | (uintptr_t)kplane | (uintptr_t)vplane) & 15) return CJ_ERR_ALIGN;
@@ -552,13 +596,28 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
     const dim3 grid(T, n_kv * head_batches, splits);
     auto kern = hd == 128 ? (rows == 8 ? decode_e4m3_kernel<128, 8> : decode_e4m3_kernel<128, 16>)
                           : (rows == 8 ? decode_e4m3_kernel<64, 8> : decode_e4m3_kernel<64, 16>);
-    const int smem = max(WARPS * STAGES * 2 * STEP * hd, WARPS * rows * (hd + 4) * 4);
+    const int smem = max(WARPS * STAGES * 2 * STEP * hd, WARPS * rows * (hd + 4) * 4 + rows * hd * 4);
+    if (splits == 1) part_acc = part_ml = nullptr;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    cj::launch(kern, dim3(grid), dim3(WARPS * 32), smem, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane,
-               (const uint8_t*)vplane, (const uint8_t*)kexp, (const uint8_t*)vexp, positions, row_req, req_start, req_prior, n_requests, table,
-               table_stride, page_tokens, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, n_pages, n_heads, n_kv, head_batches, window, scale * 1.4426950408889634f, splits, part_acc, part_ml);
-    if (splits > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = part_acc ? 1 : splits;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cj::overlap_launches() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kern, (const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane, (const uint8_t*)vplane,
+                       (const uint8_t*)kexp, (const uint8_t*)vexp, positions, row_req, req_start, req_prior, n_requests, table, table_stride,
+                       page_tokens, (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, n_pages, n_heads, n_kv,
+                       head_batches, window, scale * 1.4426950408889634f, splits, part_acc, part_ml);
+    if (part_acc) {
         const int status = launch_status();
         if (status != 0) return status;
         const long long n = (long long)T * n_heads;

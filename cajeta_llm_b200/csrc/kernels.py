@@ -1828,17 +1828,30 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, of_rows,
 @functools.lru_cache(maxsize=4096)
 def e4m3_splits(rows: int, n_heads: int, n_kv: int, span: int, sms: int) -> int:
     """Blocks that share a row's keys in ``decode_attention_e4m3``."""
-    group = n_heads // n_kv
-    blocks, steps = rows * n_kv * -(-group // (16 if group > 8 else 8)), -(-span // 128)
+    blocks, steps = _e4m3_blocks(rows, n_heads, n_kv), -(-span // 128)
 
-    # rounds of three blocks an SM, each a start and steps of 128 keys that take a chain of waits alone (1.1 us) and their bytes' time
-    # together; and the merge.  (us, fitted; measured at 1, 4, 12 or 14 and 32 blocks a row: 32 rows x 4,096 keys of 16 heads 120, 100, 116, 168; eight
-    # rows of up to 32,768, 4 kv heads, 297, 84, 51 or 53, 57; one of 32,768 278, 79, 33, 21; eight of 576, 16 heads, 9, 12, 16, 31)
+    # Rounds of three blocks an SM (rows of uneven lengths fill the last one: half of what it leaves), each a start and steps of 128 keys that take
+    # a chain of waits alone (1.1 us) and their bytes' time together; and what joins them.  (us, fitted; measured at 1, 2, 4, 12 and 32 blocks a row: 64 rows
+    # of up to 2,048 keys, 28 heads over 4, 60, 64, -, 115, 224; 32 rows of 4,096, 16 heads, 119, 108, 104, 114, 166; eight of up to 32,768, 4 kv heads,
+    # 296, 151, 81, 50, 55; one of 32,768 272, 143, 76, 34, 19; eight of 576, 16 heads, 9, 10, 12, 16, 29)
     def cost(n):
-        rounds = -(-blocks * n // (3 * sms))
-        return rounds * (3 + -(-steps // n) * max(1.1, 0.72 * min(3.0, blocks * n / sms))) + (2 + 0.12 * n if n > 1 else 0)
+        rounds = blocks * n / (3 * sms)
+        rounds = 1 if rounds <= 1 else (rounds + math.ceil(rounds)) / 2
+        join = 0 if n == 1 else 0.5 + 0.1 * n if _e4m3_cluster(blocks, n, sms) else 3 + 0.2 * n
+        return rounds * (3 + -(-steps // n) * max(1.1, 0.45 * min(3.0, blocks * n / sms))) + join
 
     return min(range(1, min(steps, 128) + 1), key=cost)
+
+
+def _e4m3_blocks(rows: int, n_heads: int, n_kv: int) -> int:
+    group = n_heads // n_kv
+    return rows * n_kv * -(-group // (16 if group > 8 else 8))
+
+
+def _e4m3_cluster(blocks: int, n: int, sms: int) -> bool:
+    """Whether a row's n blocks are a cluster and join their results themselves: few blocks, which wait for nobody's place.  (us, a cluster and a merge
+    kernel: one row of 576 keys in five blocks 4.9 and 7.0; eight rows of up to 32,768 in eight 62 and 56; 64 rows of up to 2,048 in two 69 and 64)"""
+    return 1 < n <= 8 and blocks * n <= sms
 
 
 def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor,
@@ -1859,7 +1872,8 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
         return
     splits = splits or e4m3_splits(T, n_heads, n_kv, min(window, max_context) if window > 0 else max(1, max_context), _sm_count())
     acc = ml = None
-    if splits > 1:
+    apart = splits > 1 and not _e4m3_cluster(_e4m3_blocks(T, n_heads, n_kv), splits, _sm_count())
+    if apart:
         acc = q.new_empty((T * n_heads * splits * (head_dim + 2),), dtype=torch.float32)       # the blocks' sums, then their maxima and divisors
         ml = acc.data_ptr() + 4 * T * n_heads * splits * head_dim
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
@@ -1867,7 +1881,7 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
         positions.data_ptr(), row_req.data_ptr(), None, None, table.shape[0], table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv,
         head_dim, window, scale, splits, _at(acc), ml, _raw())
     _check(st, "decode_attention_e4m3")
-    if splits > 1:
+    if apart:
         global launches
         launches += 1                      # the merge kernel
 

@@ -291,3 +291,34 @@ def test_another_stream_than_the_default_one():
     side.synchronize()
     want, size = attention(q, [(0, 60 + i) for i in range(40)], stands_for(k, ke), stands_for(v, ve), table, P, kv, 0, 0.1)
     close(out, want, size)
+
+
+@pytest.mark.parametrize("heads,kv,hd,rows,splits", [(16, 16, 128, 1, 8), (20, 1, 64, 3, 2), (8, 2, 128, 2, 5), (16, 16, 128, 9, 8), (8, 8, 64, 70, 3)])
+def test_a_rows_blocks_join_in_a_cluster_and_in_a_kernel_alike(heads, kv, hd, rows, splits):
+    """Both ways, whichever the sizes choose: of stretches without keys too, and of a row that sees none."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows + splits)
+    pages, page = 8 * rows, 16
+    k, v = ((torch.randn((pages, kv, page, hd), generator=g, device=DEV)).to(torch.float8_e4m3fn) for _ in range(2))
+    ke, ve = (torch.randint(120, 132, (pages, kv, page), generator=g, device=DEV).to(torch.uint8) for _ in range(2))
+    q = torch.randn((rows, heads, hd), generator=g, device=DEV).to(torch.bfloat16)
+    table = torch.randperm(pages, generator=g, device=DEV).to(torch.int32).view(rows, 8)
+    positions = (torch.arange(rows, device=DEV) * 37 % 128).to(torch.int32)
+    req = torch.arange(rows, device=DEV, dtype=torch.int32)
+    req[-1] = -1 if rows > 1 else 0
+    got = []
+    for cluster in (True, False):
+        out = torch.full_like(q, 7.0)
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(K, "_e4m3_cluster", lambda *a: cluster)
+            K.decode_attention_e4m3(q, out, k, v, ke, ve, positions, req, table, page, heads, kv, hd, 0, hd ** -0.5, 128, splits=splits)
+        got.append(out)
+    one = torch.empty_like(q)
+    K.decode_attention_e4m3(q, one, k, v, ke, ve, positions, req, table, page, heads, kv, hd, 0, hd ** -0.5, 128, splits=1)
+    # the same weights; sums in another order and roundings of the last bit
+    size = float(one.to(torch.float64).abs().max())
+    for out in got:
+        assert float((out.to(torch.float64) - one.to(torch.float64)).abs().max()) <= 2.0 ** -7 * size
+        if rows > 1:
+            assert not out[-1].any()
+    assert float((got[0].to(torch.float64) - got[1].to(torch.float64)).abs().max()) <= 2.0 ** -8 * size
