@@ -9,9 +9,12 @@
 // turn codes into the bfloat16 tiles in shared memory that both products read, and the rest is attention over a bfloat16 cache: P, as there, is
 // the one rounding.  The codes come by bulk copies of a page's run of rows, pages of any size, one warp's work: a tile's keys travel while its
 // predecessor's values are converted (half the bytes of a bfloat16 cache: 16 KB a tile; plain loads into registers, tried first, held the
-// conversions of the tile before up: 2,048 rows behind 4,096, 28 heads over 4 of 128: 290 us where this takes 254).  The two query tiles take turns between the exponential unit and the tensor
+// conversions of the tile before up: 2,048 rows behind 4,096, 28 heads over 4 of 128: 290 us where this takes 238).  The two query tiles take turns between the exponential unit and the tensor
 // core, each key tile is worked on as two halves of 64 keys, and the reference maximum moves only when it grows by more than 2^8.
-// Every wait is bounded (tc_common.cuh).
+// Where row blocks are few, two or four blocks - a cluster - take neighbouring stretches of the key tiles and join their outputs through each other's
+// shared memory (512 rows behind 4,096, 16 heads: 109 us alone, 66 in two, 42 in four; 100 behind 8,000, 28 heads: 165, 94, 54).
+// Bound, with blocks for all SMs, by what follows on one another in a key tile (3 us: exponentials 1.1, conversions, two products) and by the last
+// round of blocks.  Every wait is bounded (tc_common.cuh).
 #define CJ_LIB "attention_e4m3_tc"
 #include "common.cuh"
 #include "e4m3.cuh"
@@ -44,7 +47,7 @@ struct Args {
     const int *req_start, *req_prior, *table;
     int n_requests, table_stride, page_tokens, page_shift, n_pages, n_heads, n_kv, window;      // page_shift: -1 for a page of no power of two
     float scale_log2;
-    int total_rows, block_rows;
+    int total_rows, block_rows, splits;      // splits: blocks of a cluster that share the keys of a row block, 1, 2 or 4
 };
 
 struct QueryTile {
@@ -54,6 +57,15 @@ struct QueryTile {
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t of_block(const void* p, int rank) {      // what lies at p, in the cluster's block `rank`
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
 }
 
 // four codes times a power of two, as bfloat16
@@ -107,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     const int p0 = p.req_prior[req] + (row0 - p.req_start[req]);
     const int p_last = min(p0 + rows - 1, p.table_stride * p.page_tokens - 1);
     const int key_from = (p.window > 0 && p0 + 1 > p.window) ? p0 + 1 - p.window : 0;
-    const int kt_begin = key_from / BN;
+    int kt_begin = key_from / BN;
     QueryTile qt[QT];
 #pragma unroll
     for (int g = 0; g < QT; ++g) {
@@ -117,9 +129,22 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         qt[g].begin = from / BN - kt_begin;
         qt[g].end = qt[g].rows > 0 ? (qt[g].p0 + qt[g].rows - 1) / BN - kt_begin : qt[g].begin - 1;
     }
-    const int n_tiles = max(qt[0].end, qt[1].end) + 1;
+    int n_tiles = max(qt[0].end, qt[1].end) + 1;
+    // a cluster's blocks take neighbouring stretches of the key tiles and join their results; where that would leave less than two tiles each the first
+    // does it alone
+    const int rank = blockIdx.z;
+    const bool joined = p.splits > 1 && n_tiles >= 2 * p.splits;
+    if (joined) {
+        const int lo = rank * n_tiles / p.splits, hi = (rank + 1) * n_tiles / p.splits;
+        kt_begin += lo;
+        n_tiles = hi - lo;
+#pragma unroll
+        for (int g = 0; g < QT; ++g) qt[g].begin = max(qt[g].begin - lo, 0), qt[g].end = min(qt[g].end - lo, n_tiles - 1);
+    } else if (rank > 0)
+        return;
     const int* tab = p.table + (size_t)req * p.table_stride;
 
+    __shared__ int place[3];               // first row, rows, whether the block joins others (for the end: registers are short between)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = (uint64_t*)(smem + S::BAR);
@@ -139,6 +164,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
+        place[0] = row0, place[1] = rows, place[2] = joined;
         for (int s = 0; s < 2; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], CONV_WARPS);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&k_full[s], CONV_WARPS * 32), mbar_init(&k_empty[s], 1);
@@ -325,7 +351,6 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         const int g = (warp - SOFT0) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const QueryTile mine = g == 0 ? qt[0] : qt[1];
         const int pos = mine.p0 + r, from = (p.window > 0 && pos + 1 > p.window) ? pos + 1 - p.window : 0;
-        const size_t row_at = ((size_t)(row0 + g * BM + r) * p.n_heads + h) * HD;
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + TM_S + g * BN + lane_off, o_addr = tmem_base + TM_O + g * HD + lane_off;
         float m_ref = -INFINITY, l = 0.0f;
@@ -405,16 +430,31 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         }
         // ---- the rows' results ----------------------------------------------------------------------------------
         if (ok && n_mine > 0) ok = mbar_wait_warp(&o_done[g], 0, 18);
-        if (ok && n_mine > 0) {
-            tcgen05_fence_after();
+        tcgen05_fence_after();
+        if (place[2]) {
+            // for the cluster: O as it is, over the tiles of keys and values (both query tiles are done with them), 16-byte chunks turned by the row so
+            // that a warp's rows lie in different banks; the rows' reference maxima and sums over the codes
+            asm volatile("bar.sync 1, %0;" ::"n"(QT * BM) : "memory");
+            float* dst = (float*)(smem + S::K) + (g * BM + r) * HD;
+            const int turn = r & (HD / 4 - 1);
+            ((float2*)(smem + S::CODES))[g * BM + r] = make_float2(ok && n_mine > 0 ? m_ref : -INFINITY, l);
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD && n_mine > 0; c0 += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + c0, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) *(uint4*)(dst + (((c0 >> 2) + q) ^ turn) * 4) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            }
+        } else if (ok && n_mine > 0) {
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            __nv_bfloat16* dst = p.out + row_at;
+            __nv_bfloat16* dst = p.out + ((size_t)(place[0] + g * BM + r) * p.n_heads + blockIdx.x) * HD;
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += 16) {
                 uint32_t o[16];
                 tmem_ld16(o_addr + c0, o);
                 tmem_ld_wait();
-                if (r < mine.rows) {
+                if (g * BM + r < place[1]) {
                     uint4 u[2];
                     __nv_bfloat162* b = (__nv_bfloat162*)u;
 #pragma unroll
@@ -427,6 +467,43 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     }
     tcgen05_fence_before();
     __syncthreads();
+    if (place[2]) {
+        cluster_sync();
+        const int first_row = place[0], n_rows = place[1];
+        // the rows dealt to the cluster's blocks: a warp a row, four entries a lane, the blocks' results in their order
+        const int share = QT * BM / p.splits;
+        for (int i = warp; i < share; i += THREADS / 32) {
+            const int row = (int)blockIdx.z * share + i;
+            if (row >= n_rows) break;
+            float2 ml[4];
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                ml[b] = make_float2(-INFINITY, 0.0f);
+                if (b < p.splits)
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[b].x), "=f"(ml[b].y)
+                                 : "r"(of_block((float2*)(smem + S::CODES) + row, b)) : "memory");
+                M = fmaxf(M, ml[b].x);
+            }
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (lane < HD / 4) {
+                const float* src = (const float*)(smem + S::K) + row * HD + (lane ^ (row & (HD / 4 - 1))) * 4;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    if (ml[b].x == -INFINITY) continue;
+                    float4 v;
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(of_block(src, b)) : "memory");
+                    const float f = exp2f(ml[b].x - M);
+                    L = fmaf(ml[b].y, f, L);
+                    a.x = fmaf(v.x, f, a.x), a.y = fmaf(v.y, f, a.y), a.z = fmaf(v.z, f, a.z), a.w = fmaf(v.w, f, a.w);
+                }
+                const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+                const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+                *(uint2*)(p.out + ((size_t)(first_row + row) * p.n_heads + blockIdx.x) * HD + lane * 4) = make_uint2(*(const uint32_t*)&x, *(const uint32_t*)&y);
+            }
+        }
+        cluster_sync();                    // (the others may still read this block's shared memory)
+    }
     if (warp == PRODUCT) {
         tcgen05_fence_after();
         tmem_dealloc(tmem_base, TM_COLS);
@@ -436,10 +513,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
 }  // namespace
 
 // q, out: bf16 [total_rows, n_heads, hd]; the cache as cj_append_e4m3 writes it; rows req_start[r] .. req_start[r + 1] are request r's
-// from position req_prior[r] on.  hd: 64 or 128; scale > 0.  block_rows: query rows a block, 128 or 256 (0: by the size of the launch).
+// from position req_prior[r] on.  hd: 64 or 128; scale > 0.  block_rows: query rows a block, 128 or 256; splits: blocks that share
+// their keys, 1, 2 or 4 (0: by the size of the launch).
 CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, const void* vplane, const void* kexp, const void* vexp, int n_pages,
                                  const int* req_start, const int* req_prior, int n_requests, int total_rows, const int* table, int table_stride,
-                                 int page_tokens, int n_heads, int n_kv, int hd, int window, float scale, int block_rows, int sms,
+                                 int page_tokens, int n_heads, int n_kv, int hd, int window, float scale, int block_rows, int splits, int sms,
                                  cudaStream_t stream) {
     if (total_rows <= 0 || n_requests <= 0) return 0;
     if (!q || !out || !kplane || !vplane || !kexp || !vexp || !req_start || !req_prior || !table) return CJ_ERR_ARG;
@@ -447,11 +525,12 @@ CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, c
     if (hd != 64 && hd != 128) return CJ_ERR_SIZE;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kplane | (uintptr_t)vplane) & 15) return CJ_ERR_ALIGN;
     if ((long long)n_pages * n_kv * page_tokens > 0x7fffffffLL || (long long)table_stride * page_tokens > 0x7fffffffLL - 256) return CJ_ERR_SIZE;
-    if (block_rows != 128 && block_rows != 256) {
-        // 256 rows a block unless that leaves more than half of the SMs without one
-        const long long blocks = ((long long)(total_rows + 255) / 256 + n_requests - 1) * n_heads;
-        block_rows = 2 * blocks <= sms ? 128 : 256;
-    }
+    // 256 rows a block; where that leaves SMs without one two or four blocks share a row block's keys (a cluster), and where they still do 128 rows
+    // (us, 256 rows alone, in four, 128 alone, in four: 64 rows behind 2,000, 16 heads, 52, 24, 52, 24; 200 behind 300, heads of 64, 18, 18, 15, 16; 256 behind
+    // 1,024, 28 heads, 40, 23, 35, 38: more blocks than SMs)
+    const long long blocks = ((long long)(total_rows + 255) / 256 + n_requests - 1) * n_heads;
+    if (splits != 1 && splits != 2 && splits != 4) splits = 4 * blocks <= sms ? 4 : 2 * blocks <= sms ? 2 : 1;
+    if (block_rows != 128 && block_rows != 256) block_rows = 2 * splits * blocks <= sms ? 128 : 256;
     const long long row_blocks = ((long long)total_rows + block_rows - 1) / block_rows + n_requests;
     if (row_blocks > 65535) return CJ_ERR_SIZE;
     CUtensorMap map_q;
@@ -459,12 +538,25 @@ CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, c
     const Args a{(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const uint8_t*)kplane, (const uint8_t*)vplane, (const uint8_t*)kexp,
                  (const uint8_t*)vexp, req_start, req_prior, table, n_requests, table_stride, page_tokens,
                  (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1, n_pages, n_heads, n_kv, window,
-                 scale * 1.4426950408889634f, total_rows, block_rows};
+                 scale * 1.4426950408889634f, total_rows, block_rows, splits};
     auto kern = hd == 128 ? prefill_e4m3_tc_kernel<128> : prefill_e4m3_tc_kernel<64>;
     const int smem = hd == 128 ? Smem<128>::TOTAL : Smem<64>::TOTAL;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    cj::launch(kern, dim3(n_heads, (unsigned)row_blocks), dim3(THREADS), smem, stream, map_q, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_heads, (unsigned)row_blocks, splits);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = splits;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cj::overlap_launches() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kern, map_q, a);
     return cj::launch_status();
 }
 

@@ -1905,10 +1905,10 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     if T == 0 or R == 0:
         return
     if T > E4M3_ROW_BY_ROW:
-        st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifiip")(
+        st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifiiip")(
             q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
             req_start.data_ptr(), req_prior.data_ptr(), R, T, table.data_ptr(), table.stride(0), page_tokens, n_heads, n_kv, head_dim, window,
-            scale, 0, _sm_count(), _raw())
+            scale, 0, 0, _sm_count(), _raw())
         _check(st, "prefill_attention_e4m3")
         return
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(

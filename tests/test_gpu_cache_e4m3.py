@@ -322,3 +322,34 @@ def test_a_rows_blocks_join_in_a_cluster_and_in_a_kernel_alike(heads, kv, hd, ro
         if rows > 1:
             assert not out[-1].any()
     assert float((got[0].to(torch.float64) - got[1].to(torch.float64)).abs().max()) <= 2.0 ** -8 * size
+
+
+@pytest.mark.parametrize("heads,kv,hd,window,portions", [
+    (4, 2, 128, 0, [(1500, 300)]), (6, 3, 64, 0, [(700, 130), (0, 90), (2100, 257)]), (2, 1, 128, 400, [(3000, 600)]), (3, 1, 128, 0, [(1023, 1), (1200, 40)])])
+def test_portions_whose_keys_blocks_share(heads, kv, hd, window, portions):
+    """One, two and four blocks a row block, chosen by how many SMs there are said to be; rows of no request stay as they are."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(heads + hd)
+    T, page = sum(n for _, n in portions), 16
+    per = -(-max(p + n for p, n in portions) // page)
+    pages = per * len(portions)
+    k, v = ((torch.randn((pages, kv, page, hd), generator=g, device=DEV)).to(torch.float8_e4m3fn) for _ in range(2))
+    ke, ve = (torch.randint(122, 130, (pages, kv, page), generator=g, device=DEV).to(torch.uint8) for _ in range(2))
+    table = torch.randperm(pages, generator=g, device=DEV).to(torch.int32).view(len(portions), per)
+    q = torch.randn((T + 3, heads, hd), generator=g, device=DEV).to(torch.bfloat16)
+    start = [0]
+    for _, n in portions:
+        start.append(start[-1] + n)
+    got = []
+    blocks = -(-(T + 3) // 256) - 1 + len(portions)
+    for sms in (1, 2 * blocks * heads, 4 * blocks * heads, 148):
+        out = torch.full_like(q, 5.0)
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(K, "_sm_count", lambda: sms)
+            K.prefill_attention_e4m3(q, out, k, v, ke, ve, ints(start), ints([p for p, _ in portions]), table, page, heads, kv, hd, window, hd ** -0.5)
+        assert (out[T:] == 5.0).all()
+        got.append(out[:T].to(torch.float64))
+    # weights rounded to bfloat16 against another reference (2^-8 of a value of at most the largest, twice) and the result's rounding
+    most = float((v.to(torch.float64) * torch.exp2(ve.to(torch.float64) - 127)[..., None]).abs().max())
+    for out in got[1:]:
+        assert float((out - got[0]).abs().max()) <= 2.0 ** -7 * most + 2.0 ** -8 * float(got[0].abs().max())
