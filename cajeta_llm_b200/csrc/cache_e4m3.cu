@@ -576,7 +576,7 @@ CJ_EXPORT int cj_append_e4m3(const float* qkv, int ld, int q_off, int k_off, int
 
 // q, out: bf16 [T, n_heads, hd]; the cache as cj_append_e4m3 writes it.  splits > 1: every row's keys are dealt to that many
 // blocks, which are a cluster (up to eight) or, with scratch given, leave their results to a second kernel: part_acc float32 [T, n_heads, splits, hd] and part_ml [T, n_heads, splits, 2].  hd: 64 or 128.
-// positions null: the rows are portions of requests, req_start int32 [n_requests + 1], req_prior [n_requests] (one split).
+// positions null: the rows are portions of requests, req_start int32 [n_requests + 1], req_prior [n_requests] (no scratch).
 // table: int32 [n_requests, table_stride]; a row of no request sees no key, and a page of no number below n_pages holds none.
 CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const void* vplane, const void* kexp, const void* vexp,
                              int n_pages, const int* positions, const int* row_req, const int* req_start, const int* req_prior,
@@ -584,7 +584,7 @@ CJ_EXPORT int cj_decode_e4m3(const void* q, void* out, const void* kplane, const
                              cudaStream_t stream) {
     if (T <= 0) return 0;
     if (!q || !out || !kplane || !vplane || !kexp || !vexp || !table) return CJ_ERR_ARG;
-    if (positions ? !row_req : (!req_start || !req_prior || splits != 1)) return CJ_ERR_ARG;
+    if (positions ? !row_req : (!req_start || !req_prior || part_acc)) return CJ_ERR_ARG;
     if (splits < 1 || (splits > MOST_CLUSTER && !part_acc) || (part_acc && !part_ml)) return CJ_ERR_ARG;
     if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv != 0 || page_tokens <= 0 || window < 0 || n_requests <= 0 || n_pages <= 0 || !(scale > 0.0f)) return CJ_ERR_SIZE;
     if (hd != 64 && hd != 128) return CJ_ERR_SIZE;

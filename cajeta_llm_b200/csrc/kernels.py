@@ -1886,7 +1886,20 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
         launches += 1                      # the merge kernel
 
 
-E4M3_ROW_BY_ROW = 32     # rows of a step of portions up to which they are taken one by one
+E4M3_ROW_BY_ROW = 32     # rows of a step of portions up to which they may be taken one by one; twice as many of at most eight a request
+
+
+@functools.lru_cache(maxsize=4096)
+def e4m3_portions(rows: int, requests: int, n_heads: int, n_kv: int, span: int, sms: int) -> int:
+    """Blocks that share a row's keys where a step's portions are taken row by row, 0 where they go in tiles of query rows.  ``span``: keys that the
+    table has room for."""
+    blocks = _e4m3_blocks(rows, n_heads, n_kv)
+    # Few rows are one by one, their keys shared out as far as SMs go round; where these are taken and the requests so few that their tiles' keys can be
+    # shared out instead, tiles.  (us, row by row without sharing and tiles: one portion of 16 rows, 16 heads, behind 100 tokens 6 and 9, 1,000 19 and 14,
+    # 8,000 120 and 48; two rows, 28 heads over 4, behind 8,000 78, shared out 15, and 45; 36 rows of six requests behind 500 to 3,000, 28 heads over 4, 33 and 80)
+    if rows > (2 * E4M3_ROW_BY_ROW if rows <= 8 * requests else E4M3_ROW_BY_ROW) or (2 * blocks > sms and 2 * requests * n_heads <= sms):
+        return 0
+    return max(1, min(8, sms // blocks, -(-span // 128)))
 
 
 def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor, k_exp: torch.Tensor,
@@ -1904,7 +1917,8 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     T = q.shape[0]
     if T == 0 or R == 0:
         return
-    if T > E4M3_ROW_BY_ROW:
+    splits = e4m3_portions(T, R, n_heads, n_kv, table.shape[1] * page_tokens, _sm_count())
+    if splits == 0:
         st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifiiip")(
             q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
             req_start.data_ptr(), req_prior.data_ptr(), R, T, table.data_ptr(), table.stride(0), page_tokens, n_heads, n_kv, head_dim, window,
@@ -1913,7 +1927,7 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
         return
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
         q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0], None, None,
-        req_start.data_ptr(), req_prior.data_ptr(), R, table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv, head_dim, window, scale, 1,
+        req_start.data_ptr(), req_prior.data_ptr(), R, table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv, head_dim, window, scale, splits,
         None, None, _raw())
     _check(st, "prefill_attention_e4m3")
 

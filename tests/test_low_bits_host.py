@@ -161,6 +161,16 @@ def test_blocks_a_row():
         assert 1 <= K.e4m3_splits(rows, 28, 4, span, 148) <= max(1, -(-span // 128))
 
 
+def test_which_form_portions_take():
+    """Many rows in tiles, few one by one with their keys shared out, a few dozen of one request in tiles."""
+    assert K.e4m3_portions(33, 1, 16, 16, 4096, 148) == 0 and K.e4m3_portions(32, 1, 16, 16, 4096, 148) == 0
+    assert K.e4m3_portions(2, 1, 28, 4, 4096, 148) == 8 and K.e4m3_portions(8, 1, 28, 4, 4096, 148) == 4
+    assert K.e4m3_portions(36, 6, 28, 4, 4096, 148) == 1 and K.e4m3_portions(64, 7, 28, 4, 4096, 148) == 0
+    assert K.e4m3_portions(30, 8, 28, 4, 4096, 148) == 1 and K.e4m3_portions(1, 1, 4, 4, 100, 148) == 1
+    for rows, requests in ((1, 1), (7, 7), (20, 3), (32, 32)):
+        assert 0 <= K.e4m3_portions(rows, requests, 40, 2, 50_000, 148) <= 8
+
+
 def test_which_form_a_4_bit_product_takes():
     assert not K.q4_on_tcgen05(1, 151_936, 0) and not K.q4_on_tcgen05(8, 151_936, 0) and not K.q4_on_tcgen05(64, 2048, 0)
     assert K.q4_on_tcgen05(64, 6144, 0) and K.q4_on_tcgen05(2048, 512, 0)
