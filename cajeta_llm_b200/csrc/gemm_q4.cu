@@ -51,14 +51,13 @@ __global__ void __launch_bounds__(WARPS * 32, NTOK == 8 && AHEAD == 1 ? 4 : 0) g
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int tiles_k = (a.K + 63) / 64, tiles_f = (a.features + 127) / 128;
     const int piece0 = blockIdx.x * WM;                    // of all pieces of 16 features
-    const int grp = blockIdx.y;
-    // where this lane's codes and this lane's scales of a piece lie in the first tile along K (pieces past the last tile of features are not there; the
-    // last tile's are, filled with zeros)
+    // where this lane's codes and this lane's scales of a piece lie in the first tile along K, of a mixture's first group (pieces past the last tile of
+    // features are not there; the last tile's are, filled with zeros)
     const uint8_t* at[W][WM];
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
         const int pc = piece0 + i, ft = min(pc >> 3, tiles_f - 1);
-        const size_t off = ((size_t)grp * tiles_f + ft) * tiles_k * q4::tile_bytes(HALF) + (pc & 7) * PIECE;
+        const size_t off = (size_t)ft * tiles_k * q4::tile_bytes(HALF) + (pc & 7) * PIECE;
         at[0][i] = a.w + off;
         if (GATED) at[W - 1][i] = a.w_up + off;
     }
@@ -87,7 +86,40 @@ __global__ void __launch_bounds__(WARPS * 32, NTOK == 8 && AHEAD == 1 ? 4 : 0) g
     if (!a.offsets) fetch_first();
     cj::after_predecessor();
     cj::release_successor();
-    const int lo = a.offsets ? max(0, a.offsets[grp]) : 0, hi = a.offsets ? min(a.rows, a.offsets[grp + 1]) : a.rows;
+    int lo = 0, hi = a.rows;
+    if (a.offsets) {
+        // The groups that have rows, in their order: this block has the blockIdx.y-th (few rows leave most of 60 experts without one, and blocks
+        // that only find that out hold places: experts of 1,408 x 2,048, gated, one row 11.3 us with a block for every group, 7.7 so, eight rows 21.7 and
+        // 19.2).  No more groups have rows than there are rows.
+        int grp = -1;
+        for (int g0 = 0, seen = 0; g0 < a.groups && grp < 0; g0 += 64) {
+            int from[2], to[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int idx = g0 + 32 * i + lane;
+                from[i] = idx < a.groups ? max(0, a.offsets[idx]) : 0;
+                to[i] = idx < a.groups ? min(a.rows, a.offsets[idx + 1]) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t have = __ballot_sync(0xffffffffu, to[i] > from[i]);
+                const uint32_t mine = __ballot_sync(0xffffffffu, to[i] > from[i] && seen + __popc(have & ((1u << lane) - 1)) == (int)blockIdx.y);
+                seen += __popc(have);
+                if (mine) {
+                    const int l = __ffs(mine) - 1;
+                    grp = g0 + 32 * i + l;
+                    lo = __shfl_sync(0xffffffffu, from[i], l);
+                    hi = __shfl_sync(0xffffffffu, to[i], l);
+                }
+            }
+        }
+        if (grp < 0) return;
+        const size_t off = (size_t)grp * tiles_f * tiles_k * q4::tile_bytes(HALF);
+#pragma unroll
+        for (int i = 0; i < WM; ++i)
+#pragma unroll
+            for (int u = 0; u < W; ++u) at[u][i] += off;
+    }
     for (int row0 = lo + blockIdx.z * NTOK; row0 < hi; row0 += gridDim.z * NTOK) {
         if (a.offsets || row0 != (int)blockIdx.z * NTOK) fetch_first();
         const __nv_bfloat16* xr[NB];
@@ -311,14 +343,14 @@ CJ_EXPORT int cj_gemm_q4(const void* x, long long ldx, int x_rows, const void* w
                  features, K, groups, out_dtype == CJ_BF16 ? 1 : 0, accumulate};
     const int all = (features + 15) / 16;
     // (the blocks of a group take its rows tile by tile: how many it has is not known here)
-    const int row_tiles = offsets ? 1 : min((rows + n_tok - 1) / n_tok, 65535);
+    const int row_tiles = offsets ? 1 : min((rows + n_tok - 1) / n_tok, 65535), grid_groups = offsets ? min(groups, rows) : 1;
 #define LAUNCH(NTOK, WM, GATED, HALF, AHEAD)                                                                                     \
     {                                                                                                                     \
         constexpr int smem = WARPS * (GATED ? 2 : 1) * WM * 16 * (NTOK + 1) * 4;                                          \
         cudaError_t e = smem <= 48 * 1024 ? cudaSuccess                                                                    \
             : cudaFuncSetAttribute(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
         if (e != cudaSuccess) return (int)e;                                                                              \
-        cj::launch(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, dim3((all + WM - 1) / WM, groups, row_tiles), dim3(WARPS * 32), smem, stream, a); \
+        cj::launch(gemm_q4_kernel<NTOK, WM, GATED, HALF, AHEAD>, dim3((all + WM - 1) / WM, grid_groups, row_tiles), dim3(WARPS * 32), smem, stream, a); \
         return launch_status();                                                                                           \
     }
 #define PLAIN(NTOK, WM, AHEAD) { if (half) LAUNCH(NTOK, WM, false, true, AHEAD) else LAUNCH(NTOK, WM, false, false, AHEAD) }

@@ -2110,7 +2110,7 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
         return
     n_tok = 8 if M <= 8 or group_offsets is not None else 16 if M <= 16 else 32
     # Few blocks hide their own loads' time, four tiles ahead; where there are more than four an SM they hide each other's, with registers for that many
-    # (us, four tiles and one: 1 row x 2,048 x 6,144 4.3 and 5.1; 8 rows' experts of 1,408 x 2,048, gated, 28.9 and 21.6, one row's 14.1 and 11.1)
+    # (us, four tiles and one: 1 row x 2,048 x 6,144 4.3 and 5.1; 8 rows' experts of 1,408 x 2,048, gated and with blocks for empty groups too, 28.9 and 21.6, one row's 14.1 and 11.1)
     blocks = (min(M, w.groups) if group_offsets is not None else -(-M // 8)) * -(-w.features // 16)
     ahead = 4 if blocks < 4 * _sm_count() else 1
     st = _entry("gemm_q4", "cj_gemm_q4", "plippppiliiiiippiiip")(
