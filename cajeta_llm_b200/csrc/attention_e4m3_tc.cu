@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + TM_S + g * BN + lane_off, o_addr = tmem_base + TM_O + g * HD + lane_off;
         float m_ref = -INFINITY, l = 0.0f;
-        bool ok = true;
+        bool ok = true, seen = false;
         const int n_mine = mine.end - mine.begin + 1;
         for (int j = 0; j < n_mine && ok; ++j) {
             ok = mbar_wait_warp(&s_full[g], j & 1, 16);
@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
             tcgen05_fence_after();
             // columns [lo, lo + span] are keys this row may see (span < 0: none)
             const int kbase = (kt_begin + mine.begin + j) * BN, lo = max(from - kbase, 0), span = min(pos - kbase, BN - 1) - lo;
+            seen = seen || span >= 0;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 constexpr int HC = BN / 2;
@@ -431,13 +432,15 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         // ---- the rows' results ----------------------------------------------------------------------------------
         if (ok && n_mine > 0) ok = mbar_wait_warp(&o_done[g], 0, 18);
         tcgen05_fence_after();
+        // a row whose keys leave no weight at all has scores of -infinity alone (an infinite query's): a softmax of NaN, not the zeros of a row without keys
+        if (seen && l == 0.0f) l = NAN;
         if (place[2]) {
             // for the cluster: O as it is, over the tiles of keys and values (both query tiles are done with them), 16-byte chunks turned by the row so
             // that a warp's rows lie in different banks; the rows' reference maxima and sums over the codes
             asm volatile("bar.sync 1, %0;" ::"n"(QT * BM) : "memory");
             float* dst = (float*)(smem + S::K) + (g * BM + r) * HD;
             const int turn = r & (HD / 4 - 1);
-            ((float2*)(smem + S::CODES))[g * BM + r] = make_float2(ok && n_mine > 0 ? m_ref : -INFINITY, l);
+            ((float2*)(smem + S::CODES))[g * BM + r] = make_float2(m_ref, ok ? l : 0.0f);
 #pragma unroll 1
             for (int c0 = 0; c0 < HD && n_mine > 0; c0 += 16) {
                 uint32_t o[16];
@@ -490,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
                 const float* src = (const float*)(smem + S::K) + row * HD + (lane ^ (row & (HD / 4 - 1))) * 4;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    if (ml[b].x == -INFINITY) continue;
+                    if (ml[b].y == 0.0f) continue;      // (no key of this block's; NaN scores leave a maximum of -infinity and a sum of NaN)
                     float4 v;
                     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(of_block(src, b)) : "memory");
                     const float f = exp2f(ml[b].x - M);

@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = query_exponent(most);
-        const float up = power_of_two(e), undo = scale_log2 * power_of_two(-e);
+        // (a query that is infinite somewhere has no finite score: all are NaN, as those of one that holds a NaN are by themselves)
+        const float up = most < INFINITY ? power_of_two(e) : NAN, undo = scale_log2 * power_of_two(-e);
         back[n][0] = __shfl_sync(0xffffffffu, undo, 8 * t4);
         back[n][1] = __shfl_sync(0xffffffffu, undo, 8 * t4 + 4);
 #pragma unroll
@@ -436,7 +437,8 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
     }
     __syncthreads();                       // the ring becomes the results' place
 
-    // ---- the four warps' results, added in their order
+    // ---- the four warps' results, added in their order.  Here and below a stretch without keys is one whose sum of weights is 0 (any key leaves 1 or more):
+    // its maximum does not tell, since scores that are NaN leave none and have to be in the result
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            if (sm[w][row] == -INFINITY) continue;
+            if (sl[w][row] == 0.0f) continue;
             const float f = exp2f(sm[w][row] - M), fr = f * power_of_two(max(sr[w], -126));
             L += sl[w][row] * f;
             a.x = fmaf(red[w][row][d], fr, a.x);
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         }
         const size_t head = (size_t)t * n_heads + h0 + row;
         if (splits == 1) {
-            const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             *(__nv_bfloat162*)(out + head * HD + d) = __floats2bfloat162_rn(a.x * inv, a.y * inv);
         } else if (part_acc) {
             *(float2*)(part_acc + (head * splits + split) * HD + d) = a;
@@ -493,13 +495,13 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int b = 0; b < MOST_CLUSTER; ++b) {
-            if (ml[b].x == -INFINITY) continue;
+            if (ml[b].y == 0.0f) continue;
             const float f = exp2f(ml[b].x - M);
             L = fmaf(ml[b].y, f, L);
             a.x = fmaf(v[b].x, f, a.x);
             a.y = fmaf(v[b].y, f, a.y);
         }
-        const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         *(__nv_bfloat162*)(out + ((size_t)t * n_heads + h0 + row) * HD + d) = __floats2bfloat162_rn(a.x * inv, a.y * inv);
     }
     cluster_sync();                        // (the others may still read this block's shared memory)
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(128) decode_e4m3_merge_kernel(__nv_bfloat16* _
     for (int c = 0; c < splits; c += 32) {
         float2 ml = make_float2(-INFINITY, 0.0f);
         if (c + lane < splits) ml = *(const float2*)(part_ml + (s0 + c + lane) * 2);
-        const float mine = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        const float mine = ml.y == 0.0f ? 0.0f : exp2f(ml.x - M);
         L = fmaf(ml.y, mine, L);
         const int n = min(32, splits - c);
 #pragma unroll 8
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(128) decode_e4m3_merge_kernel(__nv_bfloat16* _
         }
     }
     L = warp_sum(L);
-    const float inv = M == -INFINITY ? 0.0f : 1.0f / L;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int j = 0; j < VEC; j += 2)
         *(__nv_bfloat162*)(out + (size_t)idx * HD + lane * VEC + j) = __floats2bfloat162_rn(a[j] * inv, a[j + 1] * inv);

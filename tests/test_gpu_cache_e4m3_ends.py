@@ -1,0 +1,128 @@
+"""The 8-bit cache where a row meets what is not a number, not there, or far apart: every form against the formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from cajeta_llm_b200.csrc import kernels as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F64 = torch.float64
+HALF = 2.0 ** -8           # a rounding to bfloat16, half a step
+
+# One row by itself, its keys dealt out to a cluster and to blocks that a kernel joins; portions row by row, alone and in a cluster; portions in tiles,
+# a block a row block and four.
+FORMS = ["one", "cluster", "merge", "rows", "rows in clusters", "tiles", "tiles in clusters"]
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def make(lengths, kv, hd, page_tokens, seed):
+    """Codes and exponents of all pages (a few more than the requests need), and the requests' pages in mixed order."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    need = [-(-n // page_tokens) for n in lengths]
+    pages, width = sum(need) + 2, max(need)
+    k, v = ((torch.randn((pages, kv, page_tokens, hd), generator=g, device=DEV) * 60).clamp(-448, 448).to(torch.float8_e4m3fn) for _ in range(2))
+    ke, ve = (torch.randint(127 - 8, 127 - 4, (pages, kv, page_tokens), generator=g, device=DEV).to(torch.uint8) for _ in range(2))
+    order = torch.randperm(pages, generator=g, device=DEV).tolist()
+    table = [[order.pop() if i < n else -1 for i in range(width)] for n in need]
+    return k, v, ke, ve, table
+
+
+def at(table, r, key, page_tokens):
+    return table[r][key // page_tokens], key % page_tokens
+
+
+def formula(q, rows, k, v, ke, ve, table, page_tokens, window, scale):
+    """Rows [(request, position)] in 64 bits: softmax over the keys from position + 1 - window to position whose page is there.  The result, and the
+    sum of weight times |value| (what a rounding of weights can move).  No key: zeros."""
+    heads, hd = q.shape[1:]
+    kv = k.shape[1]
+    held = [c.to(F64) * torch.exp2(e.to(F64) - 127)[..., None] for c, e in ((k, ke), (v, ve))]
+    out, size = torch.zeros(q.shape, dtype=F64, device=DEV), torch.zeros(q.shape, dtype=F64, device=DEV)
+    for t, (r, p) in enumerate(rows):
+        keys = torch.arange(max(0, p + 1 - window) if window else 0, max(0, p + 1), device=DEV) if r >= 0 else torch.empty(0, device=DEV, dtype=torch.int64)
+        keys = keys[keys < len(table[0]) * page_tokens]
+        page = ints(table)[r][keys // page_tokens].long()
+        there = (page >= 0) & (page < k.shape[0])
+        if not there.any():
+            continue
+        kk, vv = (x[page[there], :, keys[there] % page_tokens].transpose(0, 1) for x in held)
+        w = torch.softmax((q[t].to(F64).view(kv, -1, hd) @ kk.transpose(1, 2)) * scale, dim=-1)
+        out[t], size[t] = (w @ vv).view(heads, hd), (w @ vv.abs()).view(heads, hd)
+    return out, size
+
+
+def attend(form, q, rows, k, v, ke, ve, table, page_tokens, window, scale):
+    """The rows by one of the forms; those of portions have to be runs of neighbouring positions."""
+    heads, hd = q.shape[1:]
+    kv, out = k.shape[1], torch.full_like(q, 7.0)
+    with pytest.MonkeyPatch.context() as m:
+        if form in FORMS[:3]:
+            if form != "one":
+                m.setattr(K, "_e4m3_cluster", lambda *a: form == "cluster")
+            K.decode_attention_e4m3(q, out, k, v, ke, ve, ints([p for _, p in rows]), ints([r for r, _ in rows]), ints(table), page_tokens, heads, kv, hd,
+                                    window, scale, max(1, max(p for _, p in rows) + 1), splits={"one": 1, "cluster": 3, "merge": 5}[form])
+            return out
+        start, prior = [0], []
+        for r in range(len(table)):
+            mine = [p for s, p in rows if s == r]
+            assert mine == list(range(mine[0], mine[0] + len(mine))) if mine else True
+            start.append(start[-1] + len(mine))
+            prior.append(mine[0] if mine else 0)
+        m.setattr(K, "e4m3_portions", lambda *a: {"rows": 1, "rows in clusters": 3}.get(form, 0))
+        blocks = -(-len(rows) // 256) - 1 + len(table)
+        m.setattr(K, "_sm_count", lambda: 1 if form == "tiles" else 4 * blocks * heads)
+        K.prefill_attention_e4m3(q, out, k, v, ke, ve, ints(start), ints(prior), ints(table), page_tokens, heads, kv, hd, window, scale)
+    assert not K.wait_errors()
+    return out
+
+
+def agree(got, want, size):
+    # the result's rounding, the weights' (2^-8 of each at most: bfloat16 in tiles, f16 for single rows), and 2^-12 for exponentials of float32 scores
+    got = got.to(F64)
+    assert torch.equal(got.isnan(), want.isnan())
+    worst = ((got - want).abs() - HALF * want.abs() - (2.0 ** -8 + 2.0 ** -12) * size).nan_to_num(0.0).max()
+    assert float(worst) <= 1e-30, float(worst)
+
+
+def queries(rows, heads, hd, seed=3):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return torch.randn((rows, heads, hd), generator=g, device=DEV).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 128), (20, 1, 64)])
+@pytest.mark.parametrize("form", FORMS)
+def test_what_is_no_number_and_is_seen_is_in_the_result(form, heads, kv, hd):
+    """Queries with an entry that is NaN or infinite: all of the head's result.  A NaN in a key: all heads that share it, for every row that sees it (the
+    newest key alone in a warp's share, the first, one in between).  A NaN in a value: that entry."""
+    P = 16
+    lengths = [33, 65, 97, 300, 700, 1300]
+    k, v, ke, ve, table = make(lengths, kv, hd, P, seed=heads)
+    rows = [(r, n - 1) for r, n in enumerate(lengths)]
+    scale = 1 / math.sqrt(hd)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        q = queries(len(rows), heads, hd)
+        q[1, 1, 5] = q[3, 0, 0] = q[5, heads - 1, hd - 1] = bad
+        agree(attend(form, q, rows, k, v, ke, ve, table, P, 0, scale), *formula(q, rows, k, v, ke, ve, table, P, 0, scale))
+    # an infinite entry beside keys that are of one sign there: every score is infinite, of either sign
+    signed = k.view(torch.uint8).clone()
+    signed[..., 7] = 0xb0
+    q = queries(len(rows), heads, hd)
+    q[0, 0, 7], q[5, 1, 7] = float("inf"), -float("inf")
+    signed = signed.view(torch.float8_e4m3fn)
+    agree(attend(form, q, rows, signed, v, ke, ve, table, P, 0, scale), *formula(q, rows, signed, v, ke, ve, table, P, 0, scale))
+    q = queries(len(rows), heads, hd)
+    for plane in (0, 1):
+        c = [x.view(torch.uint8).clone() for x in (k, v)]
+        for r, key in ((0, 32), (1, 64), (2, 96), (3, 0), (4, 333), (5, 900)):
+            page, i = at(table, r, key, P)
+            c[plane][page, kv - 1, i, 3] = 0x7f if r % 2 else 0xff
+        kk, vv = (x.view(torch.float8_e4m3fn) for x in c)
+        for window in (0, 64):
+            agree(attend(form, q, rows, kk, vv, ke, ve, table, P, window, scale), *formula(q, rows, kk, vv, ke, ve, table, P, window, scale))
