@@ -68,6 +68,12 @@ __device__ __forceinline__ uint32_t of_block(const void* p, int rank) {      // 
     return a;
 }
 
+// bits lo .. hi of a word, those of them that it has
+__device__ __forceinline__ uint32_t within(int lo, int hi) {
+    lo = max(lo, 0), hi = min(hi, 31);
+    return lo <= hi ? 0xffffffffu >> (31 - (hi - lo)) << lo : 0u;
+}
+
 // four codes times a power of two, as bfloat16
 __device__ __forceinline__ uint2 scaled_codes(uint32_t w, f32x2 f) {
     uint32_t lo, hi;
@@ -145,6 +151,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     const int* tab = p.table + (size_t)req * p.table_stride;
 
     __shared__ int place[3];               // first row, rows, whether the block joins others (for the end: registers are short between)
+    // Which keys of a tile are there, a bit each.  Four tiles: the loader writes tile i's when the keys of i - 1 are converted, so when the scores
+    // of i - 3 are done, which follow the products that read the weights of i - 4.
+    __shared__ uint4 there[4];
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = (uint64_t*)(smem + S::BAR);
@@ -240,6 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         bool ok = true;
         for (int i = 0; i < n_tiles && ok; ++i) {
             int row[4], run[4], have = 0;
+            uint32_t keys[4];
             uint32_t ek[4], ev[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -249,7 +259,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
                 ev[j] = row[j] >= 0 ? p.vexp[row[j]] : 0;
                 const bool first = row[j] >= 0 && (lane == 0 || at_page[j] == 0 || key == key_from);
                 run[j] = first ? min(min(p.page_tokens - at_page[j], 32 - lane), p_last + 1 - key) : 0;
-                have += __popc(__ballot_sync(0xffffffffu, row[j] >= 0));
+                keys[j] = __ballot_sync(0xffffffffu, row[j] >= 0);
+                have += __popc(keys[j]);
             }
             if (i + 1 < n_tiles) ask_pages(i + 1);
 #pragma unroll
@@ -258,6 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
                 if (!ok) break;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) factors[values * BN + j * 32 + lane] = __uint_as_float((values ? ev[j] : ek[j]) << 23);
+                if (values == 0 && lane == 0) there[i & 3] = make_uint4(keys[0], keys[1], keys[2], keys[3]);
                 __syncwarp();
                 if (lane == 0) mbar_expect_tx(&c_full[values], have * HD);
                 __syncwarp();
@@ -360,9 +372,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
             ok = mbar_wait_warp(&s_full[g], j & 1, 16);
             if (!ok) break;
             tcgen05_fence_after();
-            // columns [lo, lo + span] are keys this row may see (span < 0: none)
-            const int kbase = (kt_begin + mine.begin + j) * BN, lo = max(from - kbase, 0), span = min(pos - kbase, BN - 1) - lo;
-            seen = seen || span >= 0;
+            const int kbase = (kt_begin + mine.begin + j) * BN;
+            const uint32_t* present = (const uint32_t*)&there[(mine.begin + j) & 3];
+            const bool whole = from <= kbase && pos >= kbase + BN - 1 && (present[0] & present[1] & present[2] & present[3]) == 0xffffffffu;
+            seen = seen || whole;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 constexpr int HC = BN / 2;
@@ -370,10 +383,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
                 tmem_ld32<0>(s_addr + half * HC, v);
                 tmem_ld32<32>(s_addr + half * HC + 32, v);
                 tmem_ld_wait();
-                if (lo != 0 || span != BN - 1) {
+                if (!whole) {
+                    // a bit for each key this row sees: one of its range that is there
+                    const uint32_t see0 = within(from - kbase - half * HC, pos - kbase - half * HC) & present[2 * half];
+                    const uint32_t see1 = within(from - kbase - half * HC - 32, pos - kbase - half * HC - 32) & present[2 * half + 1];
+                    seen = seen || (see0 | see1) != 0;
 #pragma unroll
                     for (int c = 0; c < HC; ++c)
-                        if (!((unsigned)(half * HC + c - lo) <= (unsigned)span && span >= 0)) v[c] = 0xff800000u;       // -inf
+                        if (!((c < 32 ? see0 : see1) >> (c & 31) & 1)) v[c] = 0xff800000u;       // -inf
                 }
                 // The largest score first, in four chains of three-way maxima, then one pass of exponentials.  (One pass with the reference
                 // maximum so far, which finds the largest on its way and is repeated where that moves the reference, is shorter by the wait for

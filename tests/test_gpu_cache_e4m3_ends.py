@@ -126,3 +126,32 @@ def test_what_is_no_number_and_is_seen_is_in_the_result(form, heads, kv, hd):
         kk, vv = (x.view(torch.float8_e4m3fn) for x in c)
         for window in (0, 64):
             agree(attend(form, q, rows, kk, vv, ke, ve, table, P, window, scale), *formula(q, rows, kk, vv, ke, ve, table, P, window, scale))
+
+
+@pytest.mark.parametrize("page_tokens,hd,window", [(16, 128, 0), (5, 64, 0), (128, 128, 0), (16, 64, 150)])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_page_that_is_not_there_holds_no_key(form, page_tokens, hd, window):
+    """Pages of no number and beyond the pool, at a row's start, in its midst and at its end; a row of which nothing is there."""
+    heads, kv = 6, 2
+    lengths = [40, 300, 700, 290, 200, 1300]
+    k, v, ke, ve, table = make(lengths, kv, hd, page_tokens, seed=page_tokens)
+    for r, key, page in ((0, 39, -1), (1, 0, len(k)), (1, 177, -1), (2, 300, -7), (2, 555, 2 ** 31 - 1), (2, 690, len(k)), (3, 130, -1), (5, 40, -1), (5, 1000, -1)):
+        table[r][key // page_tokens] = page
+    table[4] = [-1] * len(table[4])
+    q = queries(len(lengths) * 3, heads, hd)
+    rows = [(r, n - 3 + i) for r, n in enumerate(lengths) for i in range(3)]
+    scale = 1 / math.sqrt(hd)
+    want, size = formula(q, rows, k, v, ke, ve, table, page_tokens, window, scale)
+    assert not want[12:15].any()
+    agree(attend(form, q, rows, k, v, ke, ve, table, page_tokens, window, scale), want, size)
+
+
+@pytest.mark.parametrize("form", FORMS[5:])
+def test_a_whole_prompt_with_pages_that_are_not_there(form):
+    heads, kv, hd, P = 3, 3, 128, 16
+    k, v, ke, ve, table = make([420], kv, hd, P, seed=1)
+    for i in (0, 3, 4, 11, 25):
+        table[0][i] = -1
+    q = queries(420, heads, hd)
+    rows = [(0, p) for p in range(420)]
+    agree(attend(form, q, rows, k, v, ke, ve, table, P, 0, 0.09), *formula(q, rows, k, v, ke, ve, table, P, 0, 0.09))
