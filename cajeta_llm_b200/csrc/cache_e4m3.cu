@@ -125,13 +125,15 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 // as their first operand, so that all 16 rows of a product are keys (or entries) and its columns the heads.  (mma.sync takes e4m3 operands
 // too; with them 64 rows of up to 2,048 keys took 80 us where this takes 61.)
 //     S^T = code_k . q^T                              s = S scale 2^e_k
-//     O^T = code_v^T . (p 2^(e_v - R))^T              R: the largest exponent of the values so far; the weights are at most 1 in f16
+//     O^T = code_v^T . (p 2^(m + e_v - N))^T          m: a head's largest score so far, N: its reference of what keys bring, both in octaves
 // The order of a product's K, and of its rows, is free as long as both sides keep it: a lane's share of a key is HD / 4 neighbouring bytes and
 // of four value rows HD / 8 each (two keys' bytes side by side after a byte permute), 8- and 16-byte loads.  The weights turn from S^T's layout
 // into an operand by movmatrix.  Queries are brought to [2^7, 2^8) at their largest entry by a power of two: f16 keeps an entry's eight
 // bits down to 2^-21 of that.
-// R is the row's, not the key's: values of a token that are more than 2^14 smaller than the largest the row has met keep fewer bits of their
-// weights, and none beyond 2^24.
+// N is an integer, 12 below the largest s + e_v when it was last moved; it moves when a key may bring more than 2^15 of it.  So the factors are at most
+// 2^15 in f16 and keep its 11 bits down to 2^-26 of the largest contribution, some down to 2^-36, whatever weight and value make it up, and the rest is what
+// float32 weights lose too (those below 2^-126).  A reference of the values' exponents alone, one for a warp, was 2 to 4 % faster (64 rows of up to 2,048 keys
+// 61 us, 62 so; eight of up to 32,768 49 and 51) and lost all others to a large value that the row hardly looks at.  The divisor's weights are not rounded.
 // Bound by DRAM: 2 (HD + 1) bytes a key (64 rows of up to 2,048 keys, 28 heads over 4: 61 us, 73 % of a copy's rate; 32 rows of 4,096: 101 us, 81 %).
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
@@ -187,8 +189,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
     cj::release_successor();
     extern __shared__ __align__(128) uint8_t ring[];                   // [WARPS][STAGES][keys, values][STEP][HD], then the warps' results
     float (*red)[ROWS][HD + 4] = (float (*)[ROWS][HD + 4])ring;
-    __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS];
-    __shared__ int sr[WARPS];
+    __shared__ float sm[WARPS][ROWS], sl[WARPS][ROWS], sn[WARPS][ROWS];
     float* together = (float*)(ring + sizeof(float) * WARPS * ROWS * (HD + 4));    // a cluster's block: its four warps' sums [ROWS][HD] ...
     __shared__ float2 together_ml[ROWS];                                          // ... and maximum and divisor
     __shared__ uint64_t bars[WARPS][STAGES];
@@ -287,12 +288,11 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
-    float m[NB][2], l[NB][2];
+    float m[NB][2], l[NB][2], N[NB][2], h[NB][2];      // h: 2^(m - N)
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.0f;
-    int R = 0;                             // + 127
+        for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.0f, N[n][e] = -1e30f, h[n][e] = 0.0f;      // (N finite: m - N stays -infinity)
 
     uint32_t phase = 0;
     for (int stage = 0; k0 < last; k0 += STRIDE) {
@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
 #pragma unroll
                     for (int n = 0; n < NB; ++n) s[n][b >> 1][2 * (b & 1)] = s[n][b >> 1][2 * (b & 1) + 1] = -INFINITY;
         }
-        const int most = max(R, __reduce_max_sync(0xffffffffu, v_exp));
-        bool moved = most != R;
+        const float most = (float)(__reduce_max_sync(0xffffffffu, v_exp) - 127);
+        bool moved = false;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -362,11 +362,10 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 mx[n][e] = fmaxf(m[n][e], x * back[n][e]);
-                moved = moved || mx[n][e] != m[n][e];
+                // (no key brings more than the largest score and the largest exponent together; whether one does is looked at below)
+                moved = moved || mx[n][e] != m[n][e] || fmaf(x, back[n][e], most) > N[n][e] + 15.0f;
             }
         if (__any_sync(0xffffffffu, moved)) {
-            const float down = power_of_two(max(R - most, -126));
-            R = most;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 float old[2];
@@ -374,8 +373,18 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
                 for (int e = 0; e < 2; ++e) {
                     old[e] = mx[n][e] == -INFINITY ? 1.0f : ex2(m[n][e] - mx[n][e]);
                     l[n][e] *= old[e];
-                    old[e] *= down;
                     m[n][e] = mx[n][e];
+                    float y = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        y = fmaxf(y, fmaf(s[n][b >> 1][2 * (b & 1) + e], back[n][e], (float)(__shfl_sync(0xffffffffu, v_exp, b * 8 + g) - 127)));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                    y = y > N[n][e] + 15.0f ? ceilf(y) - 12.0f : N[n][e];
+                    old[e] = ex2(N[n][e] - y);
+                    N[n][e] = y;
+                    h[n][e] = ex2(m[n][e] - y);
                 }
 #pragma unroll
                 for (int i = 0; i < NT; ++i)
@@ -384,7 +393,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
             }
         }
         // ---- weights: pb[n][b] of head 8 n + g and keys 8 b + 2 t4 + {0, 1}
-        const float vf = power_of_two(max(v_exp - R, -126));
+        const float vf = power_of_two(max(v_exp - 127, -126));
         uint32_t pb[NB][4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -396,7 +405,7 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
                 for (int e = 0; e < 2; ++e) {
                     const float w = ex2(fmaf(s[n][b >> 1][2 * (b & 1) + e], back[n][e], m[n][e] == -INFINITY ? 0.0f : -m[n][e]));
                     l[n][e] += w;
-                    x[e] = w * f;
+                    x[e] = w * f * h[n][e];          // (in this order: f h alone could leave float32)
                 }
                 pb[n][b] = transposed(pack_f16(x[0], x[1]));
             }
@@ -447,11 +456,10 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
             l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
-            if (g == 0) sm[warp][head] = m[n][e], sl[warp][head] = l[n][e];
+            if (g == 0) sm[warp][head] = m[n][e], sl[warp][head] = l[n][e], sn[warp][head] = N[n][e];
 #pragma unroll
             for (int i = 0; i < NT; ++i) *(float2*)&red[warp][head][g * (HD / 8) + 2 * i] = make_float2(o[n][i][e], o[n][i][2 + e]);
         }
-    if (lane == 0) sr[warp] = R - 127;
     __syncthreads();
     for (int i = tid; i < n_h * (HD / 2); i += WARPS * 32) {
         const int row = i / (HD / 2), d = 2 * (i % (HD / 2));
@@ -463,8 +471,8 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             if (sl[w][row] == 0.0f) continue;
-            const float f = exp2f(sm[w][row] - M), fr = f * power_of_two(max(sr[w], -126));
-            L += sl[w][row] * f;
+            const float fr = exp2f(sn[w][row] - M);      // (weights that were kept beside N, as sums beside M)
+            L += sl[w][row] * exp2f(sm[w][row] - M);
             a.x = fmaf(red[w][row][d], fr, a.x);
             a.y = fmaf(red[w][row][d + 1], fr, a.y);
         }

@@ -155,3 +155,47 @@ def test_a_whole_prompt_with_pages_that_are_not_there(form):
     q = queries(420, heads, hd)
     rows = [(0, p) for p in range(420)]
     agree(attend(form, q, rows, k, v, ke, ve, table, P, 0, 0.09), *formula(q, rows, k, v, ke, ve, table, P, 0, 0.09))
+
+
+@pytest.mark.parametrize("below,above,n,where", [
+    (40, 25, 200, 0), (40, 25, 200, 77), (40, 25, 200, 199), (20, 30, 200, 5), (100, 90, 200, 40), (12, 60, 130, 129), (30, 0, 200, 0), (-40, -30, 200, 100),
+    (-25, -60, 200, 0), (60, 40, 5000, 2500)])
+@pytest.mark.parametrize("form", FORMS)
+def test_a_large_value_that_a_row_hardly_looks_at_takes_nothing_from_the_others(form, below, above, n, where):
+    """One key whose score lies `below` octaves under the others' and whose value `above` octaves over theirs (all of one sign)."""
+    heads, kv, hd, P = 4, 2, 128, 16
+    k, v, ke, ve, table = make([n], kv, hd, P, seed=n)
+    v = (v.float().abs() + 1).to(torch.float8_e4m3fn)
+    k = torch.zeros_like(k.float())
+    page, i = at(table, 0, where, P)
+    k[page, :, i, 0] = -1.0
+    k = k.to(torch.float8_e4m3fn)
+    ke.fill_(127), ve.fill_(127 - 8)
+    ve[page, :, i] += above if above >= 0 else 256 + above
+    scale = 0.125
+    q = torch.zeros((2, heads, hd), device=DEV)
+    q[..., 0] = below / (scale * math.log2(math.e))
+    q = q.to(torch.bfloat16)
+    rows = [(0, n - 2), (0, n - 1)]
+    agree(attend(form, q, rows, k, v, ke, ve, table, P, 0, scale), *formula(q, rows, k, v, ke, ve, table, P, 0, scale))
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_many_small_weights_beside_a_large_value_and_a_large_weight(form):
+    """The largest weight is of a value of nothing, the largest value of a weight of nothing: what is left is most of the result."""
+    heads, kv, hd, P, n = 4, 4, 64, 16, 20_000
+    k, v, ke, ve, table = make([n], kv, hd, P, seed=6)
+    v = (v.float().abs() + 1).to(torch.float8_e4m3fn)
+    ve.fill_(127 - 8), ke.fill_(127)
+    k = torch.zeros_like(k.float())
+    for key, score, e in ((17, 12.0, -60), (2066, -60.0, 13)):
+        page, i = at(table, 0, key, P)
+        k[page, :, i, 0] = score
+        ve[page, :, i] = 127 - 8 + e
+    k = k.to(torch.float8_e4m3fn)
+    q = torch.zeros((1, heads, hd), device=DEV)
+    q[..., 0] = 1.0
+    q = q.to(torch.bfloat16)
+    scale = 1 / math.log2(math.e)
+    rows = [(0, n - 1)]
+    agree(attend(form, q, rows, k, v, ke, ve, table, P, 0, scale), *formula(q, rows, k, v, ke, ve, table, P, 0, scale))
