@@ -209,12 +209,13 @@ __global__ void __launch_bounds__(WARPS * 32, ROWS == 16 ? 2 : BLOCKS) decode_e4
         if (req == n_requests || t < req_start[req]) return;
         p = req_prior[req] + t - req_start[req];
     }
-    p = req >= 0 ? min(p, table_stride * page_tokens - 1) : -1;
-    const int from = window > 0 && p + 1 > window ? p + 1 - window : 0;
-    const int n_keys = p - from + 1;
+    if (req < 0) p = -1;
+    // keys [from, end): the window is the position's, also where the table ends before it
+    const int from = window > 0 && p >= window ? p - window + 1 : 0, end = min(p, table_stride * page_tokens - 1) + 1;
+    const int n_keys = max(0, end - from);
     // equal stretches of whole steps
     const int per = (((n_keys + splits - 1) / splits + STEP - 1) / STEP) * STEP;
-    const int first = from + split * per, last = min(p + 1, first + per);
+    const int first = from + split * per, last = min(end, first + per);
     const int* tab = table + (size_t)max(req, 0) * table_stride;
 
     // Lane j looks up key j of a step: its page two steps before the products, from it the key's row in the planes (-1: none) and its exponents one

@@ -199,3 +199,13 @@ def test_many_small_weights_beside_a_large_value_and_a_large_weight(form):
     scale = 1 / math.log2(math.e)
     rows = [(0, n - 1)]
     agree(attend(form, q, rows, k, v, ke, ve, table, P, 0, scale), *formula(q, rows, k, v, ke, ve, table, P, 0, scale))
+
+
+@pytest.mark.parametrize("window", [0, 1, 30, 100, 500])
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_behind_the_tables_last_page_see_the_keys_of_their_window(form, window):
+    heads, kv, hd, P = 4, 2, 128, 16
+    k, v, ke, ve, table = make([256, 256, 256], kv, hd, P, seed=4)
+    rows = [(0, 253), (0, 254), (0, 255), (0, 256), (0, 257), (1, 280), (1, 281), (2, 700), (2, 701)]
+    q = queries(len(rows), heads, hd)
+    agree(attend(form, q, rows, k, v, ke, ve, table, P, window, 0.1), *formula(q, rows, k, v, ke, ve, table, P, window, 0.1))
