@@ -123,17 +123,19 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     if (rows <= 0) return;
     const int h = blockIdx.x, kvh = h / (p.n_heads / p.n_kv);
     const int p0 = p.req_prior[req] + (row0 - p.req_start[req]);
-    const int p_last = min(p0 + rows - 1, p.table_stride * p.page_tokens - 1);
-    const int key_from = (p.window > 0 && p0 + 1 > p.window) ? p0 + 1 - p.window : 0;
-    int kt_begin = key_from / BN;
+    // (rows before the first position or behind the table's last page have a tile of the table too, in which they see no key)
+    const int last_key = p.table_stride * p.page_tokens - 1, p_last = min(p0 + rows - 1, last_key);
+    const int key_from = (p.window > 0 && p0 >= p.window) ? p0 - p.window + 1 : 0;
+    auto tile_of = [&](int key) { return min(max(key, 0), last_key) / BN; };
+    int kt_begin = tile_of(key_from);
     QueryTile qt[QT];
 #pragma unroll
     for (int g = 0; g < QT; ++g) {
         qt[g].rows = max(0, min(BM, rows - g * BM));
         qt[g].p0 = p0 + g * BM;
-        const int from = (p.window > 0 && qt[g].p0 + 1 > p.window) ? qt[g].p0 + 1 - p.window : 0;
-        qt[g].begin = from / BN - kt_begin;
-        qt[g].end = qt[g].rows > 0 ? (qt[g].p0 + qt[g].rows - 1) / BN - kt_begin : qt[g].begin - 1;
+        const int from = (p.window > 0 && qt[g].p0 >= p.window) ? qt[g].p0 - p.window + 1 : 0;
+        qt[g].begin = tile_of(from) - kt_begin;
+        qt[g].end = qt[g].rows > 0 ? tile_of(qt[g].p0 + qt[g].rows - 1) - kt_begin : qt[g].begin - 1;
     }
     int n_tiles = max(qt[0].end, qt[1].end) + 1;
     // a cluster's blocks take neighbouring stretches of the key tiles and join their results; where that would leave less than two tiles each the first
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         // ---- softmax of one query tile, a row a thread ------------------------------------------------------------
         const int g = (warp - SOFT0) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const QueryTile mine = g == 0 ? qt[0] : qt[1];
-        const int pos = mine.p0 + r, from = (p.window > 0 && pos + 1 > p.window) ? pos + 1 - p.window : 0;
+        const int pos = mine.p0 + r, from = (p.window > 0 && pos >= p.window) ? pos - p.window + 1 : 0;
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + TM_S + g * BN + lane_off, o_addr = tmem_base + TM_O + g * HD + lane_off;
         float m_ref = -INFINITY, l = 0.0f;

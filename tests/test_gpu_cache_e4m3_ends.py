@@ -209,3 +209,15 @@ def test_rows_behind_the_tables_last_page_see_the_keys_of_their_window(form, win
     rows = [(0, 253), (0, 254), (0, 255), (0, 256), (0, 257), (1, 280), (1, 281), (2, 700), (2, 701)]
     q = queries(len(rows), heads, hd)
     agree(attend(form, q, rows, k, v, ke, ve, table, P, window, 0.1), *formula(q, rows, k, v, ke, ve, table, P, window, 0.1))
+
+
+@pytest.mark.parametrize("prior,rows,window", [(-300, 150, 0), (-300, 150, 20), (-1000, 400, 0), (-40, 200, 0), (10_000_000, 40, 0), (10_000_000, 40, 1000),
+                                               (150, 300, 0), (150, 300, 90)])
+@pytest.mark.parametrize("form", FORMS[3:])
+def test_rows_outside_the_table_see_the_keys_that_are_there(form, prior, rows, window):
+    """Before the first position, behind the last page, and on both sides of it: no key, or those of the table that are in reach."""
+    heads, kv, hd, P = 2, 1, 64, 16
+    k, v, ke, ve, table = make([200], kv, hd, P, seed=2)
+    q = queries(rows, heads, hd)
+    at_ = [(0, prior + i) for i in range(rows)]
+    agree(attend(form, q, at_, k, v, ke, ve, table, P, window, 0.1), *formula(q, at_, k, v, ke, ve, table, P, window, 0.1))
