@@ -68,6 +68,17 @@ __device__ __forceinline__ uint32_t of_block(const void* p, int rank) {      // 
     return a;
 }
 
+// The codes of a word that are NaN (0x7f and 0xff) made zeros; whether there were any
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ bool drop_nan(uint32_t& w) {
+    const uint32_t hit = nan_codes(w);
+    w &= ~((hit >> 7) * 0xffu);
+    return hit != 0;
+}
+
+// the first position that a row at `pos` sees
+__device__ __forceinline__ int from_of(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+
 // bits lo .. hi of a word, those of them that it has
 __device__ __forceinline__ uint32_t within(int lo, int hi) {
     lo = max(lo, 0), hi = min(hi, 31);
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     const int p0 = p.req_prior[req] + (row0 - p.req_start[req]);
     // (rows before the first position or behind the table's last page have a tile of the table too, in which they see no key)
     const int last_key = p.table_stride * p.page_tokens - 1, p_last = min(p0 + rows - 1, last_key);
-    const int key_from = (p.window > 0 && p0 >= p.window) ? p0 - p.window + 1 : 0;
+    const int key_from = from_of(p0, p.window);
     auto tile_of = [&](int key) { return min(max(key, 0), last_key) / BN; };
     int kt_begin = tile_of(key_from);
     QueryTile qt[QT];
@@ -133,8 +144,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     for (int g = 0; g < QT; ++g) {
         qt[g].rows = max(0, min(BM, rows - g * BM));
         qt[g].p0 = p0 + g * BM;
-        const int from = (p.window > 0 && qt[g].p0 >= p.window) ? qt[g].p0 - p.window + 1 : 0;
-        qt[g].begin = tile_of(from) - kt_begin;
+        qt[g].begin = tile_of(from_of(qt[g].p0, p.window)) - kt_begin;
         qt[g].end = qt[g].rows > 0 ? tile_of(qt[g].p0 + qt[g].rows - 1) - kt_begin : qt[g].begin - 1;
     }
     int n_tiles = max(qt[0].end, qt[1].end) + 1;
@@ -152,7 +162,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         return;
     const int* tab = p.table + (size_t)req * p.table_stride;
 
-    __shared__ int place[3];               // first row, rows, whether the block joins others (for the end: registers are short between)
+    __shared__ int place[7];               // first row, rows, whether the block joins others and more (for the end: registers are short between)
+    // A weight of 0 times a value of NaN is NaN, for rows that do not see the key.  In key tiles that some rows see part of, NaN among the values are put
+    // down as zeros, and written at the end to the rows that see them.
+    __shared__ int dropped;
     // Which keys of a tile are there, a bit each.  Four tiles: the loader writes tile i's when the keys of i - 1 are converted, so when the scores
     // of i - 3 are done, which follow the products that read the weights of i - 4.
     __shared__ uint4 there[4];
@@ -175,7 +188,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        place[0] = row0, place[1] = rows, place[2] = joined;
+        place[0] = row0, place[1] = rows, place[2] = joined, place[3] = p0, place[4] = kt_begin, place[5] = n_tiles, place[6] = req;
+        dropped = 0;
         for (int s = 0; s < 2; ++s) mbar_init(&c_full[s], 1), mbar_init(&c_empty[s], CONV_WARPS);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&k_full[s], CONV_WARPS * 32), mbar_init(&k_empty[s], 1);
@@ -202,6 +216,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         const int piece = PIECES == 8 ? ((lane & 3) | (lane >> 4 << 2)) ^ ((in_warp & 1) << 2) : lane & 3;
         const int chunk = (piece & 3) * 2, r0 = warp * ROWS_WARP + in_warp;
         const float* factors = (const float*)(smem + S::FACTORS);
+        // key tiles [all_from, all_to) are seen whole by every row
+        const int all_from = from_of(p0 + rows - 1, p.window), all_to = p0 + 1;
         bool ok = true;
         for (int i = 0; i < 2 * n_tiles && ok; ++i) {
             const int values = i & 1, t = i >> 1, s = t % STAGES;
@@ -209,6 +225,16 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
             if (!ok) break;
             const uint8_t* codes = smem + S::CODES + values * BN * HD + piece * 16;
             uint8_t* dst = smem + (values ? S::V : S::K) + s * TILE + (piece >> 2) * HALF_BYTES;
+            // (where the codes lie, each lane its own: a branch among the conversions costs the tiles that need none 5 %)
+            if (values && ((kt_begin + t) * BN < all_from || (kt_begin + t + 1) * BN > all_to)) {
+#pragma unroll 1
+                for (int r = r0; r < BN; r += ROWS_PASS) {
+                    uint4* at = (uint4*)(smem + S::CODES + (BN + r) * HD + piece * 16);
+                    uint4 c = *at;
+                    const bool x = drop_nan(c.x), y = drop_nan(c.y), z = drop_nan(c.z), w = drop_nan(c.w);
+                    if ((x || y || z || w) && factors[BN + r] != 0.0f) *at = c, dropped = 1;
+                }
+            }
             // (the passes' chains side by side: all loads first, and only the last pass may have no row)
             uint4 c[PASSES];
             float scale[PASSES];
@@ -364,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
         // ---- softmax of one query tile, a row a thread ------------------------------------------------------------
         const int g = (warp - SOFT0) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const QueryTile mine = g == 0 ? qt[0] : qt[1];
-        const int pos = mine.p0 + r, from = (p.window > 0 && pos >= p.window) ? pos - p.window + 1 : 0;
+        const int pos = mine.p0 + r, from = from_of(pos, p.window);
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t s_addr = tmem_base + TM_S + g * BN + lane_off, o_addr = tmem_base + TM_O + g * HD + lane_off;
         float m_ref = -INFINITY, l = 0.0f;
@@ -525,6 +551,19 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
             }
         }
         cluster_sync();                    // (the others may still read this block's shared memory)
+    }
+    if (dropped) {                         // rare: a warp a key, the rows that see it
+        const int first_row = place[0], n_rows = place[1], pos0 = place[3], key0 = place[4] * BN, end = min(pos0 + n_rows, p.table_stride * p.page_tokens);
+        for (int key = key0 + warp; key < min(key0 + place[5] * BN, end); key += THREADS / 32) {
+            if (key < from_of(pos0, p.window)) continue;
+            const int tile0 = key / BN * BN, page = p.table[(size_t)place[6] * p.table_stride + key / p.page_tokens];
+            if ((tile0 >= from_of(pos0 + n_rows - 1, p.window) && tile0 + BN <= pos0 + 1) || page < 0 || page >= p.n_pages) continue;
+            const size_t at = ((size_t)(page * p.n_kv + blockIdx.x / (p.n_heads / p.n_kv)) * p.page_tokens + key % p.page_tokens) * HD;
+            const int to = p.window > 0 && key - pos0 < n_rows - p.window ? key - pos0 + p.window : n_rows;
+            for (int d = lane; d < HD; d += 32)
+                if (nan_codes(p.vplane[at + d]) & 0x80)
+                    for (int r = max(0, key - pos0); r < to; ++r) p.out[((size_t)(first_row + r) * p.n_heads + blockIdx.x) * HD + d] = __float2bfloat16_rn(NAN);
+        }
     }
     if (warp == PRODUCT) {
         tcgen05_fence_after();

@@ -221,3 +221,21 @@ def test_rows_outside_the_table_see_the_keys_that_are_there(form, prior, rows, w
     q = queries(rows, heads, hd)
     at_ = [(0, prior + i) for i in range(rows)]
     agree(attend(form, q, at_, k, v, ke, ve, table, P, window, 0.1), *formula(q, at_, k, v, ke, ve, table, P, window, 0.1))
+
+
+@pytest.mark.parametrize("prior,rows,window", [(0, 300, 0), (100, 200, 0), (1000, 520, 0), (300, 400, 90), (0, 130, 1)])
+@pytest.mark.parametrize("form", FORMS[3:])
+def test_a_value_that_is_no_number_reaches_the_rows_that_see_it_alone(form, prior, rows, window):
+    """Rows before it, and those whose window has left it behind, share tiles and blocks with the rows that do."""
+    heads, kv, hd, P = 4, 2, 128, 16
+    k, v, ke, ve, table = make([prior + rows], kv, hd, P, seed=rows)
+    c = v.view(torch.uint8).clone()
+    for key, head, entry in ((prior + rows // 2, 0, 3), (prior + rows - 1, 1, 127), (prior + rows - 2, 0, 0), (prior + 7, 1, 64), (max(0, prior - 40), 0, 77)):
+        page, i = at(table, 0, key, P)
+        c[page, head, i, entry] = 0xff
+    v = c.view(torch.float8_e4m3fn)
+    q = queries(rows, heads, hd)
+    where = [(0, prior + i) for i in range(rows)]
+    want, size = formula(q, where, k, v, ke, ve, table, P, window, 0.09)
+    assert want.isnan().any() and not want[:, 0, 0].isnan()[0]
+    agree(attend(form, q, where, k, v, ke, ve, table, P, window, 0.09), want, size)
