@@ -463,7 +463,8 @@ CJ_EXPORT int cj_gemm_q4_tc(const void* x, long long ldx, int x_rows, const void
     const long long most = offsets ? sms : (long long)feat_tiles * ((rows + tok - 1) / tok);
     auto kern = w_up ? (half ? gemm_q4_tc_kernel<true, true> : gemm_q4_tc_kernel<true, false>)
                      : (half ? gemm_q4_tc_kernel<false, true> : gemm_q4_tc_kernel<false, false>);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // (the most that any call asks for: the attribute is the kernel's, and another thread may set it between here and the launch)
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
     if (e != cudaSuccess) return (int)e;
     cj::launch(kern, dim3((unsigned)(most < sms ? most : sms)), dim3(THREADS), smem, stream, map, a);
     return cj::launch_status();
