@@ -1825,10 +1825,14 @@ def _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, of_rows,
         _need_same_device(what, q, out, k_plane, v_plane, k_exp, v_exp, table, of_rows, of_requests)
 
 
-@functools.lru_cache(maxsize=4096)
 def e4m3_splits(rows: int, n_heads: int, n_kv: int, span: int, sms: int) -> int:
     """Blocks that share a row's keys in ``decode_attention_e4m3``."""
-    blocks, steps = _e4m3_blocks(rows, n_heads, n_kv), -(-span // 128)
+    return _e4m3_splits(rows, n_heads, n_kv, -(-span // 128), sms)
+
+
+@functools.lru_cache(maxsize=4096)
+def _e4m3_splits(rows: int, n_heads: int, n_kv: int, steps: int, sms: int) -> int:
+    blocks = _e4m3_blocks(rows, n_heads, n_kv)
 
     # Rounds of three blocks an SM (rows of uneven lengths fill the last one: half of what it leaves), each a start and steps of 128 keys that take
     # a chain of waits alone (1.1 us) and their bytes' time together; and what joins them.  (us, fitted; measured at 1, 2, 4, 12 and 32 blocks a row: 64 rows
