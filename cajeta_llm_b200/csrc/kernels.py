@@ -1799,7 +1799,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
         _need_same_device("rope_kv_write_e4m3", q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
     st = _entry("cache_e4m3", "cj_append_e4m3", "piiiippppppppiiiiiiiiipip")(
         qkv.data_ptr(), qkv.stride(0), q_off, k_off if write_kv else 0, v_off if write_kv else 0, q_out.data_ptr(), _at(k_plane), _at(v_plane),
-        _at(k_exp), _at(v_exp), positions.data_ptr(), _at(row_req), _at(table), table.shape[0] if write_kv else 0, table.stride(0) if write_kv else 0,
+        _at(k_exp), _at(v_exp), positions.data_ptr(), _at(row_req), _at(table), table.shape[0] if write_kv else 0, table.shape[1] if write_kv else 0,
         page_tokens, k_plane.shape[0] if write_kv else 0, T, n_heads, n_kv, head_dim, rotary_dim, _at(inv_freq), 1 if write_kv else 0, _raw())
     _check(st, "rope_kv_write_e4m3")
 
@@ -1882,7 +1882,7 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
         ml = acc.data_ptr() + 4 * T * n_heads * splits * head_dim
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
         q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
-        positions.data_ptr(), row_req.data_ptr(), None, None, table.shape[0], table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv,
+        positions.data_ptr(), row_req.data_ptr(), None, None, table.shape[0], table.data_ptr(), table.shape[1], page_tokens, T, n_heads, n_kv,
         head_dim, window, scale, splits, _at(acc), ml, _raw())
     _check(st, "decode_attention_e4m3")
     if apart:
@@ -1925,13 +1925,13 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
     if splits == 0:
         st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifiiip")(
             q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
-            req_start.data_ptr(), req_prior.data_ptr(), R, T, table.data_ptr(), table.stride(0), page_tokens, n_heads, n_kv, head_dim, window,
+            req_start.data_ptr(), req_prior.data_ptr(), R, T, table.data_ptr(), table.shape[1], page_tokens, n_heads, n_kv, head_dim, window,
             scale, 0, 0, _sm_count(), _raw())
         _check(st, "prefill_attention_e4m3")
         return
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
         q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0], None, None,
-        req_start.data_ptr(), req_prior.data_ptr(), R, table.data_ptr(), table.stride(0), page_tokens, T, n_heads, n_kv, head_dim, window, scale, splits,
+        req_start.data_ptr(), req_prior.data_ptr(), R, table.data_ptr(), table.shape[1], page_tokens, T, n_heads, n_kv, head_dim, window, scale, splits,
         None, None, _raw())
     _check(st, "prefill_attention_e4m3")
 

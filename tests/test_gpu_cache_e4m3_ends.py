@@ -239,3 +239,32 @@ def test_a_value_that_is_no_number_reaches_the_rows_that_see_it_alone(form, prio
     want, size = formula(q, where, k, v, ke, ve, table, P, window, 0.09)
     assert want.isnan().any() and not want[:, 0, 0].isnan()[0]
     agree(attend(form, q, where, k, v, ke, ve, table, P, window, 0.09), want, size)
+
+
+def test_a_table_of_one_row_is_as_wide_as_it_is():
+    """Its stride says nothing: a column turned over, and a row cut out of a wider table."""
+    heads, kv, hd, P, n = 4, 2, 128, 16, 100
+    k, v, ke, ve, table = make([n], kv, hd, P, seed=9)
+    q = queries(3, heads, hd)
+    rows = [(0, n - 3 + i) for i in range(3)]
+    want, size = formula(q, rows, k, v, ke, ve, table, P, 0, 0.1)
+    x = torch.randn((3, (heads + 2 * kv) * hd), device=DEV)
+    row = ints(table[0])
+    wide = torch.cat([ints(table), ints(table)], dim=1)
+    for one in (row[:, None].contiguous().t(), wide[:, :len(table[0])]):
+        assert one.is_contiguous() and one.stride(0) != one.shape[1]
+        out = torch.full_like(q, 7.0)
+        K.decode_attention_e4m3(q, out, k, v, ke, ve, ints([p for _, p in rows]), ints([0] * 3), one, P, heads, kv, hd, 0, 0.1, n)
+        agree(out, want, size)
+        for form in (0, 1):
+            out = torch.full_like(q, 7.0)
+            with pytest.MonkeyPatch.context() as m:
+                m.setattr(K, "e4m3_portions", lambda *a: form)
+                K.prefill_attention_e4m3(q, out, k, v, ke, ve, ints([0, 3]), ints([n - 3]), one, P, heads, kv, hd, 0, 0.1)
+            agree(out, want, size)
+        kk, ee = torch.zeros_like(k), torch.zeros_like(ke)
+        K.rope_kv_write_e4m3(x, 0, heads * hd, (heads + kv) * hd, torch.empty_like(q), kk, torch.zeros_like(v), ee, torch.zeros_like(ve),
+                             ints([p for _, p in rows]), ints([0] * 3), one, P, heads, kv, hd, 0, None, True)
+        for r, p in rows:
+            page, i = at(table, r, p, P)
+            assert (ee[page, :, i] > 0).all()
