@@ -1798,7 +1798,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
     if not plain:
         _need_same_device("rope_kv_write_e4m3", q_out, positions, *((k_plane, v_plane, k_exp, v_exp, row_req, table) if write_kv else ()))
     st = _entry("cache_e4m3", "cj_append_e4m3", "piiiippppppppiiiiiiiiipip")(
-        qkv.data_ptr(), qkv.stride(0), q_off, k_off if write_kv else 0, v_off if write_kv else 0, q_out.data_ptr(), _at(k_plane), _at(v_plane),
+        qkv.data_ptr(), qkv.stride(0) if T > 1 else 0, q_off, k_off if write_kv else 0, v_off if write_kv else 0, q_out.data_ptr(), _at(k_plane), _at(v_plane),
         _at(k_exp), _at(v_exp), positions.data_ptr(), _at(row_req), _at(table), table.shape[0] if write_kv else 0, table.shape[1] if write_kv else 0,
         page_tokens, k_plane.shape[0] if write_kv else 0, T, n_heads, n_kv, head_dim, rotary_dim, _at(inv_freq), 1 if write_kv else 0, _raw())
     _check(st, "rope_kv_write_e4m3")
@@ -2097,18 +2097,19 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
     if a.shape[0] == 0:
         raise KernelError("gemm_q4: a has no rows")
     half = 1 if w.group == 32 else 0
-    if q4_on_tcgen05(M, w.features, w.groups if group_offsets is not None else 0) and a.stride(0) % 8 == 0 and a.data_ptr() % 16 == 0 \
-            and (a_row_index is not None or a.stride(0) >= w.k):
+    lda = a.stride(0) if a.shape[0] > 1 else w.k          # (a single row's stride says nothing)
+    if q4_on_tcgen05(M, w.features, w.groups if group_offsets is not None else 0) and lda % 8 == 0 and a.data_ptr() % 16 == 0 \
+            and (a_row_index is not None or lda >= w.k):
         global launches
-        x, x_rows = a, a.shape[0]
+        x, ldx, x_rows = a, lda, a.shape[0]
         if a_row_index is not None:
             x = torch.empty((M, w.k), dtype=torch.bfloat16, device=a.device)
-            st = _entry("gemm_q4_tc", "cj_q4_gather", "plippiip")(a.data_ptr(), a.stride(0), x_rows, a_row_index.data_ptr(), x.data_ptr(), M, w.k, _raw())
+            st = _entry("gemm_q4_tc", "cj_q4_gather", "plippiip")(a.data_ptr(), lda, x_rows, a_row_index.data_ptr(), x.data_ptr(), M, w.k, _raw())
             _check(st, "gemm_q4")
-            x_rows = M
+            ldx, x_rows = w.k, M
         tok = q4_tile_rows(M, w.features, w.groups if group_offsets is not None else 0, w_up is not None, _sm_count())
         st = _entry("gemm_q4_tc", "cj_gemm_q4_tc", "plippppiliiiiipiiip")(
-            x.data_ptr(), x.stride(0), x_rows, w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
+            x.data_ptr(), ldx, x_rows, w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
             out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), 1 if accumulate else 0, tok, _sm_count(), _raw())
         _check(st, "gemm_q4")
         return
@@ -2118,6 +2119,6 @@ def gemm_q4(a: torch.Tensor, w: Q4Weight, out: torch.Tensor, bias: Optional[torc
     blocks = (min(M, w.groups) if group_offsets is not None else -(-M // 8)) * -(-w.features // 16)
     ahead = 4 if blocks < 4 * _sm_count() else 1
     st = _entry("gemm_q4", "cj_gemm_q4", "plippppiliiiiippiiip")(
-        a.data_ptr(), a.stride(0), a.shape[0], w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
+        a.data_ptr(), lda, a.shape[0], w.data.data_ptr(), None if w_up is None else w_up.data.data_ptr(), _at(bias), out.data_ptr(), _code(out),
         out.stride(0), M, w.features, w.k, w.groups, half, _at(group_offsets), _at(a_row_index), 1 if accumulate else 0, n_tok, ahead, _raw())
     _check(st, "gemm_q4")
