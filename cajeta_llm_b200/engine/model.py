@@ -49,7 +49,8 @@ class Model:
                 what = f"the {name.replace('_', '-')} '{kind}' of '{block.prefix}' with its parameters"
                 if runtime.e4m3_cache and name == "mixer" and part.cache_need() is not None and not part.takes_e4m3_cache:
                     raise ValueError(f"an 8-bit cache is not built into {what}")
-                if runtime.q4_weights and not part.takes_q4_weights:
+                # (products with 4-bit weights do not scale their sums; the block has set this by now)
+                if runtime.q4_weights and not (part.takes_q4_weights and getattr(part, "out_scale", 1.0) == 1.0):
                     raise ValueError(f"4-bit weights are not built into {what}")
 
     def parts(self):

@@ -119,7 +119,7 @@ class PagedAttention(Part):
         self.general = self.general or self.mixed
         # an 8-bit cache and 4-bit weights are built for the plain path (no optional parameter)
         self.takes_q4_weights = not self.general and self.hidden % 8 == 0 and self.q_dim % 8 == 0
-        self.takes_e4m3_cache = not self.general and self.head_dim in (64, 128)
+        self.takes_e4m3_cache = not self.general and self.head_dim in (64, 128) and self.scale > 0.0
         if self.general and (self.qkv_bias or self.out_bias):
             raise ValueError("the general attention path is built without biases")
         if self.mixed and (self.softcap > 0.0 or self.head_gate or self.values_from_keys):
