@@ -243,11 +243,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         // ---- codes: weights are written by no kernel of a step, so that a dense product's leave before the wait for the kernel that makes x
         if (elect_one()) {
             Ring st{0, 0};
-            bool ok = true;
+            bool ok = true, settled = p.offsets != nullptr;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 const Tile t = tile_of(p, tile, feat_tiles, before, edge);
                 const int turn = first_pair(t.f, feat_tiles, n_pairs);
                 for (int pair = 0; pair < n_pairs; ++pair, st.move(1, CODE_STAGES)) {
+                    if (!settled && st.phase) cj::after_predecessor(), settled = true;      // (from the second round on, places wait for products)
                     const int kb = 2 * turned(pair, turn, n_pairs), blocks = min(2, n_kb - kb);
                     uint8_t* dst = code_ring + st.at * 2 * TILE;
                     uint64_t* bar = &code_full[st.at];
@@ -267,7 +268,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
             }
         }
     } else if (warp == PRODUCT) {
-        // ---- products
+        // ---- products (no wait with a limit begins before the kernel that makes x is done: how long that takes is not this kernel's to say)
+        if (!p.offsets) cj::after_predecessor();
         if (elect_one()) {
             // One thread's instructions come one after the other, four clocks and more each, beside those of the warps that share its scheduler: waits, commits and
             // sums are for two blocks of K at a time, and the loop keeps addresses and descriptors instead of working them out of a place in a ring.
@@ -319,7 +321,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
         const uint8_t* mine = code_ring + (GATED ? upper * 4 + q : q * 2 + upper) * PIECE;
         Ring st{set, 0}, sl{0, 0};
         sl.move(set, p.stages);
+        bool settled = p.offsets != nullptr;
         for (int left = my_tiles * n_pairs - set; left > 0; left -= CONV_SETS, st.move(CONV_SETS, CODE_STAGES), sl.move(CONV_SETS, p.stages)) {
+            if (!settled && sl.phase) cj::after_predecessor(), settled = true;
             if (!mbar_wait_warp(&code_full[st.at], st.phase, 5)) break;
             // (where a pair has one block, what lies there is put down for the other and nobody reads it)
             const uint8_t* src = mine + st.at * 2 * TILE;
