@@ -54,14 +54,6 @@ struct QueryTile {
     int rows, p0, begin, end;      // rows of the step (0: empty), position of the first, key tiles [begin, end] of the block's
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ uint32_t of_block(const void* p, int rank) {      // what lies at p, in the cluster's block `rank`
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
@@ -304,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (run[j] > 0)
-                        bulk_load(smem + S::CODES + (values * BN + j * 32 + lane) * HD, (values ? p.vplane : p.kplane) + (size_t)row[j] * HD,
+                        bulk_load(smem_u32(smem + S::CODES + (values * BN + j * 32 + lane) * HD), (values ? p.vplane : p.kplane) + (size_t)row[j] * HD,
                                   run[j] * HD, &c_full[values]);
             }
         }
@@ -574,11 +566,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_e4m3_tc_kernel(const __gri
 }  // namespace
 
 // q, out: bf16 [total_rows, n_heads, hd]; the cache as cj_append_e4m3 writes it; rows req_start[r] .. req_start[r + 1] are request r's
-// from position req_prior[r] on.  hd: 64 or 128; scale > 0.  block_rows: query rows a block, 128 or 256; splits: blocks that share
-// their keys, 1, 2 or 4 (0: by the size of the launch).
+// from position req_prior[r] on.  hd: 64 or 128; scale > 0.
 CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, const void* vplane, const void* kexp, const void* vexp, int n_pages,
                                  const int* req_start, const int* req_prior, int n_requests, int total_rows, const int* table, int table_stride,
-                                 int page_tokens, int n_heads, int n_kv, int hd, int window, float scale, int block_rows, int splits, int sms,
+                                 int page_tokens, int n_heads, int n_kv, int hd, int window, float scale, int sms,
                                  cudaStream_t stream) {
     if (total_rows <= 0 || n_requests <= 0) return 0;
     if (!q || !out || !kplane || !vplane || !kexp || !vexp || !req_start || !req_prior || !table) return CJ_ERR_ARG;
@@ -590,8 +581,7 @@ CJ_EXPORT int cj_prefill_e4m3_tc(const void* q, void* out, const void* kplane, c
     // (us, 256 rows alone, in four, 128 alone, in four: 64 rows behind 2,000, 16 heads, 52, 24, 52, 24; 200 behind 300, heads of 64, 18, 18, 15, 16; 256 behind
     // 1,024, 28 heads, 40, 23, 35, 38: more blocks than SMs)
     const long long blocks = ((long long)(total_rows + 255) / 256 + n_requests - 1) * n_heads;
-    if (splits != 1 && splits != 2 && splits != 4) splits = 4 * blocks <= sms ? 4 : 2 * blocks <= sms ? 2 : 1;
-    if (block_rows != 128 && block_rows != 256) block_rows = 2 * splits * blocks <= sms ? 128 : 256;
+    const int splits = 4 * blocks <= sms ? 4 : 2 * blocks <= sms ? 2 : 1, block_rows = 2 * splits * blocks <= sms ? 128 : 256;
     const long long row_blocks = ((long long)total_rows + block_rows - 1) / block_rows + n_requests;
     if (row_blocks > 65535) return CJ_ERR_SIZE;
     CUtensorMap map_q;

@@ -14,6 +14,9 @@
 #include "tc_common.cuh"
 
 using namespace cj;
+using tc::bulk_load;
+using tc::cluster_sync;
+using tc::ex2;
 using tc::mbar_expect_tx;
 using tc::mbar_init;
 using tc::mbar_wait_warp;
@@ -140,11 +143,6 @@ constexpr int WARPS = 4;
 constexpr int STEP = 32;                   // keys of a warp's step
 constexpr int STAGES = 2, BLOCKS = 3;      // steps of a warp's ring, blocks an SM
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)) : "memory");
-}
-
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -163,9 +161,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // A row's blocks, up to eight, can be a cluster and add their results through each other's shared memory; otherwise they leave them to a kernel of its own.
 constexpr int MOST_CLUSTER = 8;
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float2 ld_of_block(const float* p, int rank) {      // what lies at p in the shared memory of the cluster's block `rank`
     uint32_t a;
     float2 v;

@@ -29,13 +29,6 @@ __device__ __forceinline__ int query_exponent(float most) {
 __device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// 2^x, 0 for -inf (relative error 2^-22)
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // four codes as two pairs of f16 (every e4m3 number is an f16 number)
 __device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
     asm("{\n\t.reg .b16 a, b;\n\t"

@@ -80,11 +80,6 @@ __device__ __forceinline__ Tile tile_of(const Args& p, int tile, int feat_tiles,
     return t;
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
-
 // 16 lanes x 32 columns: lane (g, t) gives, for the eight columns of step j, columns 2 t, 2 t + 1 of row g and then of row g + 8
 __device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -259,11 +254,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_q4_tc_kernel(const __grid_con
                         // of each block the gate's four pieces and the other weight's
                         const size_t at = (((size_t)t.group * tiles_f + (t.f >> 1)) * n_kb + kb) * TILE + (t.f & 1) * 4 * PIECE;
                         for (int b = 0; b < blocks; ++b) {
-                            bulk_load(dst + b * TILE, p.w + at + b * TILE, 4 * PIECE, bar);
-                            bulk_load(dst + b * TILE + 4 * PIECE, p.w_up + at + b * TILE, 4 * PIECE, bar);
+                            bulk_load(smem_u32(dst + b * TILE), p.w + at + b * TILE, 4 * PIECE, bar);
+                            bulk_load(smem_u32(dst + b * TILE + 4 * PIECE), p.w_up + at + b * TILE, 4 * PIECE, bar);
                         }
                     } else
-                        bulk_load(dst, p.w + (((size_t)t.group * tiles_f + t.f) * n_kb + kb) * TILE, blocks * TILE, bar);
+                        bulk_load(smem_u32(dst), p.w + (((size_t)t.group * tiles_f + t.f) * n_kb + kb) * TILE, blocks * TILE, bar);
                 }
             }
         }

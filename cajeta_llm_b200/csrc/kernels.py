@@ -1923,10 +1923,10 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
         return
     splits = e4m3_portions(T, R, n_heads, n_kv, table.shape[1] * page_tokens, _sm_count())
     if splits == 0:
-        st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifiiip")(
+        st = _entry("attention_e4m3_tc", "cj_prefill_e4m3_tc", "ppppppippiipiiiiiifip")(
             q.data_ptr(), out.data_ptr(), k_plane.data_ptr(), v_plane.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k_plane.shape[0],
             req_start.data_ptr(), req_prior.data_ptr(), R, T, table.data_ptr(), table.shape[1], page_tokens, n_heads, n_kv, head_dim, window,
-            scale, 0, 0, _sm_count(), _raw())
+            scale, _sm_count(), _raw())
         _check(st, "prefill_attention_e4m3")
         return
     st = _entry("cache_e4m3", "cj_decode_e4m3", "ppppppippppipiiiiiiifippp")(
@@ -1947,7 +1947,7 @@ class Q4Weight:
 
     MOST_SCALE = 2.0 ** 123        # scales lie below it: the products' 24 scales and more stay finite numbers
 
-    def __init__(self, data: torch.Tensor, shape, group: int, features: int = 0, groups: int = 0):
+    def __init__(self, data: torch.Tensor, shape, group: int):
         self.data = data                       # uint8, the layout
         self.shape = tuple(shape)
         self.group = group                     # 32 or 64
