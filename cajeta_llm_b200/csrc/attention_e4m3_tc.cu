@@ -9,7 +9,7 @@
 // turn codes into the bfloat16 tiles in shared memory that both products read, and the rest is attention over a bfloat16 cache: P, as there, is
 // the one rounding.  The codes come by bulk copies of a page's run of rows, pages of any size, one warp's work: a tile's keys travel while its
 // predecessor's values are converted (half the bytes of a bfloat16 cache: 16 KB a tile; plain loads into registers, tried first, held the
-// conversions of the tile before up: 2,048 rows behind 4,096, 28 heads over 4 of 128: 290 us where this takes 238).  The two query tiles take turns between the exponential unit and the tensor
+// conversions of the tile before up: 2,048 rows behind 4,096, 28 heads over 4 of 128: 290 us where this takes 240).  The two query tiles take turns between the exponential unit and the tensor
 // core, each key tile is worked on as two halves of 64 keys, and the reference maximum moves only when it grows by more than 2^8.
 // Where row blocks are few, two or four blocks - a cluster - take neighbouring stretches of the key tiles and join their outputs through each other's
 // shared memory (512 rows behind 4,096, 16 heads: 109 us alone, 66 in two, 42 in four; 100 behind 8,000, 28 heads: 165, 94, 54).

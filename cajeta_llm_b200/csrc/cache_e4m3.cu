@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 // own, filled by bulk copies of a page's run of rows a step ahead (registers that loads are on their way to would make every shuffle and
 // exponential wait for them).  An e4m3 code is an f16 number exactly: the products are mma.sync m16n8k16 of f16 numbers, float32 out, with the codes
 // as their first operand, so that all 16 rows of a product are keys (or entries) and its columns the heads.  (mma.sync takes e4m3 operands
-// too; with them 64 rows of up to 2,048 keys took 80 us where this takes 61.)
+// too; with them 64 rows of up to 2,048 keys, 16 heads over 16, took 80 us where this took 61.)
 //     S^T = code_k . q^T                              s = S scale 2^e_k
 //     O^T = code_v^T . (p 2^(m + e_v - N))^T          m: a head's largest score so far, N: its reference of what keys bring, both in octaves
 // The order of a product's K, and of its rows, is free as long as both sides keep it: a lane's share of a key is HD / 4 neighbouring bytes and
@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(256) append_e4m3_kernel(
 // N is an integer, 12 below the largest s + e_v when it was last moved; it moves when a key may bring more than 2^15 of it.  So the factors are at most
 // 2^15 in f16 and keep its 11 bits down to 2^-26 of the largest contribution, some down to 2^-36, whatever weight and value make it up, and the rest is what
 // float32 weights lose too (those below 2^-126).  A reference of the values' exponents alone, one for a warp, was 2 to 4 % faster (64 rows of up to 2,048 keys
-// 61 us, 62 so; eight of up to 32,768 49 and 51) and lost all others to a large value that the row hardly looks at.  The divisor's weights are not rounded.
-// Bound by DRAM: 2 (HD + 1) bytes a key (64 rows of up to 2,048 keys, 28 heads over 4: 61 us, 73 % of a copy's rate; 32 rows of 4,096: 101 us, 81 %).
+// 60.7 us, 61.6 so; eight of up to 32,768 48 and 50) and lost all others to a large value that the row hardly looks at.  The divisor's weights are not rounded.
+// Bound by DRAM, 2 (HD + 1) bytes a key and kv head, where heads have keys of their own (16 over 16: 64 rows of up to 2,048 keys 61.6 us, 72 % of a copy's rate;
+// 32 rows of 4,096 107, 76 %); by a step's chain where few blocks hold the keys of many heads (28 over 4: 64 rows of up to 2,048 35 us, 34 %).
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int WARPS = 4;
 constexpr int STEP = 32;                   // keys of a warp's step

@@ -17,7 +17,8 @@
 // clocks each, a pair of blocks is 230 clocks of the integer pipe a scheduler, and the one thread that issues eight products, a wait and an arrival
 // a pair does so between the others' instructions: 670 clocks a pair in all (64 rows x 6,144 x 6,144: 20 us; with waits, arrivals and ring
 // sums for each block of 64, three instructions more a word of codes, and codes freed only after the product, 31 us).  Beyond, the tensor core
-// (832 clocks a pair at 208 rows) and, with one accumulator, the time to drain it: 2,048 rows x 3,584 x 3,584 take 46 us, 1.14 PFLOP/s.
+// (832 clocks a pair at 208 rows) and, with one accumulator, the time to drain it: 2,048 rows x 3,584 x 3,584 take 46 us, 1.14 PFLOP/s, in a
+// burst and 55, 0.96, call after call (the power cap's clock).
 #define CJ_LIB "gemm_q4_tc"
 #include "common.cuh"
 #include "q4.cuh"
@@ -49,7 +50,7 @@ struct Args {
     int x_bytes;               // of a block of 64 of K; a stage has two
     // A float32 result's K goes in parts of so many pairs of blocks of 64, each summed from zero and added to what the parts before left: tcgen05 cuts its sums off
     // rather than rounding them, and an error that grows with their length stays that of 2,560 entries (2,048 x 3,584 x 3,584: 1.2e-6 of the result
-    // in one part, 7e-7 in two).
+    // in one part, 5e-7 in two).
     int part_pairs;
 };
 

@@ -1768,7 +1768,8 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, q_
                        rotary_dim: int, inv_freq: Optional[torch.Tensor], write_kv: bool) -> None:
     """``rope_kv_write`` into the 8-bit cache: every (token, kv head) of keys and of values becomes ``head_dim`` e4m3 codes and one
     exponent e (``k_exp`` and ``v_exp``, uint8 [pages, n_kv, page_tokens], hold e + 127), the smallest with max|x| <= 448 2^e;
-    an entry is its code times 2^e.  Zeros, and what lies below 448 2^-100, take e = -100; what lies beyond 448 2^119 is cut to it.
+    an entry is its code times 2^e.  Zeros, and what lies below 448 2^-100, take e = -100; what lies beyond 448 2^119 is cut to it; NaN stays NaN.
+    No two rows of a call are of one request and one position (their codes and exponents would mix).
     A row whose request (none of ``table``'s) or page (-1) is not there is rotated and not written.  q_out: bfloat16 [T, heads, head_dim];
     head_dim 64 or 128."""
     plain = write_kv and _plain((k_plane, v_plane, k_exp, v_exp, q_out, positions, row_req, table), _APPEND_TYPES)
@@ -1836,8 +1837,9 @@ def _e4m3_splits(rows: int, n_heads: int, n_kv: int, steps: int, sms: int) -> in
 
     # Rounds of three blocks an SM (rows of uneven lengths fill the last one: half of what it leaves), each a start and steps of 128 keys that take
     # a chain of waits alone (1.1 us) and their bytes' time together; and what joins them.  (us, fitted; measured at 1, 2, 4, 12 and 32 blocks a row: 64 rows
-    # of up to 2,048 keys, 28 heads over 4, 60, 64, -, 115, 224; 32 rows of 4,096, 16 heads, 119, 108, 104, 114, 166; eight of up to 32,768, 4 kv heads,
-    # 296, 151, 81, 50, 55; one of 32,768 272, 143, 76, 34, 19; eight of 576, 16 heads, 9, 10, 12, 16, 29)
+    # of up to 2,048 keys, 16 heads over 16, 62, 65, 74, 119, 226; 32 rows of 4,096, the same heads, 121, 108, 101, 117, 167; eight of up to 32,768, 28 heads
+    # over 4, 303, 155, 82, 52, 56; one of 32,768 288, 154, 80, 36, 20; eight of 576, 16 heads over 16, 9, 10, 12, 16, 29; 64 of up to 2,048, 28 over 4,
+    # 38, 31, 32, 49, 89)
     def cost(n):
         rounds = blocks * n / (3 * sms)
         rounds = 1 if rounds <= 1 else (rounds + math.ceil(rounds)) / 2
@@ -1854,7 +1856,7 @@ def _e4m3_blocks(rows: int, n_heads: int, n_kv: int) -> int:
 
 def _e4m3_cluster(blocks: int, n: int, sms: int) -> bool:
     """Whether a row's n blocks are a cluster and join their results themselves: few blocks, which wait for nobody's place.  (us, a cluster and a merge
-    kernel: one row of 576 keys in five blocks 4.9 and 7.0; eight rows of up to 32,768 in eight 62 and 56; 64 rows of up to 2,048 in two 69 and 64)"""
+    kernel: one row of 576 keys in five blocks 5.0 and 7.4; eight rows of up to 32,768 in eight 65 and 59; 64 rows of up to 2,048 in two 70 and 65)"""
     return 1 < n <= 8 and blocks * n <= sms
 
 
@@ -1863,7 +1865,7 @@ def decode_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Ten
                           n_heads: int, n_kv: int, head_dim: int, window: int, scale: float, max_context: int, splits: int = 0) -> None:
     """Attention of bfloat16 query rows [T, heads, head_dim], each over its request's keys in the 8-bit cache that
     ``rope_kv_write_e4m3`` writes: row t sees the positions from ``positions[t] + 1 - window`` (0 without a window) to
-    ``positions[t]``.  A row of none of ``table``'s requests (-1) sees none: zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
+    ``positions[t]`` whose page the table names (one of the pool's).  A row of none of ``table``'s requests (-1), or without such keys, gets zeros.  ``max_context``: positions + 1 at most.  ``splits``: blocks
     that share a row's keys (0: by the size of the launch; the results' last bits depend on it).  head_dim 64 or 128."""
     _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, positions, row_req, ("positions", "row_req"), page_tokens, n_heads, n_kv,
                          head_dim, window, scale, "decode_attention_e4m3")
@@ -1899,8 +1901,8 @@ def e4m3_portions(rows: int, requests: int, n_heads: int, n_kv: int, span: int, 
     table has room for."""
     blocks = _e4m3_blocks(rows, n_heads, n_kv)
     # Few rows are one by one, their keys shared out as far as SMs go round; where these are taken and the requests so few that their tiles' keys can be
-    # shared out instead, tiles.  (us, row by row without sharing and tiles: one portion of 16 rows, 16 heads, behind 100 tokens 6 and 9, 1,000 19 and 14,
-    # 8,000 120 and 48; two rows, 28 heads over 4, behind 8,000 78, shared out 15, and 45; 36 rows of six requests behind 500 to 3,000, 28 heads over 4, 33 and 80)
+    # shared out instead, tiles.  (us, row by row without sharing and tiles: one portion of 16 rows, 16 heads, behind 100 tokens 6 and 9, 1,000 20 and 14,
+    # 8,000 121 and 48; two rows, 28 heads over 4, behind 8,000 77, shared out 16, and 44; 29 rows of six requests behind 500 to 3,000, 28 heads over 4, 34 and 84)
     if rows > (2 * E4M3_ROW_BY_ROW if rows <= 8 * requests else E4M3_ROW_BY_ROW) or (2 * blocks > sms and 2 * requests * n_heads <= sms):
         return 0
     return max(1, min(8, sms // blocks, -(-span // 128)))
@@ -1911,8 +1913,8 @@ def prefill_attention_e4m3(q: torch.Tensor, out: torch.Tensor, k_plane: torch.Te
                            n_heads: int, n_kv: int, head_dim: int, window: int, scale: float) -> None:
     """Attention of portions of prompts over the 8-bit cache (which holds the portions' own keys and values already): rows
     ``req_start[r]`` to ``req_start[r + 1]`` of q [T, heads, head_dim] (bfloat16) are request r's tokens from position
-    ``req_prior[r]`` on, each sees its request's keys up to its own position, under a window the last ``window`` of them.  Rows of no
-    request are left as they were.  head_dim 64 or 128."""
+    ``req_prior[r]`` on, each sees the keys of the positions up to its own, under a window the last ``window`` of them, whose page the table names
+    (zeros where there is none).  Rows of no request are left as they were.  head_dim 64 or 128."""
     _need_e4m3_attention(q, out, k_plane, v_plane, k_exp, v_exp, table, req_start, req_prior, ("req_start", "req_prior"), page_tokens, n_heads,
                          n_kv, head_dim, window, scale, "prefill_attention_e4m3")
     R = req_prior.numel()
